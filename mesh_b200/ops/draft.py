@@ -1,0 +1,106 @@
+"""Attention of drafted tokens over a key/value cache, and the trees between them.
+
+A step hands the model T drafted tokens per sequence instead of one: the last accepted token (node 0, the root) and guesses
+that continue it, each with a parent among the nodes before it.  Node t lies in slot ``pos + t`` of the cache; it sees what was
+accepted (slots before ``pos``), itself and its ancestors.  With one token per sequence this is ordinary decoding, over caches
+of 8 bits too.
+
+Reference semantics: blockwise attention with (m, s, acc) merging and grouped query heads
+(compiler/mesh_compiler/operations.py:7072-7166).
+"""
+from __future__ import annotations
+
+import ctypes
+from ctypes import c_float, c_int, c_longlong, c_void_p
+
+import torch
+
+from .. import _native
+from .cache import KVCache, _ints, _launch
+
+MAX_DRAFTS = 64
+
+
+class _Draft(ctypes.Structure):
+    """``MeshDraftAttention`` (csrc/ops/draft_api.h)."""
+    _fields_ = [("q", c_void_p), ("out", c_void_p), ("q_sb", c_longlong), ("q_st", c_longlong), ("o_sb", c_longlong), ("o_st", c_longlong),
+                ("pos", c_void_p), ("counts", c_void_p), ("visible", c_void_p),
+                ("T", c_int), ("q_heads", c_int), ("window", c_int), ("splits", c_int), ("scale", c_float), ("scratch", c_void_p)]
+
+
+def tree_visible(parents) -> torch.Tensor:
+    """``parents [B, T]`` (a list or an integer tensor; ``parents[b][t] < t``, negative: no parent) -> int64 ``[B, T]`` on the host: bit j
+    of a node's word is set for itself and its ancestors.  A tree that does not change is turned into words once."""
+    rows = parents.tolist() if isinstance(parents, torch.Tensor) else parents
+    words = []
+    for row in rows:
+        if len(row) > MAX_DRAFTS:
+            raise ValueError(f"tree_visible: at most {MAX_DRAFTS} drafts, got {len(row)}")
+        seen: list[int] = []
+        for t, p in enumerate(row):
+            if p >= t:
+                raise ValueError(f"tree_visible: node {t} has parent {p}; a parent comes before its children")
+            seen.append((seen[p] if p >= 0 else 0) | 1 << t)
+        words.append([w - (1 << 64) if w >> 63 else w for w in seen])
+    return torch.tensor(words, dtype=torch.int64).reshape(len(rows), len(words[0]) if words else 0)
+
+
+def tree_depth(visible: torch.Tensor) -> torch.Tensor:
+    """Depth of every node (the root: 0) from its word, int32: its position is ``pos`` plus this."""
+    bits = torch.arange(64, device=visible.device)
+    return (((visible[..., None] >> bits) & 1).sum(-1).clamp(min=1) - 1).to(torch.int32)
+
+
+def draft_attention(q: torch.Tensor, cache: KVCache, pos: torch.Tensor, *, counts: torch.Tensor | None = None,
+                    visible: torch.Tensor | None = None, window: int = 0, scale: float | None = None,
+                    out: torch.Tensor | None = None, splits: int = 0) -> torch.Tensor:
+    """``q [B, T, q_heads, head_dim]`` bf16 (heads dense, T <= 64) against ``cache`` -> ``out`` of the same shape.
+
+    ``pos [B]`` int32: slots before it are seen by every node (with ``window``: those less than ``window`` positions back; a
+    node's position is ``pos`` plus the bits set in its word, less one); node t lies in slot ``pos[b] + t``, where
+    :meth:`KVCache.append` has put it.  ``visible [B, T]`` int64: bit j says that the node sees node j (``None``: the ones before it and itself);
+    ``counts [B]`` int32: nodes of each sequence (``None``: T); later ones are neither computed nor written.  A node that
+    sees nothing gets zeros.  A ``window`` must not be shorter than T.  ``splits``: CTAs that share the keys of a sequence and KV
+    head (0: chosen from the sizes).
+
+    Sums of the softmax are fp32; its weights are rounded to fp16 (8-bit rows) or bf16 (bf16 rows) before the second product."""
+    B, H, S, hd = cache.k.shape
+    if q.dim() != 4 or q.shape[0] != B or q.shape[3] != hd or q.dtype != torch.bfloat16 or q.device != cache.device:
+        raise ValueError(f"draft_attention: q must be bf16 [{B}, T, q_heads, {hd}] on {cache.device}, got {q.dtype} {list(q.shape)} on {q.device}")
+    T, qh = q.shape[1], q.shape[2]
+    if T > MAX_DRAFTS:
+        raise ValueError(f"draft_attention: at most {MAX_DRAFTS} drafts per sequence, got {T}")
+    if qh % H or qh == 0:
+        raise ValueError(f"draft_attention: {qh} query heads are not a multiple of {H} KV heads")
+    if out is None:
+        # nodes behind counts are not written: zeros there rather than what the memory held
+        out = (torch.empty if counts is None else torch.zeros)((B, T, qh, hd), dtype=torch.bfloat16, device=q.device)
+    elif out.shape != q.shape or out.dtype != torch.bfloat16 or out.device != q.device:
+        raise ValueError("draft_attention: out must be like q")
+    for x, name in ((q, "q"), (out, "out")):
+        if x.stride(3) != 1 or x.stride(2) != hd:
+            raise ValueError(f"draft_attention: heads of {name} must be dense")
+    if visible is not None and (visible.dtype != torch.int64 or visible.shape != (B, T) or visible.device != q.device or not visible.is_contiguous()):
+        raise ValueError(f"draft_attention: visible must be a contiguous int64 [{B}, {T}] on {q.device}")
+    p, n = _ints(pos, "draft_attention: pos", q.device, B), _ints(counts, "draft_attention: counts", q.device, B)
+    a = _Draft(q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), out.stride(0), out.stride(1), p, n,
+               0 if visible is None else visible.data_ptr(), T, qh, window, splits, hd ** -0.5 if scale is None else scale, 0)
+    key = (T, qh, window, splits)
+    floats = cache._scratch.get(key)
+    if floats is None:                           # a function of the sizes alone; also checks the arguments
+        fn = _native.lib().mesh_draft_attention_scratch
+        fn.restype = c_longlong
+        floats = int(fn(ctypes.byref(cache._c), ctypes.byref(a)))
+        if floats < 0:
+            raise ValueError(_native.last_error())
+        cache._scratch[key] = floats
+    if B == 0 or T == 0:
+        return out
+    if q.device.type != "cuda":
+        raise ValueError(f"draft_attention: the tensors are on {q.device}; the kernel needs a GPU")
+    # scratch of the call's own: calls on other streams and other captured graphs share nothing
+    scratch = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
+    a.scratch = scratch.data_ptr() if scratch is not None else 0
+    _launch(q.device, "mesh_draft_attention", ctypes.byref(cache._c), ctypes.byref(a))
+    _native.count_launch(2 if floats else 1)
+    return out
