@@ -9,7 +9,7 @@ Reference: the E2B decode analysis's KV cache (design/e2b-crossover-2026-09-16.m
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_int, c_longlong, c_void_p
+from ctypes import c_char_p, c_int, c_longlong, c_void_p
 
 import torch
 
@@ -22,24 +22,50 @@ class _Cache(ctypes.Structure):
                 ("B", c_int), ("kv_heads", c_int), ("max_seq", c_int), ("head_dim", c_int), ("bits", c_int)]
 
 
-def _launch(device: torch.device, name: str, *args) -> None:
-    """Calls ``name(*args, stream)`` with ``device`` current, on its current stream."""
-    if device.type != "cuda":
-        raise ValueError(f"{name}: the tensors are on {device}; the kernels need a GPU")
-    fn = getattr(_native.lib(), name)
-    if device.index == torch._C._cuda_getDevice():
-        rc = fn(*args, c_void_p(_native.stream()))
+_I32 = torch.int32
+_bound = None
+
+
+def _lib() -> ctypes.CDLL:
+    """The library with the signatures of this family's calls set: with them, addresses and numbers go through as they are, which
+    is half of a call's host time."""
+    global _bound
+    if _bound is None:
+        L = _native.lib()
+        P, I, Q = c_void_p, c_int, c_longlong
+        for name, types in (("mesh_kv_append", [P, P, P, Q, Q, Q, Q, Q, Q, P, P, I, P]), ("mesh_kv_read", [P, P, P, P, P, I, P]),
+                            ("mesh_kv_keep", [P, I, P, P, P, I, P]), ("mesh_draft_attention", [P, c_char_p, P]),
+                            ("mesh_constrain_logits", [c_char_p, P])):
+            getattr(L, name).argtypes = types
+        L.mesh_draft_attention_scratch.argtypes, L.mesh_draft_attention_scratch.restype = [P, c_char_p], Q
+        _bound = L
+    return _bound
+
+
+def _launch(index: int, name: str, launches: int, *args) -> None:
+    """Calls ``name(*args, stream)`` on the current stream of device ``index`` (-1: not a GPU)."""
+    if index < 0:
+        raise ValueError(f"{name}: the tensors are on the host; the kernels need a GPU")
+    fn = getattr(_lib(), name)
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(device):
-            rc = fn(*args, c_void_p(_native.stream()))
-    _native.check(rc, name)
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _native.check(rc, name)
+    _native.count_launch(launches)
 
 
-def _ints(t: torch.Tensor | None, name: str, device: torch.device, *shape) -> int:
+def _index(device: torch.device) -> int:
+    return device.index if device.type == "cuda" else -1
+
+
+def _ints(t: torch.Tensor | None, name: str, device: torch.device, shape: tuple) -> int:
     """Address of an int32 tensor of this shape (0 for ``None``)."""
     if t is None:
         return 0
-    if t.dtype != torch.int32 or t.device != device or tuple(t.shape) != shape or not t.is_contiguous():
+    if t.dtype is not _I32 or t.shape != shape or t.device != device or not t.is_contiguous():
         raise ValueError(f"{name}: need a contiguous int32 tensor of shape {list(shape)} on {device}, got {t.dtype} {list(t.shape)} on {t.device}")
     return t.data_ptr()
 
@@ -71,6 +97,7 @@ class KVCache:
         B, H, S, hd = k.shape
         self._c = _Cache(k.data_ptr(), v.data_ptr(), 0 if k_scale is None else k_scale.data_ptr(),
                          0 if v_scale is None else v_scale.data_ptr(), B, H, S, hd, self.bits)
+        self._at, self._index = ctypes.addressof(self._c), _index(k.device)
         self._scratch: dict = {}                 # floats of scratch by the sizes of a call (ops/draft.py)
 
     @classmethod
@@ -90,17 +117,15 @@ class KVCache:
         B, H, S, hd = self.k.shape
         T = k.shape[1] if k.dim() == 4 else -1
         for x in (k, v):
-            if tuple(x.shape) != (B, T, H, hd) or x.dtype != torch.bfloat16 or x.device != self.device:
+            if x.shape != (B, T, H, hd) or x.dtype is not torch.bfloat16 or x.device != self.device:
                 raise ValueError(f"append: rows must be bf16 [{B}, T, {H}, {hd}] on {self.device}, got {x.dtype} {list(x.shape)} on {x.device}")
-            if x.stride(3) != 1:
-                raise ValueError("append: the last dimension must be dense")
-        p, n = _ints(pos, "append: pos", self.device, B), _ints(counts, "append: counts", self.device, B)
+        ks, vs = k.stride(), v.stride()
+        if ks[3] != 1 or vs[3] != 1:
+            raise ValueError("append: the last dimension must be dense")
+        p, n = _ints(pos, "append: pos", self.device, (B,)), _ints(counts, "append: counts", self.device, (B,))
         if B == 0 or T == 0:
             return
-        _launch(self.device, "mesh_kv_append", ctypes.byref(self._c), c_void_p(k.data_ptr()), c_void_p(v.data_ptr()),
-                c_longlong(k.stride(0)), c_longlong(k.stride(1)), c_longlong(k.stride(2)),
-                c_longlong(v.stride(0)), c_longlong(v.stride(1)), c_longlong(v.stride(2)), c_void_p(p), c_void_p(n), c_int(T))
-        _native.count_launch()
+        _launch(self._index, "mesh_kv_append", 1, self._at, k.data_ptr(), v.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], p, n, T)
 
     def read(self, start: torch.Tensor, T: int, counts: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
         """Rows ``start[b] .. start[b] + T`` as dense bf16 ``[B, T, kv_heads, head_dim]`` keys and values (what
@@ -108,12 +133,11 @@ class KVCache:
         B, H, S, hd = self.k.shape
         if T < 0:
             raise ValueError("read: T must not be negative")
-        p, n = _ints(start, "read: start", self.device, B), _ints(counts, "read: counts", self.device, B)
-        k, v = (torch.empty((B, T, H, hd), dtype=torch.bfloat16, device=self.device) for _ in range(2))
+        p, n = _ints(start, "read: start", self.device, (B,)), _ints(counts, "read: counts", self.device, (B,))
+        k = torch.empty((B, T, H, hd), dtype=torch.bfloat16, device=self.device)
+        v = torch.empty_like(k)
         if B and T:
-            _launch(self.device, "mesh_kv_read", ctypes.byref(self._c), c_void_p(k.data_ptr()), c_void_p(v.data_ptr()), c_void_p(p), c_void_p(n),
-                    c_int(T))
-            _native.count_launch()
+            _launch(self._index, "mesh_kv_read", 1, self._at, k.data_ptr(), v.data_ptr(), p, n, T)
         return k, v
 
     def dequantize(self) -> tuple[torch.Tensor, torch.Tensor]:
@@ -135,6 +159,7 @@ class CacheGroup:
                 raise ValueError("CacheGroup: the caches must have one shape, type and device")
         self.caches, self.device = list(caches), c0.device
         self._arr = (_Cache * len(caches))(*[c._c for c in caches])
+        self._at, self._index = ctypes.addressof(self._arr), c0._index
 
     def keep(self, pos: torch.Tensor, path: torch.Tensor, counts: torch.Tensor | None = None) -> None:
         """In every cache, slot ``pos[b] + i`` gets what slot ``pos[b] + path[b, i]`` held before the call, for ``i <
@@ -144,9 +169,9 @@ class CacheGroup:
         N = path.shape[1] if path.dim() == 2 else -1
         if N > 64:
             raise ValueError(f"keep: at most 64 rows per sequence, got {N}")
-        q = _ints(path, "keep: path", self.device, B, N)
-        p, n = _ints(pos, "keep: pos", self.device, B), _ints(counts, "keep: counts", self.device, B)
+        q = _ints(path, "keep: path", self.device, (B, N))
+        p, n = _ints(pos, "keep: pos", self.device, (B,)), _ints(counts, "keep: counts", self.device, (B,))
         if B == 0 or N == 0:
             return
-        _launch(self.device, "mesh_kv_keep", self._arr, c_int(len(self.caches)), c_void_p(p), c_void_p(q), c_void_p(n), c_int(N))
-        _native.count_launch(-(-len(self.caches) // 64))
+        L = len(self.caches)
+        _launch(self._index, "mesh_kv_keep", -(-L // 64), self._at, L, p, q, n, N)

@@ -10,22 +10,16 @@ Reference semantics: blockwise attention with (m, s, acc) merging and grouped qu
 """
 from __future__ import annotations
 
-import ctypes
-from ctypes import c_float, c_int, c_longlong, c_void_p
+import struct
 
 import torch
 
 from .. import _native
-from .cache import KVCache, _ints, _launch
+from .cache import KVCache, _ints, _launch, _lib
 
 MAX_DRAFTS = 64
-
-
-class _Draft(ctypes.Structure):
-    """``MeshDraftAttention`` (csrc/ops/draft_api.h)."""
-    _fields_ = [("q", c_void_p), ("out", c_void_p), ("q_sb", c_longlong), ("q_st", c_longlong), ("o_sb", c_longlong), ("o_st", c_longlong),
-                ("pos", c_void_p), ("counts", c_void_p), ("visible", c_void_p),
-                ("T", c_int), ("q_heads", c_int), ("window", c_int), ("splits", c_int), ("scale", c_float), ("scratch", c_void_p)]
+# ``MeshDraftAttention`` (csrc/ops/draft_api.h): q, out, their strides, pos, counts, visible, T, q_heads, window, splits, scale, scratch
+_ARGS = struct.Struct("@PPqqqqPPPiiiifP")
 
 
 def tree_visible(parents) -> torch.Tensor:
@@ -65,42 +59,43 @@ def draft_attention(q: torch.Tensor, cache: KVCache, pos: torch.Tensor, *, count
 
     Sums of the softmax are fp32; its weights are rounded to fp16 (8-bit rows) or bf16 (bf16 rows) before the second product."""
     B, H, S, hd = cache.k.shape
-    if q.dim() != 4 or q.shape[0] != B or q.shape[3] != hd or q.dtype != torch.bfloat16 or q.device != cache.device:
-        raise ValueError(f"draft_attention: q must be bf16 [{B}, T, q_heads, {hd}] on {cache.device}, got {q.dtype} {list(q.shape)} on {q.device}")
-    T, qh = q.shape[1], q.shape[2]
+    dev, bf16 = cache.device, torch.bfloat16
+    shape = q.shape
+    if len(shape) != 4 or shape[0] != B or shape[3] != hd or q.dtype is not bf16 or q.device != dev:
+        raise ValueError(f"draft_attention: q must be bf16 [{B}, T, q_heads, {hd}] on {dev}, got {q.dtype} {list(shape)} on {q.device}")
+    T, qh = shape[1], shape[2]
     if T > MAX_DRAFTS:
         raise ValueError(f"draft_attention: at most {MAX_DRAFTS} drafts per sequence, got {T}")
     if qh % H or qh == 0:
         raise ValueError(f"draft_attention: {qh} query heads are not a multiple of {H} KV heads")
     if out is None:
         # nodes behind counts are not written: zeros there rather than what the memory held
-        out = (torch.empty if counts is None else torch.zeros)((B, T, qh, hd), dtype=torch.bfloat16, device=q.device)
-    elif out.shape != q.shape or out.dtype != torch.bfloat16 or out.device != q.device:
+        out = (torch.empty if counts is None else torch.zeros)(shape, dtype=bf16, device=dev)
+    elif out.shape != shape or out.dtype is not bf16 or out.device != dev:
         raise ValueError("draft_attention: out must be like q")
-    for x, name in ((q, "q"), (out, "out")):
-        if x.stride(3) != 1 or x.stride(2) != hd:
-            raise ValueError(f"draft_attention: heads of {name} must be dense")
-    if visible is not None and (visible.dtype != torch.int64 or visible.shape != (B, T) or visible.device != q.device or not visible.is_contiguous()):
-        raise ValueError(f"draft_attention: visible must be a contiguous int64 [{B}, {T}] on {q.device}")
-    p, n = _ints(pos, "draft_attention: pos", q.device, B), _ints(counts, "draft_attention: counts", q.device, B)
-    a = _Draft(q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), out.stride(0), out.stride(1), p, n,
-               0 if visible is None else visible.data_ptr(), T, qh, window, splits, hd ** -0.5 if scale is None else scale, 0)
-    key = (T, qh, window, splits)
+    qs, os = q.stride(), out.stride()
+    if qs[3] != 1 or os[3] != 1 or qs[2] != hd or os[2] != hd:
+        raise ValueError("draft_attention: heads of q and out must be dense")
+    if visible is not None and (visible.dtype is not torch.int64 or visible.shape != (B, T) or visible.device != dev or not visible.is_contiguous()):
+        raise ValueError(f"draft_attention: visible must be a contiguous int64 [{B}, {T}] on {dev}")
+    p, n = _ints(pos, "draft_attention: pos", dev, (B,)), _ints(counts, "draft_attention: counts", dev, (B,))
+    args = (q.data_ptr(), out.data_ptr(), qs[0], qs[1], os[0], os[1], p, n, 0 if visible is None else visible.data_ptr(), T, qh, window, splits,
+            hd ** -0.5 if scale is None else scale)
+    key = (T, qh, window, splits, scale)
     floats = cache._scratch.get(key)
     if floats is None:                           # a function of the sizes alone; also checks the arguments
-        fn = _native.lib().mesh_draft_attention_scratch
-        fn.restype = c_longlong
-        floats = int(fn(ctypes.byref(cache._c), ctypes.byref(a)))
+        floats = _lib().mesh_draft_attention_scratch(cache._at, _ARGS.pack(*args, 0))
         if floats < 0:
             raise ValueError(_native.last_error())
+        if len(cache._scratch) > 256:            # a scale of every call's own
+            cache._scratch.clear()
         cache._scratch[key] = floats
     if B == 0 or T == 0:
         return out
-    if q.device.type != "cuda":
-        raise ValueError(f"draft_attention: the tensors are on {q.device}; the kernel needs a GPU")
-    # scratch of the call's own: calls on other streams and other captured graphs share nothing
-    scratch = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
-    a.scratch = scratch.data_ptr() if scratch is not None else 0
-    _launch(q.device, "mesh_draft_attention", ctypes.byref(cache._c), ctypes.byref(a))
-    _native.count_launch(2 if floats else 1)
+    if floats == 0 or cache._index < 0:
+        _launch(cache._index, "mesh_draft_attention", 1, cache._at, _ARGS.pack(*args, 0))
+    else:
+        # scratch of the call's own: calls on other streams and other captured graphs share nothing
+        scratch = torch.empty(floats, dtype=torch.float32, device=dev)
+        _launch(cache._index, "mesh_draft_attention", 2, cache._at, _ARGS.pack(*args, scratch.data_ptr()))
     return out

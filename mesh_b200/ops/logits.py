@@ -5,33 +5,36 @@ Beside ``ops.decode.decode_argmax``, which chooses among the logits as they are.
 """
 from __future__ import annotations
 
-import ctypes
-from ctypes import c_int, c_longlong, c_void_p
+import struct
 
 import torch
 
-from .. import _native
-from .cache import _ints, _launch
+from .cache import _index, _ints, _launch
+
+# ``MeshLogits`` (csrc/ops/draft_api.h): logits, ldl, out, ldo, half, rows, vocab, vocab_offset, history, ldh, hist, history_len, prompt_len,
+# repetition, presence, frequency, bias_ids, bias, ldb, nbias, bias_len, allowed, ldw, tokens
+_ARGS = struct.Struct("@PqPqiiiiPqiPPPPPPPqiPPqP")
 
 
-class _Logits(ctypes.Structure):
-    """``MeshLogits`` (csrc/ops/draft_api.h)."""
-    _fields_ = [("logits", c_void_p), ("ldl", c_longlong), ("out", c_void_p), ("ldo", c_longlong), ("half", c_int),
-                ("rows", c_int), ("vocab", c_int), ("vocab_offset", c_int),
-                ("history", c_void_p), ("ldh", c_longlong), ("hist", c_int), ("history_len", c_void_p), ("prompt_len", c_void_p),
-                ("repetition", c_void_p), ("presence", c_void_p), ("frequency", c_void_p),
-                ("bias_ids", c_void_p), ("bias", c_void_p), ("ldb", c_longlong), ("nbias", c_int), ("bias_len", c_void_p),
-                ("allowed", c_void_p), ("ldw", c_longlong), ("tokens", c_void_p)]
-
-
-def _rows2d(t: torch.Tensor, name: str, dtype, device, rows: int, cols: int | None = None) -> torch.Tensor:
-    """A matrix of ``rows`` rows whose last dimension is dense; a stride of 0 between rows (one list for all) is allowed."""
-    if t.dim() != 2 or t.shape[0] != rows or (cols is not None and t.shape[1] != cols) or t.dtype != dtype or t.device != device:
+def _rows2d(t: torch.Tensor, name: str, dtype, device, rows: int, cols: int | None = None) -> tuple[int, int, int]:
+    """(address, row stride, columns) of a matrix of ``rows`` rows whose last dimension is dense; a stride of 0 between rows (one
+    list for all) is allowed."""
+    shape = t.shape
+    if len(shape) != 2 or shape[0] != rows or (cols is not None and shape[1] != cols) or t.dtype is not dtype or t.device != device:
         raise ValueError(f"constrain_logits: {name} must be {dtype} [{rows}, {'n' if cols is None else cols}] on {device}, "
-                         f"got {t.dtype} {list(t.shape)} on {t.device}")
-    if t.shape[1] > 1 and t.stride(1) != 1:
+                         f"got {t.dtype} {list(shape)} on {t.device}")
+    stride = t.stride()
+    if stride[1] != 1 and shape[1] > 1:
         raise ValueError(f"constrain_logits: rows of {name} must be dense")
-    return t
+    return t.data_ptr(), stride[0], shape[1]
+
+
+def _per_row(t: torch.Tensor | None, name: str, device, rows: int) -> int:
+    if t is None:
+        return 0
+    if t.dtype is not torch.float32 or t.shape != (rows,) or t.device != device or not t.is_contiguous():
+        raise ValueError(f"constrain_logits: {name} must be contiguous fp32 [{rows}] on {device}")
+    return t.data_ptr()
 
 
 def constrain_logits(logits: torch.Tensor, *, history: torch.Tensor | None = None, history_len: torch.Tensor | None = None,
@@ -56,48 +59,43 @@ def constrain_logits(logits: torch.Tensor, *, history: torch.Tensor | None = Non
         raise ValueError(f"constrain_logits: logits must be fp32 or bf16 [R, V] on a GPU, got {logits.dtype} {list(logits.shape)} on {logits.device}")
     R, V = logits.shape
     dev = logits.device
-    if V == 0 or (V > 1 and logits.stride(1) != 1):
+    ldl, dense = logits.stride()
+    if V == 0 or (V > 1 and dense != 1):
         raise ValueError("constrain_logits: rows of the logits must be dense and not empty")
     if out is None and tokens is None:
         raise ValueError("constrain_logits: ask for out, for tokens, or for both")
-    if R > 1 and logits.stride(0) < V:
+    if R > 1 and ldl < V:
         raise ValueError("constrain_logits: rows of the logits overlap")
-    a = _Logits(logits=logits.data_ptr(), ldl=logits.stride(0), half=int(logits.dtype == torch.bfloat16), rows=R, vocab=V, vocab_offset=vocab_offset)
+    o, ldo = 0, 0
     if out is not None:
-        _rows2d(out, "out", logits.dtype, dev, R, V)
-        if R > 1 and out.stride(0) < V:
+        o, ldo, _ = _rows2d(out, "out", logits.dtype, dev, R, V)
+        if R > 1 and ldo < V:
             raise ValueError("constrain_logits: rows of out overlap")
-        a.out, a.ldo = out.data_ptr(), out.stride(0)
+    h, ldh, hist = 0, 0, 0
     if history is not None:
-        _rows2d(history, "history", torch.int32, dev, R)
-        if history.shape[1] > 65535:
-            raise ValueError(f"constrain_logits: a history of at most 65535 tokens, got {history.shape[1]}")
-        a.history, a.ldh, a.hist = history.data_ptr(), history.stride(0), history.shape[1]
-    elif any(x is not None for x in (history_len, prompt_len, repetition, presence, frequency)):
+        h, ldh, hist = _rows2d(history, "history", torch.int32, dev, R)
+        if hist > 65535:
+            raise ValueError(f"constrain_logits: a history of at most 65535 tokens, got {hist}")
+    elif not (history_len is prompt_len is repetition is presence is frequency is None):
         raise ValueError("constrain_logits: penalties need a history")
-    a.history_len = _ints(history_len, "constrain_logits: history_len", dev, R)
-    a.prompt_len = _ints(prompt_len, "constrain_logits: prompt_len", dev, R)
-    for name, t in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
-        if t is not None:
-            if t.dtype != torch.float32 or t.shape != (R,) or t.device != dev or not t.is_contiguous():
-                raise ValueError(f"constrain_logits: {name} must be contiguous fp32 [{R}] on {dev}")
-            setattr(a, name, t.data_ptr())
     if (bias is None) != (bias_ids is None) or (bias is None and bias_len is not None):
         raise ValueError("constrain_logits: bias and bias_ids come together")
+    ids, b, ldb, nbias = 0, 0, 0, 0
     if bias is not None:
-        _rows2d(bias_ids, "bias_ids", torch.int32, dev, R)
-        _rows2d(bias, "bias", torch.float32, dev, R, bias_ids.shape[1])
-        if R > 1 and bias.stride(0) != bias_ids.stride(0):
+        ids, ld_ids, nbias = _rows2d(bias_ids, "bias_ids", torch.int32, dev, R)
+        b, ldb, _ = _rows2d(bias, "bias", torch.float32, dev, R, nbias)
+        if R > 1 and ldb != ld_ids:
             raise ValueError("constrain_logits: bias and bias_ids must have the same row stride")
-        if bias.shape[1] > 32767:
-            raise ValueError(f"constrain_logits: at most 32767 biases, got {bias.shape[1]}")
-        a.bias_ids, a.bias, a.ldb, a.nbias = bias_ids.data_ptr(), bias.data_ptr(), bias.stride(0), bias.shape[1]
-    a.bias_len = _ints(bias_len, "constrain_logits: bias_len", dev, R)
+        if nbias > 32767:
+            raise ValueError(f"constrain_logits: at most 32767 biases, got {nbias}")
+    w, ldw = 0, 0
     if allowed is not None:
-        _rows2d(allowed, "allowed", torch.int32, dev, R, (V + 31) // 32)
-        a.allowed, a.ldw = allowed.data_ptr(), allowed.stride(0)
-    a.tokens = _ints(tokens, "constrain_logits: tokens", dev, R)
+        w, ldw, _ = _rows2d(allowed, "allowed", torch.int32, dev, R, (V + 31) // 32)
+    args = _ARGS.pack(logits.data_ptr(), ldl, o, ldo, logits.dtype is torch.bfloat16, R, V, vocab_offset, h, ldh, hist,
+                      _ints(history_len, "constrain_logits: history_len", dev, (R,)), _ints(prompt_len, "constrain_logits: prompt_len", dev, (R,)),
+                      _per_row(repetition, "repetition", dev, R), _per_row(presence, "presence", dev, R), _per_row(frequency, "frequency", dev, R),
+                      ids, b, ldb, nbias, _ints(bias_len, "constrain_logits: bias_len", dev, (R,)), w, ldw,
+                      _ints(tokens, "constrain_logits: tokens", dev, (R,)))
     if R:
-        _launch(dev, "mesh_constrain_logits", ctypes.byref(a))
-        _native.count_launch()
+        _launch(_index(dev), "mesh_constrain_logits", 1, args)
     return out if out is not None else tokens
