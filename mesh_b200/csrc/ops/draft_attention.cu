@@ -1,9 +1,12 @@
 // Attention of drafted tokens over a cache of bf16 rows or of 8-bit codes.
 //
 // The T drafts of a sequence and the G query heads that share a KV head are T * G query rows over the same keys: rows
-// t * G + g.  A CTA takes 16 of them (one tile of the matrix instruction) and a slice of the keys; its warps take blocks of 16
-// keys in turn, each with a ring of its own that cp.async fills, so that nothing but the end of the slice joins them.  Slices
-// of a (sequence, KV head) are joined by a second kernel.
+// t * G + g.  An item is 16 of them (one tile of the matrix instruction) with all keys that any of them sees.  The items' keys, in
+// units of 16 a warp, are laid end to end and cut into one share per CTA, all alike: lengths differ from sequence to sequence,
+// and whole items (or equal slices of each) left most SMs waiting for the longest (282 us of a case that now takes MEASURED).  Only
+// the device knows the lengths, so every CTA finds its share itself.  A CTA's warps take blocks of 16 keys in turn, each
+// with a ring of its own that cp.async fills, so that nothing but the end of an item joins them.  Items that were cut are
+// joined by a second kernel.
 //
 // Formulas.  A score is s = scale q.k; with 8-bit rows k = ks kc and v = vs vc, where kc, vc are the codes: s = (scale ks) (q.kc),
 // and the weight of a value's codes is w = exp(s - m) vs.  The running reference m of a row is the maximum of s + log vs, so
@@ -27,15 +30,15 @@ namespace draft {
 
 constexpr int ROWS = 16;              // query rows of a tile
 constexpr int KEYS = 16;              // keys of a block
-constexpr int MOST_SPLITS = 64;
 
 struct Args {
   const __nv_bfloat16* q; __nv_bfloat16* out; long long q_sb, q_st, o_sb, o_st;
   const uint8_t* k; const uint8_t* v; const float* k_scale; const float* v_scale;
   const int* pos; const int* counts; const long long* visible;
-  int B, T, q_heads, kv_heads, max_seq, window, splits, tiles;
+  int B, T, q_heads, kv_heads, max_seq, window, tiles;
   float scale_log2;                   // scale * log2(e): exponentials are powers of two
-  float* part; float* part_ml;        // [B * kv_heads * tiles][splits][ROWS][HD] and [..][ROWS] {m, l}
+  float4* part; float2* part_ml;      // two slots per CTA: the output as the fragments lie, and {m, l} of the rows
+  int shares;                         // CTAs of the attention kernel
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -97,6 +100,63 @@ __device__ __forceinline__ Seq sequence(const Args& a, int b) {
   return s;
 }
 
+// How the work is cut.  Sequence b has `rows` query rows per KV head in `tiles` tiles and `units` units of keys; its items follow
+// one another, KV head by KV head, tile by tile.
+struct Load {
+  Seq s; int tiles, units; long long work;
+};
+__device__ __forceinline__ Load load_of(const Args& a, int b, int unit) {
+  Load l;
+  l.s = sequence(a, b);
+  const int rows = max(l.s.count, 0) * (a.q_heads / a.kv_heads);
+  l.tiles = (rows + ROWS - 1) / ROWS;
+  l.units = max(1, (l.s.hi - l.s.lo + unit - 1) / unit);   // rows that see nothing are written too
+  l.work = (long long)l.tiles * l.units * a.kv_heads;
+  return l;
+}
+// Work of all sequences before b, and of all; by a whole warp.
+__device__ __forceinline__ void work_before(const Args& a, int unit, int b, long long& before, long long& total) {
+  const int lane = threadIdx.x & 31;
+  long long lo = 0, all = 0;
+  for (int i = lane; i < a.B; i += 32) {
+    const long long w = load_of(a, i, unit).work;
+    all += w;
+    if (i < b) lo += w;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    lo += __shfl_xor_sync(0xffffffffu, lo, o);
+    all += __shfl_xor_sync(0xffffffffu, all, o);
+  }
+  before = lo;
+  total = all;
+}
+// The sequence that unit w of the work belongs to, and the work before it; by a whole warp.  w < total.
+__device__ __forceinline__ int sequence_of(const Args& a, int unit, long long w, long long& before) {
+  const int lane = threadIdx.x & 31;
+  before = 0;
+  for (int i0 = 0; i0 < a.B; i0 += 32) {
+    const long long mine = i0 + lane < a.B ? load_of(a, i0 + lane, unit).work : 0;
+    long long upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    const uint32_t past = __ballot_sync(0xffffffffu, before + upto > w);
+    if (past) {
+      const int l = __ffs(past) - 1;
+      before += __shfl_sync(0xffffffffu, upto - mine, l);
+      return i0 + l;
+    }
+    before += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return a.B;
+}
+// CTA c of n has units [c total / n, (c + 1) total / n).
+__device__ __forceinline__ long long share_begin(long long c, long long n, long long total) { return c * total / n; }
+__device__ __forceinline__ long long share_of(long long w, long long n, long long total) { return ((w + 1) * n - 1) / total; }
+
 template <int HD, bool Q8>
 struct Cfg {
   static constexpr int RB = Q8 ? HD : 2 * HD;             // bytes of a row
@@ -106,7 +166,9 @@ struct Cfg {
   static constexpr int STAGES = (200 * 1024 / WARPS) / STAGE > 8 ? 8 : (200 * 1024 / WARPS) / STAGE;
   static constexpr int RING = WARPS * STAGES * STAGE;
   static constexpr int QB = ROWS * HD * 2;
-  static constexpr int MERGE = WARPS * ROWS * (HD + 2) * 4;
+  static constexpr int UNIT = WARPS * KEYS;               // keys of a unit of work
+  static constexpr int OUT_PITCH = HD + 8;                // of a row of the result in shared memory
+  static constexpr int MERGE = WARPS * ROWS * HD * 4;
   static constexpr int SMEM = QB + (RING > MERGE ? RING : MERGE);
   static constexpr int PER = Q8 ? 16 : 8;                 // values of a chunk
   static constexpr int VW = Q8 && HD == 64 ? 8 : PER;     // columns of V a lane takes at a time
@@ -132,6 +194,10 @@ __device__ __forceinline__ bool finite_rows(const uint8_t* rows, int lane) {
   return !__any_sync(0xffffffffu, bad);
 }
 
+// Values i % VW of column group n' = 0..7 of group i / VW: the column that tile i's n' is.
+template <int VW>
+__device__ __forceinline__ int column(int i, int n) { return ((i / VW) * 8 + n) * VW + i % VW; }
+
 template <int HD, bool Q8>
 __global__ void __launch_bounds__(Cfg<HD, Q8>::WARPS * 32, 1) attention_kernel(const __grid_constant__ Args a) {
   using C = Cfg<HD, Q8>;
@@ -140,20 +206,44 @@ __global__ void __launch_bounds__(Cfg<HD, Q8>::WARPS * 32, 1) attention_kernel(c
   constexpr int NT = HD / 8;                              // column tiles of the output
   extern __shared__ __align__(128) uint8_t smem[];
   uint4* q_s = reinterpret_cast<uint4*>(smem);            // [k step][lane]: operand A of the scores
+  __shared__ float unit_s[ROWS], weight_s[C::WARPS][ROWS], m_s[ROWS], l_s[ROWS];
+  __shared__ float2 ml_s[C::WARPS][ROWS];
+  __shared__ long long start_s[2];
+  __shared__ int seq_s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = lane >> 2, t4 = lane & 3;
   uint8_t* ring = smem + C::QB + warp * (STAGES * C::STAGE);
   const uint32_t ring_u = smem_u32(ring);
-  griddep_launch_dependents();
-  griddep_wait();
-
-  const int tile = blockIdx.x, split = blockIdx.y;
-  const int hk = blockIdx.z % a.kv_heads, b = blockIdx.z / a.kv_heads;
   const int G = a.q_heads / a.kv_heads;
-  const Seq s = sequence(a, b);
-  const int n_rows = min(max(s.count, 0) * G - tile * ROWS, ROWS);
-  if (n_rows <= 0) return;                                // nothing of this tile is written: the joining kernel knows
-  const int per = ((s.hi - s.lo + a.splits - 1) / a.splits + KEYS - 1) / KEYS * KEYS;
-  const int k_lo = min(s.lo + split * per, s.hi), k_hi = min(k_lo + per, s.hi);
+  griddep_wait();
+  griddep_launch_dependents();                            // not before: the joining kernel reads lengths before its own wait
+
+  if (warp == 0) {
+    long long before, total, ignore;
+    work_before(a, C::UNIT, 0, ignore, total);
+    const long long shares = min((long long)a.shares, total);
+    if (lane == 0) { start_s[0] = 0; start_s[1] = 0; }
+    if (blockIdx.x < shares) {
+      const long long w0 = share_begin(blockIdx.x, shares, total), w1 = share_begin(blockIdx.x + 1, shares, total);
+      const int b = sequence_of(a, C::UNIT, w0, before);
+      if (lane == 0) { start_s[0] = w0 - before; start_s[1] = w1 - before; seq_s = b; }
+    }
+  }
+  __syncthreads();
+  long long at = start_s[0], stop = start_s[1];           // relative to the first unit of sequence b
+  int b = seq_s;
+  for (bool first_item = true; at < stop; first_item = false) {
+  Load load = load_of(a, b, C::UNIT);
+  while (at >= load.work) {
+    at -= load.work;
+    stop -= load.work;
+    load = load_of(a, ++b, C::UNIT);
+  }
+  const Seq s = load.s;
+  const int item = (int)(at / load.units), hk = item / load.tiles, tile = item % load.tiles;
+  const int u0 = (int)(at % load.units), u1 = (int)min((long long)load.units, u0 + stop - at);
+  at += u1 - u0;
+  const int n_rows = min(s.count * G - tile * ROWS, ROWS);
+  const int k_lo = min(s.lo + u0 * C::UNIT, s.hi), k_hi = min(s.lo + u1 * C::UNIT, s.hi);
   const int blocks = (k_hi - k_lo + KEYS - 1) / KEYS;
   const long long base = ((long long)b * a.kv_heads + hk) * a.max_seq;
   const uint8_t* kp = a.k + base * RB;
@@ -182,47 +272,55 @@ __global__ void __launch_bounds__(Cfg<HD, Q8>::WARPS * 32, 1) attention_kernel(c
 #pragma unroll
   for (int i = 0; i < STAGES - 1; ++i) fetch(i);
 
-  // ---- queries: row i of the tile as 4 consecutive values per lane and k step, in the order the keys' chunks have them
-  float q_unit[2];                                        // what a row was divided by, times the scale
-  {
-    constexpr int STEPS = HD / 16;
-    __shared__ float unit_s[ROWS];
-    for (int i = warp; i < ROWS; i += C::WARPS) {         // a warp per row: its largest value
-      float top = 0.f;
-      const int r = tile * ROWS + i, t = r / G, h = hk * G + r % G;
-      if (Q8 && i < n_rows) {
-        const __nv_bfloat16* src = a.q + b * a.q_sb + t * a.q_st + (long long)h * HD;
-        for (int d = lane; d < HD; d += 32) top = fmaxf(top, fabsf(__bfloat162float(src[d])));
+  // ---- queries: 4 consecutive values of a row are two words of a lane and k step, in the order the keys' chunks have them
+  for (int i = warp; i < ROWS; i += C::WARPS) {
+    const int r = tile * ROWS + i, t = r / G, h = hk * G + r % G;
+    const __nv_bfloat16* src = a.q + b * a.q_sb + t * a.q_st + (long long)h * HD;
+    const bool vec = (reinterpret_cast<uintptr_t>(src) & 7) == 0;
+    constexpr int PARTS = (HD + 127) / 128;
+    uint2 x[PARTS];
+    float top = 0.f;
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) {
+      x[p] = make_uint2(0, 0);
+      const int col = p * 128 + lane * 4;
+      if (i < n_rows && col < HD) {
+        if (vec) {
+          x[p] = *reinterpret_cast<const uint2*>(src + col);
+        } else {
+          const unsigned short* u = reinterpret_cast<const unsigned short*>(src + col);
+          x[p] = make_uint2(u[0] | (uint32_t)u[1] << 16, u[2] | (uint32_t)u[3] << 16);
+        }
       }
+      top = fmaxf(fmaxf(top, fmaxf(fabsf(__uint_as_float(x[p].x << 16)), fabsf(__uint_as_float(x[p].x & 0xffff0000u)))),
+                  fmaxf(fabsf(__uint_as_float(x[p].y << 16)), fabsf(__uint_as_float(x[p].y & 0xffff0000u))));
+    }
+    float up = 1.f;
+    if (Q8) {
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
       // the power of two that brings it to 2^8..2^9; bounded, so that neither it nor its inverse leaves fp32
-      const int e = top > 0.f ? min(max(8 - ilogbf(top), -110), 110) : 0;
-      if (lane == 0) unit_s[i] = Q8 ? ldexpf(1.f, e) : 1.f;
+      up = ldexpf(1.f, top > 0.f ? min(max(8 - ilogbf(top), -110), 110) : 0);
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < STEPS * 32; i += C::WARPS * 32) {
-      const int step = i / 32, l = i % 32, ln = l >> 2, lt = l & 3;
-      const int col = ((step / (PER / 4)) * 4 + lt) * PER + (step % (PER / 4)) * 4;
-      uint32_t w[2][2];
+    if (lane == 0) unit_s[i] = up;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int row = ln + 8 * j, r = tile * ROWS + row, t = r / G, h = hk * G + r % G;
-        float f[4] = {0.f, 0.f, 0.f, 0.f};
-        if (row < n_rows) {
-          const __nv_bfloat16* src = a.q + b * a.q_sb + t * a.q_st + (long long)h * HD + col;
-#pragma unroll
-          for (int x = 0; x < 4; ++x) f[x] = __bfloat162float(src[x]) * unit_s[row];
+    for (int p = 0; p < PARTS; ++p) {
+      const int col = p * 128 + lane * 4;
+      if (col < HD) {
+        const int chunk = col / PER, step = chunk / 4 * (PER / 4) + col % PER / 4;
+        uint32_t* w = reinterpret_cast<uint32_t*>(q_s + step * 32 + (i & 7) * 4 + chunk % 4) + (i >> 3);
+        if (Q8) {
+          w[0] = pack16(true, __uint_as_float(x[p].x << 16) * up, __uint_as_float(x[p].x & 0xffff0000u) * up);
+          w[2] = pack16(true, __uint_as_float(x[p].y << 16) * up, __uint_as_float(x[p].y & 0xffff0000u) * up);
+        } else {
+          w[0] = x[p].x;
+          w[2] = x[p].y;
         }
-        w[j][0] = pack16(Q8, f[0], f[1]);
-        w[j][1] = pack16(Q8, f[2], f[3]);
       }
-      q_s[i] = make_uint4(w[0][0], w[1][0], w[0][1], w[1][1]);
     }
-    __syncthreads();
-    q_unit[0] = a.scale_log2 / unit_s[n];
-    q_unit[1] = a.scale_log2 / unit_s[n + 8];
   }
+  __syncthreads();
+  const float q_unit[2] = {a.scale_log2 / unit_s[n], a.scale_log2 / unit_s[n + 8]};
 
   // ---- what this lane's two rows see
   int row_lo[2];
@@ -406,130 +504,180 @@ __global__ void __launch_bounds__(Cfg<HD, Q8>::WARPS * 32, 1) attention_kernel(c
   }
   cp_async_wait<0>();
 
-  // ---- join the warps: the ring's memory holds every warp's output
-  __syncthreads();
-  float* o_s = reinterpret_cast<float*>(smem + C::QB);    // [warp][row][HD]
-  float* ml_s = o_s + C::WARPS * ROWS * HD;               // [warp][row]{m, l}
+  // ---- join the warps: the ring's memory holds every warp's output as its fragments lie, [warp][tile of 8 columns][lane]
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     l[j] += __shfl_xor_sync(0xffffffffu, l[j], 1);
     l[j] += __shfl_xor_sync(0xffffffffu, l[j], 2);
-    if (t4 == 0) {
-      ml_s[(warp * ROWS + n + 8 * j) * 2] = m[j];
-      ml_s[(warp * ROWS + n + 8 * j) * 2 + 1] = l[j];
+    if (t4 == 0) ml_s[warp][n + 8 * j] = make_float2(m[j], l[j]);
+  }
+  __syncthreads();                                        // every warp is done with its ring
+  float4* o_s = reinterpret_cast<float4*>(smem + C::QB);
+#pragma unroll
+  for (int i = 0; i < NT; ++i) o_s[(warp * NT + i) * 32 + lane] = make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
+  if (threadIdx.x < ROWS) {
+    const int r = threadIdx.x;
+    float mm = -CUDART_INF_F, ll = 0.f;
+#pragma unroll
+    for (int w = 0; w < C::WARPS; ++w) mm = fmaxf(mm, ml_s[w][r].x);
+    const float ref = mm == -CUDART_INF_F ? 0.f : mm;
+#pragma unroll
+    for (int w = 0; w < C::WARPS; ++w) {
+      const float wt = ex2(ml_s[w][r].x - ref);           // 0 for a warp that saw no key; its sum may be NaN
+      weight_s[w][r] = wt;
+      ll += wt * ml_s[w][r].y;
     }
-#pragma unroll
-    for (int i = 0; i < NT; ++i)
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-        o_s[(warp * ROWS + n + 8 * j) * HD + ((i / VW) * 8 + 2 * t4 + e) * VW + i % VW] = o[i][2 * j + e];
+    m_s[r] = mm;
+    l_s[r] = ll;
   }
   __syncthreads();
-  const long long item = ((long long)(b * a.kv_heads + hk) * a.tiles + tile) * a.splits + split;
-  for (int i = threadIdx.x; i < n_rows * (HD / 4); i += C::WARPS * 32) {
-    const int row = i / (HD / 4), d = i % (HD / 4) * 4;
-    float mm = -CUDART_INF_F;
+  const bool whole = u1 - u0 == load.units;
+  const long long slot = 2 * (long long)blockIdx.x + (first_item ? 0 : 1);
+  __nv_bfloat16* row_s = reinterpret_cast<__nv_bfloat16*>(smem);          // the queries' memory and, after a barrier, more
+  float4 sum[(NT * 32 + C::WARPS * 32 - 1) / (C::WARPS * 32)];
 #pragma unroll
-    for (int w = 0; w < C::WARPS; ++w) mm = fmaxf(mm, ml_s[(w * ROWS + row) * 2]);
-    const float at = mm == -CUDART_INF_F ? 0.f : mm;
-    float ll = 0.f;
+  for (int x = 0; x < NT / C::WARPS; ++x) {
+    const int i = x * C::WARPS + warp;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < C::WARPS; ++w) {
-      const float wt = ex2(ml_s[(w * ROWS + row) * 2] - at);      // 0 for a warp that saw no key; its sum may be NaN
-      ll += wt * ml_s[(w * ROWS + row) * 2 + 1];
-      const float4 x = *reinterpret_cast<const float4*>(o_s + (w * ROWS + row) * HD + d);
-      acc.x += wt * x.x; acc.y += wt * x.y; acc.z += wt * x.z; acc.w += wt * x.w;
+      const float w0 = weight_s[w][n], w1 = weight_s[w][n + 8];
+      const float4 v = o_s[(w * NT + i) * 32 + lane];
+      acc.x += w0 * v.x; acc.y += w0 * v.y; acc.z += w1 * v.z; acc.w += w1 * v.w;
     }
-    if (a.splits > 1) {
-      *reinterpret_cast<float4*>(a.part + (item * ROWS + row) * HD + d) = acc;
-      if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (item * ROWS + row) * 2) = make_float2(mm, ll);
-    } else {
-      const float inv = ll == 0.f ? 0.f : 1.f / ll;
-      const int r = tile * ROWS + row;
-      __nv_bfloat162 h[2] = {__floats2bfloat162_rn(acc.x * inv, acc.y * inv), __floats2bfloat162_rn(acc.z * inv, acc.w * inv)};
-      __nv_bfloat162* dst = reinterpret_cast<__nv_bfloat162*>(a.out + b * a.o_sb + (r / G) * a.o_st + (long long)(hk * G + r % G) * HD + d);
-      dst[0] = h[0];
-      dst[1] = h[1];
+    sum[x] = acc;
+    if (!whole) a.part[(slot * NT + i) * 32 + lane] = acc;
+  }
+  if (!whole) {
+    if (threadIdx.x < ROWS) a.part_ml[slot * ROWS + threadIdx.x] = make_float2(m_s[threadIdx.x], l_s[threadIdx.x]);
+  } else {
+    __syncthreads();
+    const float i0 = l_s[n] == 0.f ? 0.f : 1.f / l_s[n], i1 = l_s[n + 8] == 0.f ? 0.f : 1.f / l_s[n + 8];
+#pragma unroll
+    for (int x = 0; x < NT / C::WARPS; ++x) {
+      const int i = x * C::WARPS + warp;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int col = column<VW>(i, 2 * t4 + e);
+        row_s[n * C::OUT_PITCH + col] = __float2bfloat16_rn((e ? sum[x].y : sum[x].x) * i0);
+        row_s[(n + 8) * C::OUT_PITCH + col] = __float2bfloat16_rn((e ? sum[x].w : sum[x].z) * i1);
+      }
     }
+    __syncthreads();
+    for (int i = threadIdx.x; i < n_rows * (HD / 2); i += C::WARPS * 32) {
+      const int row = i / (HD / 2), d = i % (HD / 2) * 2, r = tile * ROWS + row;
+      *reinterpret_cast<__nv_bfloat162*>(a.out + b * a.o_sb + (r / G) * a.o_st + (long long)(hk * G + r % G) * HD + d) =
+          *reinterpret_cast<const __nv_bfloat162*>(row_s + row * C::OUT_PITCH + d);
+    }
+  }
+  __syncthreads();                                        // shared memory is the next item's
   }
 }
 
-// Joins the slices: a warp per query row.
-template <int HD>
+// Joins the shares of the items that were cut: a CTA per item and tile of 8 columns, whose warps take the shares in turn.
+template <int HD, bool Q8>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args a) {
-  griddep_launch_dependents();
-  griddep_wait();
-  const int lane = threadIdx.x & 31, G = a.q_heads / a.kv_heads;
-  const long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int rows = a.T * G;
-  const int r = (int)(w % rows);
-  const long long bh = w / rows;
-  const int b = (int)(bh / a.kv_heads), hk = (int)(bh % a.kv_heads);
-  if (b >= a.B) return;
-  const Seq s = sequence(a, b);
-  if (r >= s.count * G) return;
-  const long long item = (bh * a.tiles + r / ROWS) * a.splits;
-  const int row = r % ROWS;
-  float ms[MOST_SPLITS / 32], ls[MOST_SPLITS / 32], mm = -CUDART_INF_F;
-#pragma unroll
-  for (int i = 0; i < MOST_SPLITS / 32; ++i) {
-    const int sp = i * 32 + lane;
-    float2 x = make_float2(-CUDART_INF_F, 0.f);
-    if (sp < a.splits) x = __ldcg(reinterpret_cast<const float2*>(a.part_ml + ((item + sp) * ROWS + row) * 2));
-    ms[i] = x.x; ls[i] = x.y;
-    mm = fmaxf(mm, x.x);
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
-  const float at = mm == -CUDART_INF_F ? 0.f : mm;
-  float l = 0.f;
-#pragma unroll
-  for (int i = 0; i < MOST_SPLITS / 32; ++i) {
-    ms[i] = ex2(ms[i] - at);
-    l += ms[i] * ls[i];
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-  constexpr int PL = HD / 32;                             // columns of a lane
-  float acc[PL];
-#pragma unroll
-  for (int i = 0; i < PL; ++i) acc[i] = 0.f;
-#pragma unroll
-  for (int i = 0; i < MOST_SPLITS / 32; ++i)
-#pragma unroll 4
-    for (int x = 0; x < min(32, a.splits - i * 32); ++x) {
-      const float wt = __shfl_sync(0xffffffffu, ms[i], x);
-      const float* p = a.part + ((item + i * 32 + x) * ROWS + row) * HD + lane * 2;
-#pragma unroll
-      for (int y = 0; y < PL / 2; ++y) {
-        const float2 v = __ldcg(reinterpret_cast<const float2*>(p + y * 64));
-        acc[2 * y] += wt * v.x;
-        acc[2 * y + 1] += wt * v.y;
+  using C = Cfg<HD, Q8>;
+  constexpr int NT = HD / 8;
+  __shared__ long long c_s[3];
+  __shared__ float m_s[8][ROWS], l_s[8][ROWS];
+  __shared__ float4 o_s[8][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = lane >> 2, t4 = lane & 3, G = a.q_heads / a.kv_heads;
+  const int i = blockIdx.y, tile = blockIdx.x % a.tiles, hk = blockIdx.x / a.tiles % a.kv_heads, b = blockIdx.x / a.tiles / a.kv_heads;
+  // the lengths are older than the kernel before this one, which lets this one start when it has seen them
+  if (warp == 0) {
+    const Load load = load_of(a, b, C::UNIT);
+    long long before, total;
+    work_before(a, C::UNIT, b, before, total);
+    if (lane == 0) {
+      c_s[0] = c_s[1] = 0;
+      if (tile < load.tiles) {
+        const long long shares = min((long long)a.shares, total), w = before + ((long long)hk * load.tiles + tile) * load.units;
+        c_s[0] = share_of(w, shares, total);
+        c_s[1] = share_of(w + load.units - 1, shares, total);
+        c_s[2] = share_begin(c_s[0], shares, total) >= w ? 0 : 1;        // whether the item is the first of its first share
       }
     }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  __nv_bfloat16* dst = a.out + b * a.o_sb + (r / G) * a.o_st + (long long)(hk * G + r % G) * HD + lane * 2;
+  }
+  __syncthreads();
+  const long long c0 = c_s[0], c1 = c_s[1];
+  const int odd = (int)c_s[2];
+  griddep_wait();                                         // all wait: what comes after this kernel relies on the one before it
+  if (c0 == c1) return;                                   // whole in one CTA, or not there
+  float m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.f, 0.f};
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (long long c = c0 + warp; c <= c1; c += 8 * 4) {
+    float2 x[4][2];
+    float4 v[4];
 #pragma unroll
-  for (int y = 0; y < PL / 2; ++y)
-    *reinterpret_cast<__nv_bfloat162*>(dst + y * 64) = __floats2bfloat162_rn(acc[2 * y] * inv, acc[2 * y + 1] * inv);
+    for (int y = 0; y < 4; ++y) {
+      const long long cc = c + 8 * y, slot = 2 * cc + (cc == c0 ? odd : 0);
+      x[y][0] = x[y][1] = make_float2(-CUDART_INF_F, 0.f);
+      v[y] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (cc <= c1) {
+        x[y][0] = __ldcg(a.part_ml + slot * ROWS + n);
+        x[y][1] = __ldcg(a.part_ml + slot * ROWS + n + 8);
+        v[y] = __ldcg(a.part + (slot * NT + i) * 32 + lane);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float now = m[j];
+#pragma unroll
+      for (int y = 0; y < 4; ++y) now = fmaxf(now, x[y][j].x);
+      const float ref = now == -CUDART_INF_F ? 0.f : now, old = ex2(m[j] - ref);
+      m[j] = now;
+      l[j] *= old;
+      if (j == 0) { acc.x *= old; acc.y *= old; } else { acc.z *= old; acc.w *= old; }
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const float wt = ex2(x[y][j].x - ref);
+        l[j] += wt * x[y][j].y;
+        if (j == 0) { acc.x += wt * v[y].x; acc.y += wt * v[y].y; } else { acc.z += wt * v[y].z; acc.w += wt * v[y].w; }
+      }
+    }
+  }
+  o_s[warp][lane] = acc;
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+    if (t4 == 0) { m_s[warp][n + 8 * j] = m[j]; l_s[warp][n + 8 * j] = l[j]; }
+  __syncthreads();
+  // 16 rows x 8 columns: thread -> row, column
+  if (threadIdx.x >= ROWS * 8) return;
+  const int row = threadIdx.x >> 3, c = threadIdx.x & 7, r = tile * ROWS + row;
+  float mm = -CUDART_INF_F, ll = 0.f, sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) mm = fmaxf(mm, m_s[w][row]);
+  const float ref = mm == -CUDART_INF_F ? 0.f : mm;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    const float wt = ex2(m_s[w][row] - ref);
+    ll += wt * l_s[w][row];
+    sum += wt * reinterpret_cast<const float*>(&o_s[w][(row & 7) * 4 + (c >> 1)])[2 * (row >> 3) + (c & 1)];
+  }
+  const Seq s = sequence(a, b);
+  if (r < s.count * G)
+    a.out[b * a.o_sb + (r / G) * a.o_st + (long long)(hk * G + r % G) * HD + column<C::VW>(i, c)] = __float2bfloat16_rn(ll == 0.f ? 0.f : sum / ll);
 }
 
 static int tiles_of(const MeshKvCache* c, const MeshDraftAttention* a) {
   return (a->T * (a->q_heads / c->kv_heads) + ROWS - 1) / ROWS;
 }
 
-// Slices per (sequence, KV head): enough that every SM has a CTA, at most one per 256 keys of the longest range.
-static int splits_of(const MeshKvCache* c, const MeshDraftAttention* a) {
-  if (a->splits > 0) return a->splits < MOST_SPLITS ? a->splits : MOST_SPLITS;
-  const long long work = (long long)c->B * c->kv_heads * tiles_of(c, a);
+template <int HD, bool Q8> static int unit_of() { return Cfg<HD, Q8>::UNIT; }
+static int unit_of(const MeshKvCache* c) {
+  const bool q8 = c->bits == 8;
+  return c->head_dim == 64 ? (q8 ? unit_of<64, true>() : unit_of<64, false>()) : c->head_dim == 128 ? (q8 ? unit_of<128, true>() : unit_of<128, false>())
+                           : (q8 ? unit_of<256, true>() : unit_of<256, false>());
+}
+
+// CTAs: one per SM, or per unit of work where the longest sequences have fewer.
+static int shares_of(const MeshKvCache* c, const MeshDraftAttention* a) {
   long long keys = c->max_seq;
-  if (a->window > 0 && a->window + a->T < keys) keys = a->window + a->T;
-  long long n = work > 0 ? sm_count() / work : 1;
-  const long long most = (keys + 255) / 256;
-  if (n > most) n = most;
-  if (n > MOST_SPLITS) n = MOST_SPLITS;
-  return n < 1 ? 1 : (int)n;
+  if (a->window > 0 && (long long)a->window + a->T < keys) keys = (long long)a->window + a->T;
+  const long long units = (long long)c->B * c->kv_heads * tiles_of(c, a) * ((keys + unit_of(c) - 1) / unit_of(c));
+  const long long most = a->splits > 0 ? a->splits : sm_count();
+  return (int)(units < most ? units : most);
 }
 
 static int check(const MeshKvCache* c, const MeshDraftAttention* a) {
@@ -561,10 +709,11 @@ static cudaError_t launch(void (*kern)(P...), dim3 grid, int threads, int smem, 
   return cudaLaunchKernelEx(&cfg, kern, a);
 }
 
+template <int HD, bool Q8> constexpr bool NT_OK = HD / 8 % Cfg<HD, Q8>::WARPS == 0 && ROWS * Cfg<HD, Q8>::OUT_PITCH * 2 <= Cfg<HD, Q8>::SMEM;
 template <int HD, bool Q8>
 static int run(const Args& p, void* stream) {
   using C = Cfg<HD, Q8>;
-  static_assert(C::STAGES >= 3 && C::SMEM <= 227 * 1024, "ring of a warp");
+  static_assert(C::STAGES >= 3 && C::SMEM <= 226 * 1024 && NT_OK<HD, Q8>, "ring of a warp");
   static std::atomic<unsigned long long> configured{0};   // a bit per device
   int dev = 0;
   MESH_CUDA_OK(cudaGetDevice(&dev));
@@ -572,11 +721,8 @@ static int run(const Args& p, void* stream) {
     MESH_CUDA_OK(cudaFuncSetAttribute(attention_kernel<HD, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
     configured.fetch_or(1ull << (dev & 63));
   }
-  MESH_CUDA_OK(launch(attention_kernel<HD, Q8>, dim3(p.tiles, p.splits, p.B * p.kv_heads), C::WARPS * 32, C::SMEM, stream, p));
-  if (p.splits > 1) {
-    const long long rows = (long long)p.B * p.q_heads * p.T;
-    MESH_CUDA_OK(launch(join_kernel<HD>, dim3((unsigned)((rows + 7) / 8)), 256, 0, stream, p));
-  }
+  MESH_CUDA_OK(launch(attention_kernel<HD, Q8>, dim3(p.shares), C::WARPS * 32, C::SMEM, stream, p));
+  if (p.part) MESH_CUDA_OK(launch(join_kernel<HD, Q8>, dim3((unsigned)(p.B * p.kv_heads * p.tiles), HD / 8), 256, 0, stream, p));
   return 0;
 }
 
@@ -586,9 +732,9 @@ static int run(const Args& p, void* stream) {
 extern "C" long long mesh_draft_attention_scratch(const MeshKvCache* c, const MeshDraftAttention* a) {
   using namespace mesh::draft;
   if (check(c, a)) return -1;
-  const int splits = splits_of(c, a);
-  if (splits <= 1) return 0;
-  return (long long)c->B * c->kv_heads * tiles_of(c, a) * splits * ROWS * (c->head_dim + 2);
+  const int shares = shares_of(c, a);
+  if (shares <= 1) return 0;
+  return 2ll * shares * ROWS * (c->head_dim + 2);
 }
 
 extern "C" int mesh_draft_attention(const MeshKvCache* c, const MeshDraftAttention* a, void* stream) {
@@ -596,7 +742,7 @@ extern "C" int mesh_draft_attention(const MeshKvCache* c, const MeshDraftAttenti
   using namespace mesh::draft;
   if (int rc = check(c, a)) return rc;
   if (c->B == 0 || a->T == 0) return 0;
-  if ((long long)c->B * c->kv_heads > 65535) return set_error(-2, "draft_attention: more than 65535 sequences times KV heads");
+  if ((long long)c->B * c->kv_heads * tiles_of(c, a) > 0x7fffffff) return set_error(-2, "draft_attention: too many rows for one call");
   if (((uintptr_t)a->q % 2) || ((uintptr_t)a->out % 4) || a->o_sb % 2 || a->o_st % 2)
     return set_error(-2, "draft_attention: rows of the output must start on a multiple of 4 bytes");
   Args p;
@@ -606,14 +752,13 @@ extern "C" int mesh_draft_attention(const MeshKvCache* c, const MeshDraftAttenti
   p.k = (const uint8_t*)c->k; p.v = (const uint8_t*)c->v; p.k_scale = c->k_scale; p.v_scale = c->v_scale;
   p.pos = a->pos; p.counts = a->counts; p.visible = a->visible;
   p.B = c->B; p.T = a->T; p.q_heads = a->q_heads; p.kv_heads = c->kv_heads; p.max_seq = c->max_seq; p.window = a->window;
-  p.splits = splits_of(c, a);
   p.tiles = tiles_of(c, a);
+  p.shares = shares_of(c, a);
   p.scale_log2 = a->scale * 1.4426950408889634f;
-  if (p.splits > 1) {
-    if (!a->scratch) return set_error(-2, "draft_attention: no scratch memory");
-    const long long items = (long long)c->B * c->kv_heads * p.tiles * p.splits;
-    p.part = a->scratch;
-    p.part_ml = a->scratch + items * ROWS * c->head_dim;
+  if (p.shares > 1) {
+    if (!a->scratch || (uintptr_t)a->scratch % 16) return set_error(-2, "draft_attention: scratch memory must be given and start on a multiple of 16 bytes");
+    p.part = (float4*)a->scratch;
+    p.part_ml = (float2*)(a->scratch + 2ll * p.shares * ROWS * c->head_dim);
   }
   switch (c->head_dim * 2 + (c->bits == 8)) {
     case 128: return run<64, false>(p, stream);
