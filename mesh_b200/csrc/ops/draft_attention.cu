@@ -15,15 +15,7 @@
 // 2^8..2^9 (what is smaller than 2^-32 of that is lost, less than the products' own rounding in fp32).  w is multiplied
 // by 2^14 first (in m), so that fp16 holds it down to 2^-38; its rounding to 11 bits is an eighth of bf16's.  With a bf16 cache
 // queries and values are bf16 as they are and w is rounded to bf16, half a step of the result's own type.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-#include <cuda_runtime.h>
-#include <math_constants.h>
-#include <atomic>
-#include <cstring>
-#include "draft_api.h"
-#include "../device/ptx.cuh"
-#include "../runtime/host_common.h"
+#include "draft_attention.cuh"
 
 namespace mesh {
 namespace draft {
@@ -31,26 +23,6 @@ namespace draft {
 constexpr int ROWS = 16;              // query rows of a tile
 constexpr int KEYS = 16;              // keys of a block
 
-struct Args {
-  const __nv_bfloat16* q; __nv_bfloat16* out; long long q_sb, q_st, o_sb, o_st;
-  const uint8_t* k; const uint8_t* v; const float* k_scale; const float* v_scale;
-  const int* pos; const int* counts; const long long* visible;
-  int B, T, q_heads, kv_heads, max_seq, window, tiles;
-  float scale_log2;                   // scale * log2(e): exponentials are powers of two
-  float4* part; float2* part_ml;      // two slots per CTA: the output as the fragments lie, and {m, l} of the rows
-  int shares;                         // CTAs of the attention kernel
-};
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float lg2(float x) {
-  float y;
-  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -70,92 +42,6 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-
-// Two codes as fp16: the bytes of x (already code + 128) that `sel` puts under the exponent of 1024, minus 1152.
-__device__ __forceinline__ uint32_t codes2(uint32_t x, uint32_t sel) {
-  const uint32_t t = __byte_perm(x, 0x64646464u, sel);
-  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&t), __half2half2(__ushort_as_half(0x6480)));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-
-__device__ __forceinline__ uint32_t pack16(bool half, float lo, float hi) {
-  if (half) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-// What the rows of a sequence see.
-struct Seq {
-  int pos, count, lo, hi;             // keys of any row: slots [lo, hi)
-};
-__device__ __forceinline__ Seq sequence(const Args& a, int b) {
-  Seq s;
-  s.pos = min(max(__ldg(a.pos + b), 0), a.max_seq);
-  s.count = a.counts ? min(__ldg(a.counts + b), a.T) : a.T;
-  s.hi = min(s.pos + max(s.count, 0), a.max_seq);
-  s.lo = a.window > 0 ? max(0, s.pos - a.window + 1) : 0;          // the root's; its descendants see less
-  return s;
-}
-
-// How the work is cut.  Sequence b has `rows` query rows per KV head in `tiles` tiles and `units` units of keys; its items follow
-// one another, KV head by KV head, tile by tile.
-struct Load {
-  Seq s; int tiles, units; long long work;
-};
-__device__ __forceinline__ Load load_of(const Args& a, int b, int unit) {
-  Load l;
-  l.s = sequence(a, b);
-  const int rows = max(l.s.count, 0) * (a.q_heads / a.kv_heads);
-  l.tiles = (rows + ROWS - 1) / ROWS;
-  l.units = max(1, (l.s.hi - l.s.lo + unit - 1) / unit);   // rows that see nothing are written too
-  l.work = (long long)l.tiles * l.units * a.kv_heads;
-  return l;
-}
-// Work of all sequences before b, and of all; by a whole warp.
-__device__ __forceinline__ void work_before(const Args& a, int unit, int b, long long& before, long long& total) {
-  const int lane = threadIdx.x & 31;
-  long long lo = 0, all = 0;
-  for (int i = lane; i < a.B; i += 32) {
-    const long long w = load_of(a, i, unit).work;
-    all += w;
-    if (i < b) lo += w;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    lo += __shfl_xor_sync(0xffffffffu, lo, o);
-    all += __shfl_xor_sync(0xffffffffu, all, o);
-  }
-  before = lo;
-  total = all;
-}
-// The sequence that unit w of the work belongs to, and the work before it; by a whole warp.  w < total.
-__device__ __forceinline__ int sequence_of(const Args& a, int unit, long long w, long long& before) {
-  const int lane = threadIdx.x & 31;
-  before = 0;
-  for (int i0 = 0; i0 < a.B; i0 += 32) {
-    const long long mine = i0 + lane < a.B ? load_of(a, i0 + lane, unit).work : 0;
-    long long upto = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long v = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += v;
-    }
-    const uint32_t past = __ballot_sync(0xffffffffu, before + upto > w);
-    if (past) {
-      const int l = __ffs(past) - 1;
-      before += __shfl_sync(0xffffffffu, upto - mine, l);
-      return i0 + l;
-    }
-    before += __shfl_sync(0xffffffffu, upto, 31);
-  }
-  return a.B;
-}
-// CTA c of n has units [c total / n, (c + 1) total / n).
-__device__ __forceinline__ long long share_begin(long long c, long long n, long long total) { return c * total / n; }
-__device__ __forceinline__ long long share_of(long long w, long long n, long long total) { return ((w + 1) * n - 1) / total; }
 
 template <int HD, bool Q8>
 struct Cfg {
@@ -208,8 +94,7 @@ __global__ void __launch_bounds__(Cfg<HD, Q8>::WARPS * 32, 1) attention_kernel(c
   uint4* q_s = reinterpret_cast<uint4*>(smem);            // [k step][lane]: operand A of the scores
   __shared__ float unit_s[ROWS], weight_s[C::WARPS][ROWS], m_s[ROWS], l_s[ROWS];
   __shared__ float2 ml_s[C::WARPS][ROWS];
-  __shared__ long long start_s[2];
-  __shared__ int seq_s;
+  __shared__ Walk walk_s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = lane >> 2, t4 = lane & 3;
   uint8_t* ring = smem + C::QB + warp * (STAGES * C::STAGE);
   const uint32_t ring_u = smem_u32(ring);
@@ -217,33 +102,13 @@ __global__ void __launch_bounds__(Cfg<HD, Q8>::WARPS * 32, 1) attention_kernel(c
   griddep_wait();
   griddep_launch_dependents();                            // not before: the joining kernel reads lengths before its own wait
 
-  if (warp == 0) {
-    long long before, total, ignore;
-    work_before(a, C::UNIT, 0, ignore, total);
-    const long long shares = min((long long)a.shares, total);
-    if (lane == 0) { start_s[0] = 0; start_s[1] = 0; }
-    if (blockIdx.x < shares) {
-      const long long w0 = share_begin(blockIdx.x, shares, total), w1 = share_begin(blockIdx.x + 1, shares, total);
-      const int b = sequence_of(a, C::UNIT, w0, before);
-      if (lane == 0) { start_s[0] = w0 - before; start_s[1] = w1 - before; seq_s = b; }
-    }
-  }
+  if (warp == 0) begin_walk(a, &walk_s);
   __syncthreads();
-  long long at = start_s[0], stop = start_s[1];           // relative to the first unit of sequence b
-  int b = seq_s;
-  for (bool first_item = true; at < stop; first_item = false) {
-  Load load = load_of(a, b, C::UNIT);
-  while (at >= load.work) {
-    at -= load.work;
-    stop -= load.work;
-    load = load_of(a, ++b, C::UNIT);
-  }
-  const Seq s = load.s;
-  const int item = (int)(at / load.units), hk = item / load.tiles, tile = item % load.tiles;
-  const int u0 = (int)(at % load.units), u1 = (int)min((long long)load.units, u0 + stop - at);
-  at += u1 - u0;
-  const int n_rows = min(s.count * G - tile * ROWS, ROWS);
-  const int k_lo = min(s.lo + u0 * C::UNIT, s.hi), k_hi = min(s.lo + u1 * C::UNIT, s.hi);
+  Walk walk = walk_s;
+  Stretch x;
+  while (next(a, walk, x)) {
+  const Seq s = x.s;
+  const int b = x.b, hk = x.hk, tile = x.tile, n_rows = x.n_rows, k_lo = x.k_lo, k_hi = x.k_hi;
   const int blocks = (k_hi - k_lo + KEYS - 1) / KEYS;
   const long long base = ((long long)b * a.kv_heads + hk) * a.max_seq;
   const uint8_t* kp = a.k + base * RB;
@@ -531,13 +396,13 @@ __global__ void __launch_bounds__(Cfg<HD, Q8>::WARPS * 32, 1) attention_kernel(c
     l_s[r] = ll;
   }
   __syncthreads();
-  const bool whole = u1 - u0 == load.units;
-  const long long slot = 2 * (long long)blockIdx.x + (first_item ? 0 : 1);
+  const bool whole = x.whole;
+  const long long slot = x.slot;
   __nv_bfloat16* row_s = reinterpret_cast<__nv_bfloat16*>(smem);          // the queries' memory and, after a barrier, more
   float4 sum[(NT * 32 + C::WARPS * 32 - 1) / (C::WARPS * 32)];
 #pragma unroll
-  for (int x = 0; x < NT / C::WARPS; ++x) {
-    const int i = x * C::WARPS + warp;
+  for (int y = 0; y < NT / C::WARPS; ++y) {
+    const int i = y * C::WARPS + warp;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < C::WARPS; ++w) {
@@ -545,7 +410,7 @@ __global__ void __launch_bounds__(Cfg<HD, Q8>::WARPS * 32, 1) attention_kernel(c
       const float4 v = o_s[(w * NT + i) * 32 + lane];
       acc.x += w0 * v.x; acc.y += w0 * v.y; acc.z += w1 * v.z; acc.w += w1 * v.w;
     }
-    sum[x] = acc;
+    sum[y] = acc;
     if (!whole) a.part[(slot * NT + i) * 32 + lane] = acc;
   }
   if (!whole) {
@@ -554,13 +419,13 @@ __global__ void __launch_bounds__(Cfg<HD, Q8>::WARPS * 32, 1) attention_kernel(c
     __syncthreads();
     const float i0 = l_s[n] == 0.f ? 0.f : 1.f / l_s[n], i1 = l_s[n + 8] == 0.f ? 0.f : 1.f / l_s[n + 8];
 #pragma unroll
-    for (int x = 0; x < NT / C::WARPS; ++x) {
-      const int i = x * C::WARPS + warp;
+    for (int y = 0; y < NT / C::WARPS; ++y) {
+      const int i = y * C::WARPS + warp;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int col = column<VW>(i, 2 * t4 + e);
-        row_s[n * C::OUT_PITCH + col] = __float2bfloat16_rn((e ? sum[x].y : sum[x].x) * i0);
-        row_s[(n + 8) * C::OUT_PITCH + col] = __float2bfloat16_rn((e ? sum[x].w : sum[x].z) * i1);
+        row_s[n * C::OUT_PITCH + col] = __float2bfloat16_rn((e ? sum[y].y : sum[y].x) * i0);
+        row_s[(n + 8) * C::OUT_PITCH + col] = __float2bfloat16_rn((e ? sum[y].w : sum[y].z) * i1);
       }
     }
     __syncthreads();
@@ -585,20 +450,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = lane >> 2, t4 = lane & 3, G = a.q_heads / a.kv_heads;
   const int i = blockIdx.y, tile = blockIdx.x % a.tiles, hk = blockIdx.x / a.tiles % a.kv_heads, b = blockIdx.x / a.tiles / a.kv_heads;
   // the lengths are older than the kernel before this one, which lets this one start when it has seen them
-  if (warp == 0) {
-    const Load load = load_of(a, b, C::UNIT);
-    long long before, total;
-    work_before(a, C::UNIT, b, before, total);
-    if (lane == 0) {
-      c_s[0] = c_s[1] = 0;
-      if (tile < load.tiles) {
-        const long long shares = min((long long)a.shares, total), w = before + ((long long)hk * load.tiles + tile) * load.units;
-        c_s[0] = share_of(w, shares, total);
-        c_s[1] = share_of(w + load.units - 1, shares, total);
-        c_s[2] = share_begin(c_s[0], shares, total) >= w ? 0 : 1;        // whether the item is the first of its first share
-      }
-    }
-  }
+  if (warp == 0) shares_of_item(a, b, hk, tile, c_s);
   __syncthreads();
   const long long c0 = c_s[0], c1 = c_s[1];
   const int odd = (int)c_s[2];
@@ -660,24 +512,22 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args 
     a.out[b * a.o_sb + (r / G) * a.o_st + (long long)(hk * G + r % G) * HD + column<C::VW>(i, c)] = __float2bfloat16_rn(ll == 0.f ? 0.f : sum / ll);
 }
 
-static int tiles_of(const MeshKvCache* c, const MeshDraftAttention* a) {
-  return (a->T * (a->q_heads / c->kv_heads) + ROWS - 1) / ROWS;
-}
+// The kernel for many rows, with tiles of 128, from 17 query rows per KV head on.
+static bool wide(const MeshKvCache* c, const MeshDraftAttention* a) { return a->T * (a->q_heads / c->kv_heads) > ROWS; }
 
-template <int HD, bool Q8> static int unit_of() { return Cfg<HD, Q8>::UNIT; }
-static int unit_of(const MeshKvCache* c) {
-  const bool q8 = c->bits == 8;
-  return c->head_dim == 64 ? (q8 ? unit_of<64, true>() : unit_of<64, false>()) : c->head_dim == 128 ? (q8 ? unit_of<128, true>() : unit_of<128, false>())
-                           : (q8 ? unit_of<256, true>() : unit_of<256, false>());
-}
-
-// CTAs: one per SM, or per unit of work where the longest sequences have fewer.
-static int shares_of(const MeshKvCache* c, const MeshDraftAttention* a) {
+static void cut(const MeshKvCache* c, const MeshDraftAttention* a, Args& p) {
+  const bool w = wide(c, a), q8 = c->bits == 8;
+  p.rows = w ? WIDE_ROWS : ROWS;
+  p.unit = w ? WIDE_UNIT
+             : c->head_dim == 64 ? (q8 ? Cfg<64, true>::UNIT : Cfg<64, false>::UNIT)
+             : c->head_dim == 128 ? (q8 ? Cfg<128, true>::UNIT : Cfg<128, false>::UNIT) : (q8 ? Cfg<256, true>::UNIT : Cfg<256, false>::UNIT);
+  p.tiles = (a->T * (a->q_heads / c->kv_heads) + p.rows - 1) / p.rows;
+  // CTAs: one per SM, or per unit of work where the longest sequences have fewer
   long long keys = c->max_seq;
   if (a->window > 0 && (long long)a->window + a->T < keys) keys = (long long)a->window + a->T;
-  const long long units = (long long)c->B * c->kv_heads * tiles_of(c, a) * ((keys + unit_of(c) - 1) / unit_of(c));
+  const long long units = (long long)c->B * c->kv_heads * p.tiles * ((keys + p.unit - 1) / p.unit);
   const long long most = a->splits > 0 ? a->splits : sm_count();
-  return (int)(units < most ? units : most);
+  p.shares = (int)(units < most ? units : most);
 }
 
 static int check(const MeshKvCache* c, const MeshDraftAttention* a) {
@@ -691,22 +541,6 @@ static int check(const MeshKvCache* c, const MeshDraftAttention* a) {
   if (!(a->scale > 0.f)) return set_error(-2, "draft_attention: scale must be positive");
   if (((uintptr_t)c->k | (uintptr_t)c->v) % 16) return set_error(-2, "draft_attention: the cache must start on a multiple of 16 bytes");
   return 0;
-}
-
-template <class... P>
-static cudaError_t launch(void (*kern)(P...), dim3 grid, int threads, int smem, void* stream, const Args& a) {
-  cudaLaunchConfig_t cfg;
-  memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = (cudaStream_t)stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, a);
 }
 
 template <int HD, bool Q8> constexpr bool NT_OK = HD / 8 % Cfg<HD, Q8>::WARPS == 0 && ROWS * Cfg<HD, Q8>::OUT_PITCH * 2 <= Cfg<HD, Q8>::SMEM;
@@ -732,9 +566,9 @@ static int run(const Args& p, void* stream) {
 extern "C" long long mesh_draft_attention_scratch(const MeshKvCache* c, const MeshDraftAttention* a) {
   using namespace mesh::draft;
   if (check(c, a)) return -1;
-  const int shares = shares_of(c, a);
-  if (shares <= 1) return 0;
-  return 2ll * shares * ROWS * (c->head_dim + 2);
+  Args p;
+  cut(c, a, p);
+  return p.shares <= 1 ? 0 : 2ll * p.shares * p.rows * (c->head_dim + 2);
 }
 
 extern "C" int mesh_draft_attention(const MeshKvCache* c, const MeshDraftAttention* a, void* stream) {
@@ -742,7 +576,6 @@ extern "C" int mesh_draft_attention(const MeshKvCache* c, const MeshDraftAttenti
   using namespace mesh::draft;
   if (int rc = check(c, a)) return rc;
   if (c->B == 0 || a->T == 0) return 0;
-  if ((long long)c->B * c->kv_heads * tiles_of(c, a) > 0x7fffffff) return set_error(-2, "draft_attention: too many rows for one call");
   if (((uintptr_t)a->q % 2) || ((uintptr_t)a->out % 4) || a->o_sb % 2 || a->o_st % 2)
     return set_error(-2, "draft_attention: rows of the output must start on a multiple of 4 bytes");
   Args p;
@@ -752,14 +585,16 @@ extern "C" int mesh_draft_attention(const MeshKvCache* c, const MeshDraftAttenti
   p.k = (const uint8_t*)c->k; p.v = (const uint8_t*)c->v; p.k_scale = c->k_scale; p.v_scale = c->v_scale;
   p.pos = a->pos; p.counts = a->counts; p.visible = a->visible;
   p.B = c->B; p.T = a->T; p.q_heads = a->q_heads; p.kv_heads = c->kv_heads; p.max_seq = c->max_seq; p.window = a->window;
-  p.tiles = tiles_of(c, a);
-  p.shares = shares_of(c, a);
+  p.status = (Status*)a->status;
+  cut(c, a, p);
+  if ((long long)c->B * c->kv_heads * p.tiles > 0x7fffffff) return set_error(-2, "draft_attention: too many rows for one call");
   p.scale_log2 = a->scale * 1.4426950408889634f;
   if (p.shares > 1) {
     if (!a->scratch || (uintptr_t)a->scratch % 16) return set_error(-2, "draft_attention: scratch memory must be given and start on a multiple of 16 bytes");
     p.part = (float4*)a->scratch;
-    p.part_ml = (float2*)(a->scratch + 2ll * p.shares * ROWS * c->head_dim);
+    p.part_ml = (float2*)(a->scratch + 2ll * p.shares * p.rows * c->head_dim);
   }
+  if (wide(c, a)) return run_wide(p, c->head_dim, c->bits == 8, stream);
   switch (c->head_dim * 2 + (c->bits == 8)) {
     case 128: return run<64, false>(p, stream);
     case 129: return run<64, true>(p, stream);

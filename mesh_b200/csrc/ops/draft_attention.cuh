@@ -1,0 +1,209 @@
+// What the two kernels for the attention of drafts have in common: their arguments, what a sequence's rows see, and how the work is
+// cut into shares.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math_constants.h>
+#include <atomic>
+#include <cstring>
+#include "draft_api.h"
+#include "../device/ptx.cuh"
+#include "../runtime/host_common.h"
+
+namespace mesh {
+namespace draft {
+
+struct Args {
+  const __nv_bfloat16* q; __nv_bfloat16* out; long long q_sb, q_st, o_sb, o_st;
+  const uint8_t* k; const uint8_t* v; const float* k_scale; const float* v_scale;
+  const int* pos; const int* counts; const long long* visible;
+  int B, T, q_heads, kv_heads, max_seq, window;
+  int rows, unit, tiles;              // query rows of a tile, keys of a unit of work, most tiles of a (sequence, KV head)
+  float scale_log2;                   // scale * log2(e): exponentials are powers of two
+  float4* part; float2* part_ml;      // two slots per CTA: the output as its threads hold it, and {m, l} of the rows
+  int shares;                         // CTAs of the attention kernel
+  Status* status;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Two codes as fp16: the bytes of x (already code + 128) that `sel` puts under the exponent of 1024, minus 1152.
+__device__ __forceinline__ uint32_t codes2(uint32_t x, uint32_t sel) {
+  const uint32_t t = __byte_perm(x, 0x64646464u, sel);
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&t), __half2half2(__ushort_as_half(0x6480)));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+__device__ __forceinline__ uint32_t pack16(bool half, float lo, float hi) {
+  if (half) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// What the rows of a sequence see.
+struct Seq {
+  int pos, count, lo, hi;             // keys of any row: slots [lo, hi)
+};
+__device__ __forceinline__ Seq sequence(const Args& a, int b) {
+  Seq s;
+  s.pos = min(max(__ldg(a.pos + b), 0), a.max_seq);
+  s.count = a.counts ? min(__ldg(a.counts + b), a.T) : a.T;
+  s.hi = min(s.pos + max(s.count, 0), a.max_seq);
+  s.lo = a.window > 0 ? max(0, s.pos - a.window + 1) : 0;          // the root's; its descendants see less
+  return s;
+}
+
+// How the work is cut.  Sequence b has `rows` query rows per KV head in `tiles` tiles and `units` units of keys; its items follow
+// one another, KV head by KV head, tile by tile.
+struct Load {
+  Seq s; int tiles, units; long long work;
+};
+__device__ __forceinline__ Load load_of(const Args& a, int b) {
+  Load l;
+  l.s = sequence(a, b);
+  const int rows = max(l.s.count, 0) * (a.q_heads / a.kv_heads);
+  l.tiles = (rows + a.rows - 1) / a.rows;
+  l.units = max(1, (l.s.hi - l.s.lo + a.unit - 1) / a.unit);   // rows that see nothing are written too
+  l.work = (long long)l.tiles * l.units * a.kv_heads;
+  return l;
+}
+// Work of all sequences before b, and of all; by a whole warp.
+__device__ __forceinline__ void work_before(const Args& a, int b, long long& before, long long& total) {
+  const int lane = threadIdx.x & 31;
+  long long lo = 0, all = 0;
+  for (int i = lane; i < a.B; i += 32) {
+    const long long w = load_of(a, i).work;
+    all += w;
+    if (i < b) lo += w;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    lo += __shfl_xor_sync(0xffffffffu, lo, o);
+    all += __shfl_xor_sync(0xffffffffu, all, o);
+  }
+  before = lo;
+  total = all;
+}
+// The sequence that unit w of the work belongs to, and the work before it; by a whole warp.  w < total.
+__device__ __forceinline__ int sequence_of(const Args& a, long long w, long long& before) {
+  const int lane = threadIdx.x & 31;
+  before = 0;
+  for (int i0 = 0; i0 < a.B; i0 += 32) {
+    const long long mine = i0 + lane < a.B ? load_of(a, i0 + lane).work : 0;
+    long long upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    const uint32_t past = __ballot_sync(0xffffffffu, before + upto > w);
+    if (past) {
+      const int l = __ffs(past) - 1;
+      before += __shfl_sync(0xffffffffu, upto - mine, l);
+      return i0 + l;
+    }
+    before += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return a.B;
+}
+// CTA c of n has units [c total / n, (c + 1) total / n).
+__device__ __forceinline__ long long share_begin(long long c, long long n, long long total) { return c * total / n; }
+__device__ __forceinline__ long long share_of(long long w, long long n, long long total) { return ((w + 1) * n - 1) / total; }
+
+// The stretches of a CTA's share, each within one item.  `begin` by warp 0, then a barrier; `next` by any thread that keeps a Walk.
+struct Stretch {
+  Seq s; int b, hk, tile, n_rows;     // n_rows: query rows of the tile that exist
+  int k_lo, k_hi;                     // slots
+  bool whole;                         // all of the item: its result is final
+  long long slot;                     // where it goes otherwise
+};
+struct Walk {
+  long long at, stop;                 // units, relative to the first of sequence b
+  int b; bool first;
+};
+__device__ __forceinline__ void begin_walk(const Args& a, Walk* w) {
+  long long before, total, none;
+  work_before(a, 0, none, total);
+  const long long shares = min((long long)a.shares, total);
+  if ((threadIdx.x & 31) == 0) { w->at = w->stop = 0; w->b = 0; w->first = true; }
+  if (blockIdx.x < shares) {
+    const long long w0 = share_begin(blockIdx.x, shares, total), w1 = share_begin(blockIdx.x + 1, shares, total);
+    const int b = sequence_of(a, w0, before);
+    if ((threadIdx.x & 31) == 0) { w->at = w0 - before; w->stop = w1 - before; w->b = b; }
+  }
+}
+__device__ __forceinline__ bool next(const Args& a, Walk& w, Stretch& x) {
+  if (w.at >= w.stop) return false;
+  Load load = load_of(a, w.b);
+  while (w.at >= load.work) {
+    w.at -= load.work;
+    w.stop -= load.work;
+    load = load_of(a, ++w.b);
+  }
+  const int item = (int)(w.at / load.units);              // the items of a sequence are fewer than 2^31
+  const int u0 = (int)(w.at - (long long)item * load.units), u1 = (int)min((long long)load.units, u0 + w.stop - w.at);
+  x.s = load.s;
+  x.b = w.b;
+  x.hk = item / load.tiles;
+  x.tile = item % load.tiles;
+  x.n_rows = min(load.s.count * (a.q_heads / a.kv_heads) - x.tile * a.rows, a.rows);
+  x.k_lo = min(load.s.lo + u0 * a.unit, load.s.hi);
+  x.k_hi = min(load.s.lo + u1 * a.unit, load.s.hi);
+  x.whole = u1 - u0 == load.units;
+  x.slot = 2 * (long long)blockIdx.x + (w.first ? 0 : 1);
+  w.at += u1 - u0;
+  w.first = false;
+  return true;
+}
+
+// The shares that an item was cut into, by warp 0: c[0] .. c[1], and whether it is not the first stretch of the first of them
+// (equal shares: not cut, or there is no such item).
+__device__ __forceinline__ void shares_of_item(const Args& a, int b, int hk, int tile, long long (&c)[3]) {
+  const Load load = load_of(a, b);
+  long long before, total;
+  work_before(a, b, before, total);
+  if ((threadIdx.x & 31) == 0) {
+    c[0] = c[1] = c[2] = 0;
+    if (tile < load.tiles) {
+      const long long shares = min((long long)a.shares, total), w = before + ((long long)hk * load.tiles + tile) * load.units;
+      c[0] = share_of(w, shares, total);
+      c[1] = share_of(w + load.units - 1, shares, total);
+      c[2] = share_begin(c[0], shares, total) >= w ? 0 : 1;
+    }
+  }
+}
+
+template <class... P>
+static cudaError_t launch(void (*kern)(P...), dim3 grid, int threads, int smem, void* stream, const Args& a) {
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = (cudaStream_t)stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, a);
+}
+
+// The kernel for many query rows (draft_attention_wide.cu): rows of a tile, keys of a unit, and the call.
+constexpr int WIDE_ROWS = 128, WIDE_UNIT = 128;
+int run_wide(const Args& p, int head_dim, bool q8, void* stream);
+
+}  // namespace draft
+}  // namespace mesh

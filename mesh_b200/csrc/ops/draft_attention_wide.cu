@@ -1,0 +1,582 @@
+// Attention of drafts with many query rows (more than 16 drafts times heads of a group) on the 5th-generation tensor cores.
+//
+// A tile is 128 query rows of one (sequence, KV head); a CTA goes through its stretches of 128-key blocks (how the work is cut and
+// the formulas: draft_attention.cuh, draft_attention.cu).  Warps 0-3: softmax, a thread per query row.  Warps 4-11: keys and
+// values, loaded into registers ahead of their turn, widened (8-bit codes to fp16) and stored to shared memory in the
+// 128-byte swizzle of the operands.  Warp 12: the products S = Q K^T and O += P V by one elected lane, S of the next block
+// before P V of this one; S is double-buffered in tensor memory, P (16 bits) overwrites the first half of its S and is
+// operand A from there, O stays in tensor memory and is rescaled only when a row's maximum has grown by more than 2^8.
+//
+// Codes are widened once per 128 rows, in registers: as operands of a product in 8 bits the queries and probabilities would have to be
+// rounded to 8 bits too.  Two passes over a row's scores instead of holding all 128: 13 warps with 152 registers each
+// then fit, so the widening has eight warps of its own.  With heads of 256 one tile of keys and one of values fill shared
+// memory beside the queries; the store of one runs under the product of the other.
+#include "draft_attention.cuh"
+
+namespace mesh {
+namespace draft {
+namespace {
+
+constexpr int TT = WIDE_ROWS;
+constexpr int SOFT = 128, LOADERS = 256, THREADS = SOFT + LOADERS + 32;
+constexpr int SCALES = 4;                                  // blocks whose scales are kept: more than a loader is ahead of the softmax
+
+template <int HD, bool Q8>
+struct Wide {
+  static constexpr int TILE = TT * HD * 2;
+  static constexpr int STAGES = HD == 256 ? 1 : 2;
+  static constexpr int RB = Q8 ? HD : 2 * HD, NC = RB / 16;           // bytes and 16-byte pieces of a stored row
+  static constexpr int VPT = TT * NC / LOADERS;            // pieces of a loader thread per tile
+  static constexpr int DEPTH = VPT >= 16 ? 1 : VPT >= 8 ? 2 : 4;      // tiles in registers
+  static constexpr int N_BARS = 1 + 4 * STAGES + 2 + 2 + 1 + SCALES;
+  static constexpr int SCALE_BYTES = Q8 ? SCALES * 3 * TT * 4 : 0;
+  static constexpr int SMEM = (1 + 2 * STAGES) * TILE + SCALE_BYTES + 8 * N_BARS + 64 + 1024;
+};
+
+// two fp32 at a time
+struct F2 { unsigned long long v; };
+__device__ __forceinline__ F2 f2(float lo, float hi) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack(F2 a, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(a.v)); }
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+
+__device__ __forceinline__ int blocks_of(const Stretch& x) { return (x.k_hi - x.k_lo + TT - 1) / TT; }
+// Whether some row may not see some key of the block.
+__device__ __forceinline__ bool masked_block(const Args& a, const Stretch& x, int slot0) {
+  return (a.window > 0 && slot0 < x.s.pos + 64 - a.window) || slot0 + TT > min(x.s.pos, x.k_hi);
+}
+// Bits of the slots first .. first + 32 that a row sees.
+__device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; }
+__device__ __forceinline__ uint32_t seen(const Stretch& x, int row_lo, unsigned long long vis, int first) {
+  const int d = first - x.s.pos;
+  const uint32_t past = below(-d) & ~below(row_lo - first);
+  const uint32_t drafts = d >= 64 ? 0u : d >= 0 ? (uint32_t)(vis >> d) : d > -32 ? (uint32_t)(vis << -d) : 0u;
+  return (past | drafts) & below(x.k_hi - first);
+}
+__device__ __forceinline__ bool not_finite(uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; }
+__device__ __forceinline__ uint32_t finite_or_zero(uint32_t w) {
+  return ((w & 0x7f80u) == 0x7f80u ? 0u : w & 0xffffu) | ((w & 0x7f800000u) == 0x7f800000u ? 0u : w & 0xffff0000u);
+}
+
+template <int HD, bool Q8>
+__global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant__ Args a) {
+  using C = Wide<HD, Q8>;
+  constexpr int STAGES = C::STAGES, VPT = C::VPT, NC = C::NC;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
+  const uint32_t sQ = base, sK = sQ + C::TILE, sV = sK + STAGES * C::TILE, sScale = sV + STAGES * C::TILE, bars = sScale + C::SCALE_BYTES;
+  float* scale_s = reinterpret_cast<float*>(gen + (sScale - base));        // [buffer]{key scale, lg2 of the value scale, value scale}[key]
+  auto bar = [&](int i) { return bars + 8u * i; };
+  constexpr int Q_FULL = 0, K_FULL = 1, K_EMPTY = K_FULL + STAGES, V_FULL = K_EMPTY + STAGES, V_EMPTY = V_FULL + STAGES,
+                S_FULL = V_EMPTY + STAGES, P_FULL = S_FULL + 2, O_DONE = P_FULL + 2, SC_FULL = O_DONE + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen + (bars - base) + 8 * C::N_BARS);
+  volatile int* abort_smem = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* spoilt_s = reinterpret_cast<volatile int*>(tmem_slot + 2);     // [4]: stretch + 1 whose values had to be cleaned
+  __shared__ Walk walk_s;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = a.q_heads / a.kv_heads;
+
+  if (threadIdx.x == 0) {
+    mbar_init(bar(Q_FULL), SOFT);
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(bar(K_FULL + s), LOADERS);
+      mbar_init(bar(V_FULL + s), LOADERS);
+      mbar_init(bar(K_EMPTY + s), 1);
+      mbar_init(bar(V_EMPTY + s), 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(bar(S_FULL + s), 1);
+      mbar_init(bar(P_FULL + s), SOFT);
+    }
+    mbar_init(bar(O_DONE), 1);
+    for (int s = 0; s < SCALES; ++s) mbar_init(bar(SC_FULL + s), LOADERS);
+    *abort_smem = 0;
+    for (int s = 0; s < 4; ++s) spoilt_s[s] = 0;
+    fence_mbar_init();
+  }
+  if (warp == 12) {
+    tmem_alloc<1>(smem_u32(tmem_slot), 512);
+    tmem_relinquish<1>();
+  }
+  griddep_wait();
+  griddep_launch_dependents();                            // not before: the joining kernel reads lengths before its own wait
+  if (warp == 0) begin_walk(a, &walk_s);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+  Walk walk = walk_s;
+  Stretch x;
+  bool ok = true;
+
+  if (warp >= 4 && warp < 12) {
+    // ------------------------------------------------------------------ keys and values
+    // Per stretch, in the order the products take them: K0 K1 V0 K2 V1 ...  `load` fetches the next tile into a set of
+    // registers, `store` puts the oldest set into its place when that is free.
+    const int lt = threadIdx.x - SOFT;
+    uint4 raw[C::DEPTH][VPT];
+    float scale[C::DEPTH];
+    int what[C::DEPTH];                                   // 0 nothing, 1 key, 2 value, 3 value to be cleaned
+    int stretch_of[C::DEPTH];
+    int blocks = 0, kj = 0, vj = 0, stretch = -1;
+    bool more = true;
+    auto load = [&](int d) {
+      what[d] = 0;
+      while (more && kj >= blocks && vj >= blocks) {
+        more = next(a, walk, x);
+        ++stretch;
+        kj = vj = 0;
+        blocks = more ? blocks_of(x) : 0;
+      }
+      if (!more) return;
+      const bool key = kj < blocks && kj <= vj + 1;
+      const int j = key ? kj++ : vj++, slot0 = x.k_lo + j * TT, rows = min(x.k_hi - slot0, TT);
+      const long long at = ((long long)x.b * a.kv_heads + x.hk) * a.max_seq + slot0;
+      const uint4* src = reinterpret_cast<const uint4*>((key ? a.k : a.v) + at * C::RB) + lt;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        raw[d][i] = make_uint4(0, 0, 0, 0);               // behind the last slot: what a hidden row holds is not read
+        if ((i * LOADERS + lt) / NC < rows) raw[d][i] = __ldg(src + i * LOADERS);
+      }
+      if (Q8 && key) scale[d] = (lt & 127) < rows ? __ldg((lt < 128 ? a.k_scale : a.v_scale) + at + (lt & 127)) : 0.f;
+      what[d] = key ? 1 : !Q8 && masked_block(a, x, slot0) ? 3 : 2;
+      stretch_of[d] = stretch;
+    };
+    int nk = 0, nv = 0;                                   // tiles stored
+    auto store = [&](int d) {
+      const bool key = what[d] == 1;
+      const int n = key ? nk++ : nv++, s = n % STAGES;
+      if (n >= STAGES) ok = mbar_wait(bar((key ? K_EMPTY : V_EMPTY) + s), (n / STAGES - 1) & 1, abort_smem, a.status, SITE_SMEM_EMPTY);
+      if (!ok) return;
+      const uint32_t dst = (key ? sK : sV) + s * C::TILE - base;
+      bool spoilt = false;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const int idx = i * LOADERS + lt, r = idx / NC, c = idx % NC;
+        uint4 v = raw[d][i];
+        if (Q8) {
+          uint8_t* p = gen + dst + (c >> 2) * (TT * 128) + r * 128;
+          const uint32_t w[4] = {v.x ^ 0x80808080u, v.y ^ 0x80808080u, v.z ^ 0x80808080u, v.w ^ 0x80808080u};
+          const uint4 lo = make_uint4(codes2(w[0], 0x4140), codes2(w[0], 0x4342), codes2(w[1], 0x4140), codes2(w[1], 0x4342));
+          const uint4 hi = make_uint4(codes2(w[2], 0x4140), codes2(w[2], 0x4342), codes2(w[3], 0x4140), codes2(w[3], 0x4342));
+          // the eight lanes of a phase on eight different 16-byte banks: every other group of columns begins with its odd piece
+          const int odd = c >> 2 & 1, c0 = 2 * (c & 3);
+          *reinterpret_cast<uint4*>(p + (((c0 + odd) ^ (r & 7)) << 4)) = odd ? hi : lo;
+          *reinterpret_cast<uint4*>(p + (((c0 + 1 - odd) ^ (r & 7)) << 4)) = odd ? lo : hi;
+        } else {
+          if (what[d] == 3 && (not_finite(v.x) || not_finite(v.y) || not_finite(v.z) || not_finite(v.w))) {
+            // zero times a NaN or an infinity is not zero: hidden keys must not hold any.  Rows that see them get them at the end.
+            v = make_uint4(finite_or_zero(v.x), finite_or_zero(v.y), finite_or_zero(v.z), finite_or_zero(v.w));
+            spoilt = true;
+          }
+          *reinterpret_cast<uint4*>(gen + dst + (c >> 3) * (TT * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+        }
+      }
+      if (!Q8 && spoilt) spoilt_s[stretch_of[d] & 3] = stretch_of[d] + 1;
+      if (Q8 && key) {
+        float* sc = scale_s + (n % SCALES) * 3 * TT + (lt & 127);
+        if (lt < 128) {
+          sc[0] = scale[d];
+        } else {
+          sc[TT] = fmaxf(lg2(scale[d]), -60.f);
+          sc[2 * TT] = scale[d];
+        }
+        mbar_arrive(bar(SC_FULL + n % SCALES));
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(bar((key ? K_FULL : V_FULL) + s));
+    };
+#pragma unroll
+    for (int d = 0; d < C::DEPTH; ++d) load(d);
+    while (ok && what[0]) {
+#pragma unroll
+      for (int d = 0; d < C::DEPTH; ++d) {
+        if (ok && what[d]) {
+          store(d);
+          if (ok) load(d);
+        }
+      }
+    }
+  } else if (warp == 12) {
+    // ------------------------------------------------------------------ products (warp-uniform, one elected lane issues)
+    constexpr uint32_t half = Q8 ? (1u << 7) | (1u << 10) : 0u;              // operands in fp16 instead of bf16
+    constexpr uint32_t idesc_s = umma_idesc_bf16(TT, TT, 0, 0) & ~half, idesc_o = umma_idesc_bf16(TT, HD, 0, 1) & ~half;
+    const bool leader = elect_one();
+    const uint64_t dq0 = umma_smem_desc(sQ, 16, 1024), dk0 = umma_smem_desc(sK, 16, 1024), dv0 = umma_smem_desc(sV, TT * 128, 1024);
+    int n = 0, visit = 0;                                 // blocks and stretches done
+    auto issue_s = [&](int n) {
+      const int s = n % STAGES;
+      ok = mbar_wait_warp(bar(K_FULL + s), (n / STAGES) & 1, abort_smem, a.status, SITE_SMEM_FULL);
+      if (!ok) return;
+      tc_fence_after();
+      if (leader) {
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k) {
+          const int off = ((k / 4) * (TT * 128) + (k % 4) * 32) / 16;
+          umma_f16<1>(tmem + (n & 1) * 128, dq0 + off, dk0 + (uint32_t)(s * (C::TILE >> 4)) + off, idesc_s, k ? 1u : 0u);
+        }
+        umma_commit(bar(K_EMPTY + s));
+        umma_commit(bar(S_FULL + (n & 1)));
+      }
+      __syncwarp();
+    };
+    while (ok && next(a, walk, x)) {
+      const int blocks = blocks_of(x);
+      if (blocks == 0) continue;
+      ok = mbar_wait_warp(bar(Q_FULL), visit++ & 1, abort_smem, a.status, SITE_SMEM_FULL);
+      if (ok) issue_s(n);
+      for (int j = 0; ok && j < blocks; ++j, ++n) {
+        if (j + 1 < blocks) issue_s(n + 1);
+        const int s = n % STAGES;
+        if (ok) ok = mbar_wait_warp(bar(V_FULL + s), (n / STAGES) & 1, abort_smem, a.status, SITE_SMEM_FULL);
+        if (ok) ok = mbar_wait_warp(bar(P_FULL + (n & 1)), (n >> 1) & 1, abort_smem, a.status, SITE_TMEM_FULL);
+        if (!ok) break;
+        tc_fence_after();
+        if (leader) {
+#pragma unroll
+          for (int k = 0; k < TT / 16; ++k)
+            umma_f16_ts(tmem + 256, tmem + (n & 1) * 128 + k * 8, dv0 + (uint32_t)(s * (C::TILE >> 4)) + k * 128, idesc_o, (j | k) ? 1u : 0u);
+          umma_commit(bar(V_EMPTY + s));
+          umma_commit(bar(O_DONE));
+        }
+        __syncwarp();
+      }
+    }
+  } else if (warp < 4) {
+    // ------------------------------------------------------------------ softmax: thread = query row = TMEM lane
+    constexpr float LIFT = Q8 ? 6.f : 0.f;                // with the 2^8 that a reference may lag behind, w stays below 2^14
+    const int row = threadIdx.x;
+    const uint32_t lane_addr = tmem + ((uint32_t)(warp * 32) << 16);
+    int n = 0, stretch = -1;
+    while (ok && next(a, walk, x)) {
+      ++stretch;
+      const int blocks = blocks_of(x), r = x.tile * TT + row, t = min(r / G, a.T - 1), h = x.hk * G + r % G;
+      const bool real = row < x.n_rows;
+      float unit = 1.f;
+      if (blocks > 0) {                                   // the row of Q into its place
+        const __nv_bfloat16* src = a.q + x.b * a.q_sb + t * a.q_st + (long long)h * HD;
+        const bool vec = (reinterpret_cast<uintptr_t>(src) & 15) == 0;
+        auto piece = [&](int c) {
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (real) {
+            if (vec) {
+              v = *reinterpret_cast<const uint4*>(src + c * 8);
+            } else {
+              const unsigned short* u = reinterpret_cast<const unsigned short*>(src + c * 8);
+              v = make_uint4(u[0] | (uint32_t)u[1] << 16, u[2] | (uint32_t)u[3] << 16, u[4] | (uint32_t)u[5] << 16, u[6] | (uint32_t)u[7] << 16);
+            }
+          }
+          return v;
+        };
+        if (Q8) {
+          float top = 0.f;
+#pragma unroll 8
+          for (int c = 0; c < HD / 8; ++c) {
+            const uint4 v = piece(c);
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u))));
+          }
+          unit = ldexpf(1.f, top > 0.f ? min(max(8 - ilogbf(top), -110), 110) : 0);
+        }
+#pragma unroll 8
+        for (int c = 0; c < HD / 8; ++c) {
+          uint4 v = piece(c);
+          if (Q8) {
+            uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = pack16(true, __uint_as_float(w[i] << 16) * unit, __uint_as_float(w[i] & 0xffff0000u) * unit);
+            v = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+          *reinterpret_cast<uint4*>(gen + (c >> 3) * (TT * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = v;
+        }
+        tc_fence_before();                                // O of the stretch before has been read
+        fence_proxy_async_smem();
+        mbar_arrive(bar(Q_FULL));
+      }
+      const float q_unit = a.scale_log2 / unit;
+      const unsigned long long vis = a.visible ? (unsigned long long)__ldg(a.visible + (long long)x.b * a.T + t) : t >= 63 ? ~0ull : (2ull << t) - 1;
+      const int row_lo = a.window > 0 ? max(0, x.s.pos + max(__popcll(vis), 1) - a.window) : 0;
+      const bool works = warp * 32 < x.n_rows;            // some row of this warp is real
+      const F2 unit2 = f2(q_unit, q_unit);
+      float m = -CUDART_INF_F, l = 0.f;
+      for (int j = 0; ok && j < blocks; ++j, ++n) {
+        ok = mbar_wait_warp(bar(S_FULL + (n & 1)), (n >> 1) & 1, abort_smem, a.status, SITE_TMEM_FULL);
+        if (ok && Q8) ok = mbar_wait_warp(bar(SC_FULL + n % SCALES), (n / SCALES) & 1, abort_smem, a.status, SITE_SMEM_FULL);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t s_addr = lane_addr + (n & 1) * 128;
+        if (works) {
+          const int slot0 = x.k_lo + j * TT;
+          const bool masked = masked_block(a, x, slot0);
+          const float4* ks = reinterpret_cast<const float4*>(scale_s + (n % SCALES) * 3 * TT);
+          float top = -CUDART_INF_F;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t v[32];
+            tmem_ld_32x32(s_addr + c * 32, v);
+            tmem_ld_wait();
+            const uint32_t see = masked ? seen(x, row_lo, vis, slot0 + c * 32) : ~0u;
+            float part[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              float f[4] = {__uint_as_float(v[i]), __uint_as_float(v[i + 1]), __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])};
+              if (Q8) {
+                const float4 k4 = ks[(c * 32 + i) / 4], u4 = ks[TT / 4 + (c * 32 + i) / 4];
+                unpack(fma2(mul2(f2(f[0], f[1]), f2(k4.x, k4.y)), unit2, f2(u4.x, u4.y)), f[0], f[1]);
+                unpack(fma2(mul2(f2(f[2], f[3]), f2(k4.z, k4.w)), unit2, f2(u4.z, u4.w)), f[2], f[3]);
+              }
+              if (masked) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (!(see >> (i + e) & 1u)) f[e] = -CUDART_INF_F;
+              }
+#pragma unroll
+              for (int e = 0; e < 4; ++e) part[e] = fmaxf(part[e], f[e]);
+            }
+            top = fmaxf(top, fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])));
+          }
+          if (!Q8) top *= q_unit;
+          float alpha = 1.f;
+          if (top - LIFT > m + 8.f) {                     // also the first block with a visible key (m = -inf)
+            alpha = ex2(m - (top - LIFT));
+            m = top - LIFT;
+          }
+          // tcgen05.ld / .st are warp-collective: the decision must be the same for all rows of a warp.  Never for the first
+          // block: its product overwrites O.
+          if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+            ok = mbar_wait_warp(bar(O_DONE), (n - 1) & 1, abort_smem, a.status, SITE_TMEM_EMPTY);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < HD / 16; ++c) {
+              uint32_t o[16];
+              tmem_ld_32x16(lane_addr + 256 + c * 16, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              tmem_st_32x16(lane_addr + 256 + c * 16, o);
+            }
+          }
+          const float off = m == -CUDART_INF_F ? 0.f : -m;
+          const F2 off2 = f2(off, off);
+          F2 sum2[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t v[32], w[16];
+            tmem_ld_32x32(s_addr + c * 32, v);
+            tmem_ld_wait();
+            const uint32_t see = masked ? seen(x, row_lo, vis, slot0 + c * 32) : ~0u;
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              float4 k4, v4;
+              if (Q8) {
+                k4 = ks[(c * 32 + i) / 4];
+                v4 = ks[2 * TT / 4 + (c * 32 + i) / 4];
+              }
+#pragma unroll
+              for (int e = 0; e < 4; e += 2) {
+                F2 f = f2(__uint_as_float(v[i + e]), __uint_as_float(v[i + e + 1]));
+                if (Q8) f = mul2(f, e ? f2(k4.z, k4.w) : f2(k4.x, k4.y));
+                float p0, p1;
+                unpack(fma2(f, unit2, off2), p0, p1);
+                p0 = ex2(p0);
+                p1 = ex2(p1);
+                if (masked) {
+                  if (!(see >> (i + e) & 1u)) p0 = 0.f;
+                  if (!(see >> (i + e + 1) & 1u)) p1 = 0.f;
+                }
+                sum2[e / 2] = add2(sum2[e / 2], f2(p0, p1));
+                if (Q8) {
+                  unpack(mul2(f2(p0, p1), e ? f2(v4.z, v4.w) : f2(v4.x, v4.y)), p0, p1);
+                  if (masked) {                           // a hidden key's scale may be anything
+                    if (!(see >> (i + e) & 1u)) p0 = 0.f;
+                    if (!(see >> (i + e + 1) & 1u)) p1 = 0.f;
+                  }
+                }
+                w[(i + e) / 2] = pack16(Q8, p0, p1);
+              }
+            }
+            tmem_st_32x16(s_addr + c * 16, w);            // these scores have been read for the last time
+          }
+          float s0, s1;
+          unpack(add2(sum2[0], sum2[1]), s0, s1);
+          l = l * alpha + s0 + s1;
+          tmem_st_wait();
+        }
+        tc_fence_before();
+        mbar_arrive(bar(P_FULL + (n & 1)));
+      }
+      if (!ok) break;
+      // ---- the stretch's result: final, or a share of it
+      if (blocks > 0) {
+        ok = mbar_wait_warp(bar(O_DONE), (n - 1) & 1, abort_smem, a.status, SITE_TMEM_FULL);
+        if (!ok) break;
+        tc_fence_after();
+      }
+      if (!works) continue;
+      const bool spoilt = !Q8 && spoilt_s[stretch & 3] == stretch + 1;
+      const float inv = !x.whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
+      __nv_bfloat16* dst = a.out + x.b * a.o_sb + t * a.o_st + (long long)h * HD;
+      const bool vec = (reinterpret_cast<uintptr_t>(dst) & 15) == 0;
+#pragma unroll 1
+      for (int c = 0; c < HD / 32; ++c) {
+        uint32_t o[32];
+        if (blocks > 0) {
+          tmem_ld_32x32(lane_addr + 256 + c * 32, o);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0;
+        }
+        if (spoilt) {                                     // seldom: values of the masked blocks that are not finite
+          const __nv_bfloat16* v0 = reinterpret_cast<const __nv_bfloat16*>(a.v) + ((long long)x.b * a.kv_heads + x.hk) * a.max_seq * HD + c * 32;
+          for (int slot = x.k_lo; slot < x.k_hi; ++slot) {
+            if (!masked_block(a, x, x.k_lo + (slot - x.k_lo) / TT * TT)) continue;
+            if (!(seen(x, row_lo, vis, slot) & 1u)) continue;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const float f = __bfloat162float(v0[(long long)slot * HD + i]);
+              if (!(fabsf(f) < CUDART_INF_F)) o[i] = __float_as_uint(__uint_as_float(o[i]) + f);
+            }
+          }
+          __syncwarp();
+        }
+        // the loads above are warp-collective: every lane takes part, only the stores depend on the row being real
+        if (real && x.whole) {
+          uint32_t w[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) w[i] = pack16(false, __uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+          uint32_t* p = reinterpret_cast<uint32_t*>(dst + c * 32);
+          if (vec) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) reinterpret_cast<uint4*>(p)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) p[i] = w[i];
+          }
+        } else if (real) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            a.part[(x.slot * (HD / 4) + c * 8 + i) * TT + row] =
+                make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+        }
+        __syncwarp();
+      }
+      if (!x.whole && real) a.part_ml[x.slot * TT + row] = make_float2(m, l);
+      __syncwarp();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 12) {
+    tc_fence_after();
+    tmem_dealloc<1>(tmem, 512);
+  }
+}
+
+// Joins the shares of the items that were cut: a CTA per item and 8 columns, four groups of threads that take the shares in
+// turn, a thread per row.
+constexpr int GROUPS = 4;
+template <int HD>
+__global__ void __launch_bounds__(GROUPS * TT) wide_join_kernel(const __grid_constant__ Args a) {
+  __shared__ long long c_s[3];
+  __shared__ float2 ml_s[GROUPS][TT];
+  __shared__ float4 o_s[GROUPS][2][TT];
+  const int warp = threadIdx.x >> 5, row = threadIdx.x % TT, group = threadIdx.x / TT, G = a.q_heads / a.kv_heads;
+  const int i = blockIdx.y * 2, tile = blockIdx.x % a.tiles, hk = blockIdx.x / a.tiles % a.kv_heads, b = blockIdx.x / a.tiles / a.kv_heads;
+  if (warp == 0) shares_of_item(a, b, hk, tile, c_s);     // lengths are older than the kernel before this one
+  __syncthreads();
+  const long long c0 = c_s[0], c1 = c_s[1];
+  const int odd = (int)c_s[2];
+  const int n_rows = min(sequence(a, b).count * G - tile * TT, TT);
+  griddep_wait();                                         // all wait: what comes after this kernel relies on the one before it
+  if (c0 == c1) return;                                   // whole in one CTA, or not there
+  float m = -CUDART_INF_F, l = 0.f;
+  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (row < n_rows) {
+#pragma unroll 4
+    for (long long c = c0 + group; c <= c1; c += GROUPS) {
+      const long long slot = 2 * c + (c == c0 ? odd : 0);
+      const float2 x = __ldcg(a.part_ml + slot * TT + row);
+      const float4 u = __ldcg(a.part + (slot * (HD / 4) + i) * TT + row), v = __ldcg(a.part + (slot * (HD / 4) + i + 1) * TT + row);
+      const float now = fmaxf(m, x.x), ref = now == -CUDART_INF_F ? 0.f : now, old = ex2(m - ref), wt = ex2(x.x - ref);
+      m = now;
+      l = l * old + wt * x.y;
+      acc[0] = acc[0] * old + wt * u.x; acc[1] = acc[1] * old + wt * u.y; acc[2] = acc[2] * old + wt * u.z; acc[3] = acc[3] * old + wt * u.w;
+      acc[4] = acc[4] * old + wt * v.x; acc[5] = acc[5] * old + wt * v.y; acc[6] = acc[6] * old + wt * v.z; acc[7] = acc[7] * old + wt * v.w;
+    }
+  }
+  ml_s[group][row] = make_float2(m, l);
+  o_s[group][0][row] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+  o_s[group][1][row] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+  __syncthreads();
+  // a thread per row and pair of columns
+  const int out_row = threadIdx.x / 4, pair = threadIdx.x % 4;
+  if (out_row >= n_rows) return;
+  float mm = -CUDART_INF_F, ll = 0.f, s0 = 0.f, s1 = 0.f;
+#pragma unroll
+  for (int g = 0; g < GROUPS; ++g) mm = fmaxf(mm, ml_s[g][out_row].x);
+  const float ref = mm == -CUDART_INF_F ? 0.f : mm;
+#pragma unroll
+  for (int g = 0; g < GROUPS; ++g) {
+    const float wt = ex2(ml_s[g][out_row].x - ref);
+    const float2 v = reinterpret_cast<const float2*>(&o_s[g][pair >> 1][out_row])[pair & 1];
+    ll += wt * ml_s[g][out_row].y;
+    s0 += wt * v.x;
+    s1 += wt * v.y;
+  }
+  const float inv = ll == 0.f ? 0.f : 1.f / ll;
+  const int r = tile * TT + out_row;
+  *reinterpret_cast<uint32_t*>(a.out + b * a.o_sb + (r / G) * a.o_st + (long long)(hk * G + r % G) * HD + blockIdx.y * 8 + pair * 2) =
+      pack16(false, s0 * inv, s1 * inv);
+}
+
+template <int HD, bool Q8>
+int run(const Args& p, void* stream) {
+  using C = Wide<HD, Q8>;
+  static_assert(C::SMEM <= 226 * 1024 && TT * C::NC % LOADERS == 0, "shared memory of a CTA");
+  static std::atomic<unsigned long long> configured{0};   // a bit per device
+  int dev = 0;
+  MESH_CUDA_OK(cudaGetDevice(&dev));
+  if (!(configured.load() >> (dev & 63) & 1)) {
+    MESH_CUDA_OK(cudaFuncSetAttribute(wide_kernel<HD, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    configured.fetch_or(1ull << (dev & 63));
+  }
+  MESH_CUDA_OK(launch(wide_kernel<HD, Q8>, dim3(p.shares), THREADS, C::SMEM, stream, p));
+  if (p.part) MESH_CUDA_OK(launch(wide_join_kernel<HD>, dim3((unsigned)(p.B * p.kv_heads * p.tiles), HD / 8), GROUPS * TT, 0, stream, p));
+  return 0;
+}
+
+}  // namespace
+
+int run_wide(const Args& p, int head_dim, bool q8, void* stream) {
+  switch (head_dim * 2 + q8) {
+    case 128: return run<64, false>(p, stream);
+    case 129: return run<64, true>(p, stream);
+    case 256: return run<128, false>(p, stream);
+    case 257: return run<128, true>(p, stream);
+    case 512: return run<256, false>(p, stream);
+    default: return run<256, true>(p, stream);
+  }
+}
+
+}  // namespace draft
+}  // namespace mesh

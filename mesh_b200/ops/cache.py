@@ -14,6 +14,7 @@ from ctypes import c_char_p, c_int, c_longlong, c_void_p
 import torch
 
 from .. import _native
+from ..utils.status import status_block
 
 
 class _Cache(ctypes.Structure):
@@ -98,6 +99,7 @@ class KVCache:
         self._c = _Cache(k.data_ptr(), v.data_ptr(), 0 if k_scale is None else k_scale.data_ptr(),
                          0 if v_scale is None else v_scale.data_ptr(), B, H, S, hd, self.bits)
         self._at, self._index = ctypes.addressof(self._c), _index(k.device)
+        self._status = status_block(k.device).data_ptr() if self._index >= 0 else 0
         self._scratch: dict = {}                 # floats of scratch by the sizes of a call (ops/draft.py)
 
     @classmethod

@@ -18,8 +18,8 @@ from .. import _native
 from .cache import KVCache, _ints, _launch, _lib
 
 MAX_DRAFTS = 64
-# ``MeshDraftAttention`` (csrc/ops/draft_api.h): q, out, their strides, pos, counts, visible, T, q_heads, window, splits, scale, scratch
-_ARGS = struct.Struct("@PPqqqqPPPiiiifP")
+# ``MeshDraftAttention`` (csrc/ops/draft_api.h): q, out, their strides, pos, counts, visible, T, q_heads, window, splits, scale, scratch, status
+_ARGS = struct.Struct("@PPqqqqPPPiiiifPP")
 
 
 def tree_visible(parents) -> torch.Tensor:
@@ -84,7 +84,7 @@ def draft_attention(q: torch.Tensor, cache: KVCache, pos: torch.Tensor, *, count
     key = (T, qh, window, splits, scale)
     floats = cache._scratch.get(key)
     if floats is None:                           # a function of the sizes alone; also checks the arguments
-        floats = _lib().mesh_draft_attention_scratch(cache._at, _ARGS.pack(*args, 0))
+        floats = _lib().mesh_draft_attention_scratch(cache._at, _ARGS.pack(*args, 0, cache._status))
         if floats < 0:
             raise ValueError(_native.last_error())
         if len(cache._scratch) > 256:            # a scale of every call's own
@@ -93,9 +93,9 @@ def draft_attention(q: torch.Tensor, cache: KVCache, pos: torch.Tensor, *, count
     if B == 0 or T == 0:
         return out
     if floats == 0 or cache._index < 0:
-        _launch(cache._index, "mesh_draft_attention", 1, cache._at, _ARGS.pack(*args, 0))
+        _launch(cache._index, "mesh_draft_attention", 1, cache._at, _ARGS.pack(*args, 0, cache._status))
     else:
         # scratch of the call's own: calls on other streams and other captured graphs share nothing
         scratch = torch.empty(floats, dtype=torch.float32, device=dev)
-        _launch(cache._index, "mesh_draft_attention", 2, cache._at, _ARGS.pack(*args, scratch.data_ptr()))
+        _launch(cache._index, "mesh_draft_attention", 2, cache._at, _ARGS.pack(*args, scratch.data_ptr(), cache._status))
     return out
