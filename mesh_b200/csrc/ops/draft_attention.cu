@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(Cfg<HD, Q8>::WARPS * 32, 1) attention_kernel(c
   const uint32_t ring_u = smem_u32(ring);
   const int G = a.q_heads / a.kv_heads;
   griddep_wait();
-  griddep_launch_dependents();                            // not before: the joining kernel reads lengths before its own wait
+  griddep_launch_dependents();
 
   if (warp == 0) begin_walk(a, &walk_s);
   __syncthreads();
@@ -449,12 +449,13 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args 
   __shared__ float4 o_s[8][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = lane >> 2, t4 = lane & 3, G = a.q_heads / a.kv_heads;
   const int i = blockIdx.y, tile = blockIdx.x % a.tiles, hk = blockIdx.x / a.tiles % a.kv_heads, b = blockIdx.x / a.tiles / a.kv_heads;
-  // the lengths are older than the kernel before this one, which lets this one start when it has seen them
+  // All wait: what comes after this kernel relies on the one before it.  And none looks at the lengths before: they are older than
+  // that kernel, but only the wait keeps a read from finding what its line held before them.
+  griddep_wait();
   if (warp == 0) shares_of_item(a, b, hk, tile, c_s);
   __syncthreads();
   const long long c0 = c_s[0], c1 = c_s[1];
   const int odd = (int)c_s[2];
-  griddep_wait();                                         // all wait: what comes after this kernel relies on the one before it
   if (c0 == c1) return;                                   // whole in one CTA, or not there
   float m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.f, 0.f};
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);

@@ -58,8 +58,8 @@ struct Seq {
 };
 __device__ __forceinline__ Seq sequence(const Args& a, int b) {
   Seq s;
-  s.pos = min(max(__ldg(a.pos + b), 0), a.max_seq);
-  s.count = a.counts ? min(__ldg(a.counts + b), a.T) : a.T;
+  s.pos = min(max(__ldcg(a.pos + b), 0), a.max_seq);
+  s.count = a.counts ? min(__ldcg(a.counts + b), a.T) : a.T;
   s.hi = min(s.pos + max(s.count, 0), a.max_seq);
   s.lo = a.window > 0 ? max(0, s.pos - a.window + 1) : 0;          // the root's; its descendants see less
   return s;
@@ -202,7 +202,7 @@ static cudaError_t launch(void (*kern)(P...), dim3 grid, int threads, int smem, 
 }
 
 // The kernel for many query rows (draft_attention_wide.cu): rows of a tile, keys of a unit, and the call.
-constexpr int WIDE_ROWS = 128, WIDE_UNIT = 128;
+constexpr int WIDE_ROWS = 128, WIDE_UNIT = 64;
 int run_wide(const Args& p, int head_dim, bool q8, void* stream);
 
 }  // namespace draft

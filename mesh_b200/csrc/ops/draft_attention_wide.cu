@@ -1,36 +1,40 @@
 // Attention of drafts with many query rows (more than 16 drafts times heads of a group) on the 5th-generation tensor cores.
 //
-// A tile is 128 query rows of one (sequence, KV head); a CTA goes through its stretches of 128-key blocks (how the work is cut and
+// A tile is 128 query rows of one (sequence, KV head); a CTA goes through its stretches of 64-key blocks (how the work is cut and
 // the formulas: draft_attention.cuh, draft_attention.cu).  Warps 0-3: softmax, a thread per query row.  Warps 4-11: keys and
-// values, loaded into registers ahead of their turn, widened (8-bit codes to fp16) and stored to shared memory in the
+// values, loaded into registers four tiles ahead of their turn, widened (8-bit codes to fp16) and stored to shared memory in the
 // 128-byte swizzle of the operands.  Warp 12: the products S = Q K^T and O += P V by one elected lane, S of the next block
-// before P V of this one; S is double-buffered in tensor memory, P (16 bits) overwrites the first half of its S and is
-// operand A from there, O stays in tensor memory and is rescaled only when a row's maximum has grown by more than 2^8.
+// before P V of this one.  Tensor memory holds the queries (operand A of the first product, 16 bits), S twice, of which P (16
+// bits, operand A of the second) overwrites the first half, and O, which is rescaled only when a row's maximum has grown by
+// more than 2^8.
 //
 // Codes are widened once per 128 rows, in registers: as operands of a product in 8 bits the queries and probabilities would have to be
-// rounded to 8 bits too.  Two passes over a row's scores instead of holding all 128: 13 warps with 152 registers each
-// then fit, so the widening has eight warps of its own.  With heads of 256 one tile of keys and one of values fill shared
-// memory beside the queries; the store of one runs under the product of the other.
+// rounded to 8 bits too.  Queries in tensor memory leave shared memory to three tiles of keys and three of values with heads
+// of 256, and its bandwidth to their stores and reads.  What was slower, at 64 drafts x 4 heads over four contexts of
+// 20000-32704 keys of 256 in 8 bits: blocks of 128 keys with the queries in shared memory, where one tile of keys and one of
+// values fit and the registers one tile ahead, 126 us; the same with scores read twice from tensor memory, 165 us.
 #include "draft_attention.cuh"
 
 namespace mesh {
 namespace draft {
 namespace {
 
-constexpr int TT = WIDE_ROWS;
+constexpr int TT = WIDE_ROWS, KB = WIDE_UNIT;               // rows of a tile, keys of a block
 constexpr int SOFT = 128, LOADERS = 256, THREADS = SOFT + LOADERS + 32;
-constexpr int SCALES = 4;                                  // blocks whose scales are kept: more than a loader is ahead of the softmax
+constexpr int LOAD_WARP = SOFT / 32, PRODUCT_WARP = (SOFT + LOADERS) / 32;
+constexpr int SCALES = 8;                                   // blocks whose scales are kept: two more than there are stages, at least
 
 template <int HD, bool Q8>
 struct Wide {
-  static constexpr int TILE = TT * HD * 2;
-  static constexpr int STAGES = HD == 256 ? 1 : 2;
+  static constexpr int TILE = KB * HD * 2;
+  static constexpr int STAGES = HD == 256 ? 3 : 4;
   static constexpr int RB = Q8 ? HD : 2 * HD, NC = RB / 16;           // bytes and 16-byte pieces of a stored row
-  static constexpr int VPT = TT * NC / LOADERS;            // pieces of a loader thread per tile
-  static constexpr int DEPTH = VPT >= 16 ? 1 : VPT >= 8 ? 2 : 4;      // tiles in registers
-  static constexpr int N_BARS = 1 + 4 * STAGES + 2 + 2 + 1 + SCALES;
-  static constexpr int SCALE_BYTES = Q8 ? SCALES * 3 * TT * 4 : 0;
-  static constexpr int SMEM = (1 + 2 * STAGES) * TILE + SCALE_BYTES + 8 * N_BARS + 64 + 1024;
+  static constexpr int VPT = KB * NC / LOADERS;             // pieces of a loader thread per tile
+  static constexpr int DEPTH = VPT >= 4 ? 16 / VPT : 4;     // tiles in registers
+  static constexpr int N_BARS = 1 + 4 * STAGES + 2 + 2 + 2 + SCALES;
+  static constexpr int SCALE_BYTES = Q8 ? SCALES * 3 * KB * 4 : 0;
+  static constexpr int SMEM = 2 * STAGES * TILE + SCALE_BYTES + 8 * N_BARS + 64 + 1024;
+  static constexpr int S_COL = 0, O_COL = 2 * KB, Q_COL = O_COL + HD;  // columns of tensor memory
 };
 
 // two fp32 at a time
@@ -57,10 +61,10 @@ __device__ __forceinline__ F2 add2(F2 a, F2 b) {
   return r;
 }
 
-__device__ __forceinline__ int blocks_of(const Stretch& x) { return (x.k_hi - x.k_lo + TT - 1) / TT; }
+__device__ __forceinline__ int blocks_of(const Stretch& x) { return (x.k_hi - x.k_lo + KB - 1) / KB; }
 // Whether some row may not see some key of the block.
 __device__ __forceinline__ bool masked_block(const Args& a, const Stretch& x, int slot0) {
-  return (a.window > 0 && slot0 < x.s.pos + 64 - a.window) || slot0 + TT > min(x.s.pos, x.k_hi);
+  return (a.window > 0 && slot0 < x.s.pos + 64 - a.window) || slot0 + KB > min(x.s.pos, x.k_hi);
 }
 // Bits of the slots first .. first + 32 that a row sees.
 __device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; }
@@ -82,11 +86,11 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
-  const uint32_t sQ = base, sK = sQ + C::TILE, sV = sK + STAGES * C::TILE, sScale = sV + STAGES * C::TILE, bars = sScale + C::SCALE_BYTES;
+  const uint32_t sK = base, sV = sK + STAGES * C::TILE, sScale = sV + STAGES * C::TILE, bars = sScale + C::SCALE_BYTES;
   float* scale_s = reinterpret_cast<float*>(gen + (sScale - base));        // [buffer]{key scale, lg2 of the value scale, value scale}[key]
   auto bar = [&](int i) { return bars + 8u * i; };
   constexpr int Q_FULL = 0, K_FULL = 1, K_EMPTY = K_FULL + STAGES, V_FULL = K_EMPTY + STAGES, V_EMPTY = V_FULL + STAGES,
-                S_FULL = V_EMPTY + STAGES, P_FULL = S_FULL + 2, O_DONE = P_FULL + 2, SC_FULL = O_DONE + 1;
+                S_FULL = V_EMPTY + STAGES, P_FULL = S_FULL + 2, O_DONE = P_FULL + 2, SC_FULL = O_DONE + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen + (bars - base) + 8 * C::N_BARS);
   volatile int* abort_smem = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* spoilt_s = reinterpret_cast<volatile int*>(tmem_slot + 2);     // [4]: stretch + 1 whose values had to be cleaned
@@ -104,19 +108,19 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
     for (int s = 0; s < 2; ++s) {
       mbar_init(bar(S_FULL + s), 1);
       mbar_init(bar(P_FULL + s), SOFT);
+      mbar_init(bar(O_DONE + s), 1);
     }
-    mbar_init(bar(O_DONE), 1);
     for (int s = 0; s < SCALES; ++s) mbar_init(bar(SC_FULL + s), LOADERS);
     *abort_smem = 0;
     for (int s = 0; s < 4; ++s) spoilt_s[s] = 0;
     fence_mbar_init();
   }
-  if (warp == 12) {
+  if (warp == PRODUCT_WARP) {
     tmem_alloc<1>(smem_u32(tmem_slot), 512);
     tmem_relinquish<1>();
   }
   griddep_wait();
-  griddep_launch_dependents();                            // not before: the joining kernel reads lengths before its own wait
+  griddep_launch_dependents();
   if (warp == 0) begin_walk(a, &walk_s);
   tc_fence_before();
   __syncthreads();
@@ -126,13 +130,13 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
   Stretch x;
   bool ok = true;
 
-  if (warp >= 4 && warp < 12) {
+  if (warp >= LOAD_WARP && warp < PRODUCT_WARP) {
     // ------------------------------------------------------------------ keys and values
     // Per stretch, in the order the products take them: K0 K1 V0 K2 V1 ...  `load` fetches the next tile into a set of
     // registers, `store` puts the oldest set into its place when that is free.
     const int lt = threadIdx.x - SOFT;
     uint4 raw[C::DEPTH][VPT];
-    float scale[C::DEPTH];
+    float scale[C::DEPTH];                                // of key lt or of value lt - 64
     int what[C::DEPTH];                                   // 0 nothing, 1 key, 2 value, 3 value to be cleaned
     int stretch_of[C::DEPTH];
     int blocks = 0, kj = 0, vj = 0, stretch = -1;
@@ -147,15 +151,15 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
       }
       if (!more) return;
       const bool key = kj < blocks && kj <= vj + 1;
-      const int j = key ? kj++ : vj++, slot0 = x.k_lo + j * TT, rows = min(x.k_hi - slot0, TT);
+      const int j = key ? kj++ : vj++, slot0 = x.k_lo + j * KB, rows = min(x.k_hi - slot0, KB);
       const long long at = ((long long)x.b * a.kv_heads + x.hk) * a.max_seq + slot0;
       const uint4* src = reinterpret_cast<const uint4*>((key ? a.k : a.v) + at * C::RB) + lt;
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
         raw[d][i] = make_uint4(0, 0, 0, 0);               // behind the last slot: what a hidden row holds is not read
-        if ((i * LOADERS + lt) / NC < rows) raw[d][i] = __ldg(src + i * LOADERS);
+        if ((i * LOADERS + lt) / NC < rows) raw[d][i] = __ldcg(src + i * LOADERS);
       }
-      if (Q8 && key) scale[d] = (lt & 127) < rows ? __ldg((lt < 128 ? a.k_scale : a.v_scale) + at + (lt & 127)) : 0.f;
+      if (Q8 && key && lt < 2 * KB) scale[d] = lt % KB < rows ? __ldcg((lt < KB ? a.k_scale : a.v_scale) + at + lt % KB) : 0.f;
       what[d] = key ? 1 : !Q8 && masked_block(a, x, slot0) ? 3 : 2;
       stretch_of[d] = stretch;
     };
@@ -172,7 +176,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
         const int idx = i * LOADERS + lt, r = idx / NC, c = idx % NC;
         uint4 v = raw[d][i];
         if (Q8) {
-          uint8_t* p = gen + dst + (c >> 2) * (TT * 128) + r * 128;
+          uint8_t* p = gen + dst + (c >> 2) * (KB * 128) + r * 128;
           const uint32_t w[4] = {v.x ^ 0x80808080u, v.y ^ 0x80808080u, v.z ^ 0x80808080u, v.w ^ 0x80808080u};
           const uint4 lo = make_uint4(codes2(w[0], 0x4140), codes2(w[0], 0x4342), codes2(w[1], 0x4140), codes2(w[1], 0x4342));
           const uint4 hi = make_uint4(codes2(w[2], 0x4140), codes2(w[2], 0x4342), codes2(w[3], 0x4140), codes2(w[3], 0x4342));
@@ -186,17 +190,17 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
             v = make_uint4(finite_or_zero(v.x), finite_or_zero(v.y), finite_or_zero(v.z), finite_or_zero(v.w));
             spoilt = true;
           }
-          *reinterpret_cast<uint4*>(gen + dst + (c >> 3) * (TT * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+          *reinterpret_cast<uint4*>(gen + dst + (c >> 3) * (KB * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
         }
       }
       if (!Q8 && spoilt) spoilt_s[stretch_of[d] & 3] = stretch_of[d] + 1;
       if (Q8 && key) {
-        float* sc = scale_s + (n % SCALES) * 3 * TT + (lt & 127);
-        if (lt < 128) {
+        float* sc = scale_s + (n % SCALES) * 3 * KB + lt % KB;
+        if (lt < KB) {
           sc[0] = scale[d];
-        } else {
-          sc[TT] = fmaxf(lg2(scale[d]), -60.f);
-          sc[2 * TT] = scale[d];
+        } else if (lt < 2 * KB) {
+          sc[KB] = fmaxf(lg2(scale[d]), -60.f);
+          sc[2 * KB] = scale[d];
         }
         mbar_arrive(bar(SC_FULL + n % SCALES));
       }
@@ -214,12 +218,12 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
         }
       }
     }
-  } else if (warp == 12) {
+  } else if (warp == PRODUCT_WARP) {
     // ------------------------------------------------------------------ products (warp-uniform, one elected lane issues)
     constexpr uint32_t half = Q8 ? (1u << 7) | (1u << 10) : 0u;              // operands in fp16 instead of bf16
-    constexpr uint32_t idesc_s = umma_idesc_bf16(TT, TT, 0, 0) & ~half, idesc_o = umma_idesc_bf16(TT, HD, 0, 1) & ~half;
+    constexpr uint32_t idesc_s = umma_idesc_bf16(TT, KB, 0, 0) & ~half, idesc_o = umma_idesc_bf16(TT, HD, 0, 1) & ~half;
     const bool leader = elect_one();
-    const uint64_t dq0 = umma_smem_desc(sQ, 16, 1024), dk0 = umma_smem_desc(sK, 16, 1024), dv0 = umma_smem_desc(sV, TT * 128, 1024);
+    const uint64_t dk0 = umma_smem_desc(sK, 16, 1024), dv0 = umma_smem_desc(sV, KB * 128, 1024);
     int n = 0, visit = 0;                                 // blocks and stretches done
     auto issue_s = [&](int n) {
       const int s = n % STAGES;
@@ -229,8 +233,8 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
       if (leader) {
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k) {
-          const int off = ((k / 4) * (TT * 128) + (k % 4) * 32) / 16;
-          umma_f16<1>(tmem + (n & 1) * 128, dq0 + off, dk0 + (uint32_t)(s * (C::TILE >> 4)) + off, idesc_s, k ? 1u : 0u);
+          const int off = ((k / 4) * (KB * 128) + (k % 4) * 32) / 16;
+          umma_f16_ts(tmem + C::S_COL + (n & 1) * KB, tmem + C::Q_COL + k * 8, dk0 + (uint32_t)(s * (C::TILE >> 4)) + off, idesc_s, k ? 1u : 0u);
         }
         umma_commit(bar(K_EMPTY + s));
         umma_commit(bar(S_FULL + (n & 1)));
@@ -243,7 +247,14 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
       ok = mbar_wait_warp(bar(Q_FULL), visit++ & 1, abort_smem, a.status, SITE_SMEM_FULL);
       if (ok) issue_s(n);
       for (int j = 0; ok && j < blocks; ++j, ++n) {
-        if (j + 1 < blocks) issue_s(n + 1);
+        if (j + 1 < blocks) {
+          // S of the next block overwrites the P that the product before the last one reads, and products of different shapes are
+          // not ordered among themselves: that one's end is waited for.  (So by the time a block's scores are there, the
+          // product two blocks back is over: a wait for the end of a product, on one of two barriers in turn, cannot be
+          // answered by the phase before.)
+          if (j > 0) ok = mbar_wait_warp(bar(O_DONE + ((n - 1) & 1)), ((n - 1) >> 1) & 1, abort_smem, a.status, SITE_TMEM_EMPTY);
+          if (ok) issue_s(n + 1);
+        }
         const int s = n % STAGES;
         if (ok) ok = mbar_wait_warp(bar(V_FULL + s), (n / STAGES) & 1, abort_smem, a.status, SITE_SMEM_FULL);
         if (ok) ok = mbar_wait_warp(bar(P_FULL + (n & 1)), (n >> 1) & 1, abort_smem, a.status, SITE_TMEM_FULL);
@@ -251,15 +262,15 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
         tc_fence_after();
         if (leader) {
 #pragma unroll
-          for (int k = 0; k < TT / 16; ++k)
-            umma_f16_ts(tmem + 256, tmem + (n & 1) * 128 + k * 8, dv0 + (uint32_t)(s * (C::TILE >> 4)) + k * 128, idesc_o, (j | k) ? 1u : 0u);
+          for (int k = 0; k < KB / 16; ++k)
+            umma_f16_ts(tmem + C::O_COL, tmem + C::S_COL + (n & 1) * KB + k * 8, dv0 + (uint32_t)(s * (C::TILE >> 4)) + k * 128, idesc_o, (j | k) ? 1u : 0u);
           umma_commit(bar(V_EMPTY + s));
-          umma_commit(bar(O_DONE));
+          umma_commit(bar(O_DONE + (n & 1)));
         }
         __syncwarp();
       }
     }
-  } else if (warp < 4) {
+  } else if (warp < LOAD_WARP) {
     // ------------------------------------------------------------------ softmax: thread = query row = TMEM lane
     constexpr float LIFT = Q8 ? 6.f : 0.f;                // with the 2^8 that a reference may lag behind, w stays below 2^14
     const int row = threadIdx.x;
@@ -296,23 +307,27 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
           }
           unit = ldexpf(1.f, top > 0.f ? min(max(8 - ilogbf(top), -110), 110) : 0);
         }
-#pragma unroll 8
-        for (int c = 0; c < HD / 8; ++c) {
-          uint4 v = piece(c);
-          if (Q8) {
-            uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll 1
+        for (int c = 0; c < HD / 32; ++c) {
+          uint32_t w[16];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = pack16(true, __uint_as_float(w[i] << 16) * unit, __uint_as_float(w[i] & 0xffff0000u) * unit);
-            v = make_uint4(w[0], w[1], w[2], w[3]);
+          for (int i = 0; i < 4; ++i) {
+            const uint4 v = piece(c * 4 + i);
+            w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
           }
-          *reinterpret_cast<uint4*>(gen + (c >> 3) * (TT * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = v;
+          if (Q8) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w[i] = pack16(true, __uint_as_float(w[i] << 16) * unit, __uint_as_float(w[i] & 0xffff0000u) * unit);
+          }
+          __syncwarp();
+          tmem_st_32x16(lane_addr + C::Q_COL + c * 16, w);
         }
-        tc_fence_before();                                // O of the stretch before has been read
-        fence_proxy_async_smem();
+        tmem_st_wait();
+        tc_fence_before();                                // and O of the stretch before has been read
         mbar_arrive(bar(Q_FULL));
       }
       const float q_unit = a.scale_log2 / unit;
-      const unsigned long long vis = a.visible ? (unsigned long long)__ldg(a.visible + (long long)x.b * a.T + t) : t >= 63 ? ~0ull : (2ull << t) - 1;
+      const unsigned long long vis = a.visible ? (unsigned long long)__ldcg(a.visible + (long long)x.b * a.T + t) : t >= 63 ? ~0ull : (2ull << t) - 1;
       const int row_lo = a.window > 0 ? max(0, x.s.pos + max(__popcll(vis), 1) - a.window) : 0;
       const bool works = warp * 32 < x.n_rows;            // some row of this warp is real
       const F2 unit2 = f2(q_unit, q_unit);
@@ -322,37 +337,55 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
         if (ok && Q8) ok = mbar_wait_warp(bar(SC_FULL + n % SCALES), (n / SCALES) & 1, abort_smem, a.status, SITE_SMEM_FULL);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t s_addr = lane_addr + (n & 1) * 128;
+        const uint32_t s_addr = lane_addr + C::S_COL + (n & 1) * KB;
         if (works) {
-          const int slot0 = x.k_lo + j * TT;
+          const int slot0 = x.k_lo + j * KB;
           const bool masked = masked_block(a, x, slot0);
-          const float4* ks = reinterpret_cast<const float4*>(scale_s + (n % SCALES) * 3 * TT);
-          float top = -CUDART_INF_F;
+          const float4* ks = reinterpret_cast<const float4*>(scale_s + (n % SCALES) * 3 * KB);
+          uint32_t v[2][32];                              // scores times the keys' scales
+          tmem_ld_32x32(s_addr, v[0]);
+          tmem_ld_32x32(s_addr + 32, v[1]);
+          tmem_ld_wait();
+          if (Q8) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t v[32];
-            tmem_ld_32x32(s_addr + c * 32, v);
-            tmem_ld_wait();
-            const uint32_t see = masked ? seen(x, row_lo, vis, slot0 + c * 32) : ~0u;
-            float part[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+              for (int i = 0; i < 32; i += 4) {
+                const float4 k4 = ks[(c * 32 + i) / 4];
+                float f0, f1;
+                unpack(mul2(f2(__uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1])), f2(k4.x, k4.y)), f0, f1);
+                v[c][i] = __float_as_uint(f0);
+                v[c][i + 1] = __float_as_uint(f1);
+                unpack(mul2(f2(__uint_as_float(v[c][i + 2]), __uint_as_float(v[c][i + 3])), f2(k4.z, k4.w)), f0, f1);
+                v[c][i + 2] = __float_as_uint(f0);
+                v[c][i + 3] = __float_as_uint(f1);
+              }
+          }
+          uint32_t see[2] = {~0u, ~0u};
+          if (masked) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              see[c] = seen(x, row_lo, vis, slot0 + c * 32);
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (!(see[c] >> i & 1u)) v[c][i] = 0xff800000u;          // -inf: exp2 gives an exact zero
+            }
+          }
+          float part[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
 #pragma unroll
             for (int i = 0; i < 32; i += 4) {
-              float f[4] = {__uint_as_float(v[i]), __uint_as_float(v[i + 1]), __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])};
+              float f[4] = {__uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1]), __uint_as_float(v[c][i + 2]), __uint_as_float(v[c][i + 3])};
               if (Q8) {
-                const float4 k4 = ks[(c * 32 + i) / 4], u4 = ks[TT / 4 + (c * 32 + i) / 4];
-                unpack(fma2(mul2(f2(f[0], f[1]), f2(k4.x, k4.y)), unit2, f2(u4.x, u4.y)), f[0], f[1]);
-                unpack(fma2(mul2(f2(f[2], f[3]), f2(k4.z, k4.w)), unit2, f2(u4.z, u4.w)), f[2], f[3]);
-              }
-              if (masked) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  if (!(see >> (i + e) & 1u)) f[e] = -CUDART_INF_F;
+                const float4 u4 = ks[KB / 4 + (c * 32 + i) / 4];
+                unpack(fma2(f2(f[0], f[1]), unit2, f2(u4.x, u4.y)), f[0], f[1]);
+                unpack(fma2(f2(f[2], f[3]), unit2, f2(u4.z, u4.w)), f[2], f[3]);
               }
 #pragma unroll
               for (int e = 0; e < 4; ++e) part[e] = fmaxf(part[e], f[e]);
             }
-            top = fmaxf(top, fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])));
-          }
+          float top = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
           if (!Q8) top *= q_unit;
           float alpha = 1.f;
           if (top - LIFT > m + 8.f) {                     // also the first block with a visible key (m = -inf)
@@ -362,59 +395,43 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
           // tcgen05.ld / .st are warp-collective: the decision must be the same for all rows of a warp.  Never for the first
           // block: its product overwrites O.
           if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-            ok = mbar_wait_warp(bar(O_DONE), (n - 1) & 1, abort_smem, a.status, SITE_TMEM_EMPTY);
+            ok = mbar_wait_warp(bar(O_DONE + ((n - 1) & 1)), ((n - 1) >> 1) & 1, abort_smem, a.status, SITE_TMEM_EMPTY);
             if (!ok) break;
             tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < HD / 16; ++c) {
               uint32_t o[16];
-              tmem_ld_32x16(lane_addr + 256 + c * 16, o);
+              tmem_ld_32x16(lane_addr + C::O_COL + c * 16, o);
               tmem_ld_wait();
 #pragma unroll
               for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-              tmem_st_32x16(lane_addr + 256 + c * 16, o);
+              tmem_st_32x16(lane_addr + C::O_COL + c * 16, o);
             }
           }
           const float off = m == -CUDART_INF_F ? 0.f : -m;
           const F2 off2 = f2(off, off);
           F2 sum2[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t v[32], w[16];
-            tmem_ld_32x32(s_addr + c * 32, v);
-            tmem_ld_wait();
-            const uint32_t see = masked ? seen(x, row_lo, vis, slot0 + c * 32) : ~0u;
+          for (int c = 0; c < 2; ++c) {
+            uint32_t w[16];
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              float4 k4, v4;
+            for (int i = 0; i < 32; i += 2) {
+              float p0, p1;
+              unpack(fma2(f2(__uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1])), unit2, off2), p0, p1);
+              F2 p = f2(ex2(p0), ex2(p1));
+              sum2[(i / 2) & 1] = add2(sum2[(i / 2) & 1], p);
               if (Q8) {
-                k4 = ks[(c * 32 + i) / 4];
-                v4 = ks[2 * TT / 4 + (c * 32 + i) / 4];
+                const float4 v4 = ks[2 * KB / 4 + (c * 32 + i) / 4];
+                p = mul2(p, i & 2 ? f2(v4.z, v4.w) : f2(v4.x, v4.y));
               }
-#pragma unroll
-              for (int e = 0; e < 4; e += 2) {
-                F2 f = f2(__uint_as_float(v[i + e]), __uint_as_float(v[i + e + 1]));
-                if (Q8) f = mul2(f, e ? f2(k4.z, k4.w) : f2(k4.x, k4.y));
-                float p0, p1;
-                unpack(fma2(f, unit2, off2), p0, p1);
-                p0 = ex2(p0);
-                p1 = ex2(p1);
-                if (masked) {
-                  if (!(see >> (i + e) & 1u)) p0 = 0.f;
-                  if (!(see >> (i + e + 1) & 1u)) p1 = 0.f;
-                }
-                sum2[e / 2] = add2(sum2[e / 2], f2(p0, p1));
-                if (Q8) {
-                  unpack(mul2(f2(p0, p1), e ? f2(v4.z, v4.w) : f2(v4.x, v4.y)), p0, p1);
-                  if (masked) {                           // a hidden key's scale may be anything
-                    if (!(see >> (i + e) & 1u)) p0 = 0.f;
-                    if (!(see >> (i + e + 1) & 1u)) p1 = 0.f;
-                  }
-                }
-                w[(i + e) / 2] = pack16(Q8, p0, p1);
-              }
+              unpack(p, p0, p1);
+              w[i / 2] = pack16(Q8, p0, p1);
             }
-            tmem_st_32x16(s_addr + c * 16, w);            // these scores have been read for the last time
+            if (Q8 && masked) {                           // a hidden key's scale may be anything
+#pragma unroll
+              for (int i = 0; i < 16; ++i) w[i] &= (see[c] >> (2 * i) & 1u ? 0xffffu : 0u) | (see[c] >> (2 * i + 1) & 1u ? 0xffff0000u : 0u);
+            }
+            tmem_st_32x16(s_addr + c * 16, w);            // every score is in registers by now
           }
           float s0, s1;
           unpack(add2(sum2[0], sum2[1]), s0, s1);
@@ -427,7 +444,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
       if (!ok) break;
       // ---- the stretch's result: final, or a share of it
       if (blocks > 0) {
-        ok = mbar_wait_warp(bar(O_DONE), (n - 1) & 1, abort_smem, a.status, SITE_TMEM_FULL);
+        ok = mbar_wait_warp(bar(O_DONE + ((n - 1) & 1)), ((n - 1) >> 1) & 1, abort_smem, a.status, SITE_TMEM_FULL);
         if (!ok) break;
         tc_fence_after();
       }
@@ -440,7 +457,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
       for (int c = 0; c < HD / 32; ++c) {
         uint32_t o[32];
         if (blocks > 0) {
-          tmem_ld_32x32(lane_addr + 256 + c * 32, o);
+          tmem_ld_32x32(lane_addr + C::O_COL + c * 32, o);
           tmem_ld_wait();
         } else {
 #pragma unroll
@@ -449,7 +466,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
         if (spoilt) {                                     // seldom: values of the masked blocks that are not finite
           const __nv_bfloat16* v0 = reinterpret_cast<const __nv_bfloat16*>(a.v) + ((long long)x.b * a.kv_heads + x.hk) * a.max_seq * HD + c * 32;
           for (int slot = x.k_lo; slot < x.k_hi; ++slot) {
-            if (!masked_block(a, x, x.k_lo + (slot - x.k_lo) / TT * TT)) continue;
+            if (!masked_block(a, x, x.k_lo + (slot - x.k_lo) / KB * KB)) continue;
             if (!(seen(x, row_lo, vis, slot) & 1u)) continue;
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
@@ -486,7 +503,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == PRODUCT_WARP) {
     tc_fence_after();
     tmem_dealloc<1>(tmem, 512);
   }
@@ -502,12 +519,14 @@ __global__ void __launch_bounds__(GROUPS * TT) wide_join_kernel(const __grid_con
   __shared__ float4 o_s[GROUPS][2][TT];
   const int warp = threadIdx.x >> 5, row = threadIdx.x % TT, group = threadIdx.x / TT, G = a.q_heads / a.kv_heads;
   const int i = blockIdx.y * 2, tile = blockIdx.x % a.tiles, hk = blockIdx.x / a.tiles % a.kv_heads, b = blockIdx.x / a.tiles / a.kv_heads;
-  if (warp == 0) shares_of_item(a, b, hk, tile, c_s);     // lengths are older than the kernel before this one
+  // All wait: what comes after this kernel relies on the one before it.  And none looks at the lengths before: they are older than
+  // that kernel, but only the wait keeps a read from finding what its line held before them.
+  griddep_wait();
+  if (warp == 0) shares_of_item(a, b, hk, tile, c_s);
   __syncthreads();
   const long long c0 = c_s[0], c1 = c_s[1];
   const int odd = (int)c_s[2];
   const int n_rows = min(sequence(a, b).count * G - tile * TT, TT);
-  griddep_wait();                                         // all wait: what comes after this kernel relies on the one before it
   if (c0 == c1) return;                                   // whole in one CTA, or not there
   float m = -CUDART_INF_F, l = 0.f;
   float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -552,7 +571,7 @@ __global__ void __launch_bounds__(GROUPS * TT) wide_join_kernel(const __grid_con
 template <int HD, bool Q8>
 int run(const Args& p, void* stream) {
   using C = Wide<HD, Q8>;
-  static_assert(C::SMEM <= 226 * 1024 && TT * C::NC % LOADERS == 0, "shared memory of a CTA");
+  static_assert(C::SMEM <= 226 * 1024 && KB * C::NC % LOADERS == 0 && C::Q_COL + HD / 2 <= 512 && SCALES >= C::STAGES + 2, "shared memory of a CTA");
   static std::atomic<unsigned long long> configured{0};   // a bit per device
   int dev = 0;
   MESH_CUDA_OK(cudaGetDevice(&dev));
