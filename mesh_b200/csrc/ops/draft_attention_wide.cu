@@ -2,17 +2,18 @@
 //
 // A tile is 128 query rows of one (sequence, KV head); a CTA goes through its stretches of 64-key blocks (how the work is cut and
 // the formulas: draft_attention.cuh, draft_attention.cu).  Warps 0-3: softmax, a thread per query row.  Warps 4-11: keys and
-// values, loaded into registers four tiles ahead of their turn, widened (8-bit codes to fp16) and stored to shared memory in the
-// 128-byte swizzle of the operands.  Warp 12: the products S = Q K^T and O += P V by one elected lane, S of the next block
-// before P V of this one.  Tensor memory holds the queries (operand A of the first product, 16 bits), S twice, of which P (16
-// bits, operand A of the second) overwrites the first half, and O, which is rescaled only when a row's maximum has grown by
-// more than 2^8.
+// values, in the 128-byte swizzle of the operands: bf16 rows copied to their place by cp.async, 8-bit codes copied to a
+// staging ring and widened to fp16 from there, every thread the pieces that it has copied itself.  Warp 12: the products
+// S = Q K^T and O += P V by one elected lane, S of the next block before P V of this one.  Tensor memory holds the queries
+// (operand A of the first product, 16 bits), S twice, of which P (16 bits, operand A of the second) overwrites the first
+// half, and O, which is rescaled only when a row's maximum has grown by more than 2^8.
 //
-// Codes are widened once per 128 rows, in registers: as operands of a product in 8 bits the queries and probabilities would have to be
-// rounded to 8 bits too.  Queries in tensor memory leave shared memory to three tiles of keys and three of values with heads
-// of 256, and its bandwidth to their stores and reads.  What was slower, at 64 drafts x 4 heads over four contexts of
-// 20000-32704 keys of 256 in 8 bits: blocks of 128 keys with the queries in shared memory, where one tile of keys and one of
-// values fit and the registers one tile ahead, 126 us; the same with scores read twice from tensor memory, 165 us.
+// Codes are widened once per 128 rows: as operands of a product in 8 bits the queries and probabilities would have to be rounded to 8
+// bits too.  Queries in tensor memory leave shared memory to the rings and its bandwidth to their stores and reads.  What
+// was slower, at 64 drafts x 4 heads over four contexts of 20000-32704 keys of 256 in 8 bits: tiles held in registers ahead
+// of their turn, whose unrolled code did not stay in the instruction cache, 138 us (a tile took 1400 cycles to store, one
+// of 16-bit rows hardly fewer); blocks of 128 keys with the queries in shared memory, 126 us; the same with scores read
+// twice from tensor memory, 165 us.
 #include "draft_attention.cuh"
 
 namespace mesh {
@@ -27,15 +28,26 @@ constexpr int SCALES = 8;                                   // blocks whose scal
 template <int HD, bool Q8>
 struct Wide {
   static constexpr int TILE = KB * HD * 2;
-  static constexpr int STAGES = HD == 256 ? 3 : 4;
+  static constexpr int STAGES = HD < 256 ? 4 : Q8 ? 2 : 3;
   static constexpr int RB = Q8 ? HD : 2 * HD, NC = RB / 16;           // bytes and 16-byte pieces of a stored row
   static constexpr int VPT = KB * NC / LOADERS;             // pieces of a loader thread per tile
-  static constexpr int DEPTH = VPT >= 4 ? 16 / VPT : 4;     // tiles in registers
+  // Tiles under way.  A copy into a ring's place waits for the product that reads it, which may need any tile up to LAG ones before:
+  // at most two fewer than both rings hold, or the loaders would wait for what they have not handed over.
+  static constexpr int LAG = Q8 ? (HD < 256 ? 8 : 4) : 2 * STAGES - 2;
+  static constexpr int RAW = Q8 ? KB * HD + 2 * KB * 4 : 0, STAGING = LAG * RAW;     // codes, and for keys both scales
   static constexpr int N_BARS = 1 + 4 * STAGES + 2 + 2 + 2 + SCALES;
   static constexpr int SCALE_BYTES = Q8 ? SCALES * 3 * KB * 4 : 0;
-  static constexpr int SMEM = 2 * STAGES * TILE + SCALE_BYTES + 8 * N_BARS + 64 + 1024;
+  static constexpr int SMEM = 2 * STAGES * TILE + STAGING + SCALE_BYTES + 8 * N_BARS + 64 + 1024;
   static constexpr int S_COL = 0, O_COL = 2 * KB, Q_COL = O_COL + HD;  // columns of tensor memory
 };
+
+// 16 bytes, or zeros where `there` is false; 4 bytes.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
+}
 
 // two fp32 at a time
 struct F2 { unsigned long long v; };
@@ -86,14 +98,14 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
-  const uint32_t sK = base, sV = sK + STAGES * C::TILE, sScale = sV + STAGES * C::TILE, bars = sScale + C::SCALE_BYTES;
+  const uint32_t sK = base, sV = sK + STAGES * C::TILE, sRaw = sV + STAGES * C::TILE, sScale = sRaw + C::STAGING, bars = sScale + C::SCALE_BYTES;
   float* scale_s = reinterpret_cast<float*>(gen + (sScale - base));        // [buffer]{key scale, lg2 of the value scale, value scale}[key]
   auto bar = [&](int i) { return bars + 8u * i; };
   constexpr int Q_FULL = 0, K_FULL = 1, K_EMPTY = K_FULL + STAGES, V_FULL = K_EMPTY + STAGES, V_EMPTY = V_FULL + STAGES,
                 S_FULL = V_EMPTY + STAGES, P_FULL = S_FULL + 2, O_DONE = P_FULL + 2, SC_FULL = O_DONE + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen + (bars - base) + 8 * C::N_BARS);
   volatile int* abort_smem = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  volatile int* spoilt_s = reinterpret_cast<volatile int*>(tmem_slot + 2);     // [4]: stretch + 1 whose values had to be cleaned
+  volatile int* spoilt_s = reinterpret_cast<volatile int*>(tmem_slot + 2);     // [4]: the stretch (of 64 in turn, + 1) whose values had to be cleaned
   __shared__ Walk walk_s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = a.q_heads / a.kv_heads;
 
@@ -132,51 +144,75 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
 
   if (warp >= LOAD_WARP && warp < PRODUCT_WARP) {
     // ------------------------------------------------------------------ keys and values
-    // Per stretch, in the order the products take them: K0 K1 V0 K2 V1 ...  `load` fetches the next tile into a set of
-    // registers, `store` puts the oldest set into its place when that is free.
+    // Per stretch, in the order the products take them: K0 K1 V0 K2 V1 ...  `issue` starts the copies of a tile, `finish` hands over the
+    // one issued LAG - 1 tiles before.
     const int lt = threadIdx.x - SOFT;
-    uint4 raw[C::DEPTH][VPT];
-    float scale[C::DEPTH];                                // of key lt or of value lt - 64
-    int what[C::DEPTH];                                   // 0 nothing, 1 key, 2 value, 3 value to be cleaned
-    int stretch_of[C::DEPTH];
     int blocks = 0, kj = 0, vj = 0, stretch = -1;
+    int issued_k = 0, issued_v = 0, done_k = 0, done_v = 0, slot = 0, under_way = 0;
     bool more = true;
-    auto load = [&](int d) {
-      what[d] = 0;
+    const uint8_t* k_src = nullptr;
+    const uint8_t* v_src = nullptr;
+    long long scale_at = 0;
+    unsigned long long what = 0;                          // of the tiles under way, 8 bits each: key, to be cleaned, stretch & 63
+    auto issue = [&]() {
       while (more && kj >= blocks && vj >= blocks) {
         more = next(a, walk, x);
         ++stretch;
         kj = vj = 0;
         blocks = more ? blocks_of(x) : 0;
+        scale_at = ((long long)x.b * a.kv_heads + x.hk) * a.max_seq + x.k_lo;
+        k_src = a.k + scale_at * C::RB + lt * 16;
+        v_src = a.v + scale_at * C::RB + lt * 16;
       }
-      if (!more) return;
-      const bool key = kj < blocks && kj <= vj + 1;
-      const int j = key ? kj++ : vj++, slot0 = x.k_lo + j * KB, rows = min(x.k_hi - slot0, KB);
-      const long long at = ((long long)x.b * a.kv_heads + x.hk) * a.max_seq + slot0;
-      const uint4* src = reinterpret_cast<const uint4*>((key ? a.k : a.v) + at * C::RB) + lt;
-#pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        raw[d][i] = make_uint4(0, 0, 0, 0);               // behind the last slot: what a hidden row holds is not read
-        if ((i * LOADERS + lt) / NC < rows) raw[d][i] = __ldcg(src + i * LOADERS);
-      }
-      if (Q8 && key && lt < 2 * KB) scale[d] = lt % KB < rows ? __ldcg((lt < KB ? a.k_scale : a.v_scale) + at + lt % KB) : 0.f;
-      what[d] = key ? 1 : !Q8 && masked_block(a, x, slot0) ? 3 : 2;
-      stretch_of[d] = stretch;
-    };
-    int nk = 0, nv = 0;                                   // tiles stored
-    auto store = [&](int d) {
-      const bool key = what[d] == 1;
-      const int n = key ? nk++ : nv++, s = n % STAGES;
-      if (n >= STAGES) ok = mbar_wait(bar((key ? K_EMPTY : V_EMPTY) + s), (n / STAGES - 1) & 1, abort_smem, a.status, SITE_SMEM_EMPTY);
-      if (!ok) return;
-      const uint32_t dst = (key ? sK : sV) + s * C::TILE - base;
-      bool spoilt = false;
-#pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        const int idx = i * LOADERS + lt, r = idx / NC, c = idx % NC;
-        uint4 v = raw[d][i];
+      what <<= 8;
+      if (more) {
+        const bool key = kj < blocks && kj <= vj + 1;
+        const int j = key ? kj++ : vj++, rows = x.k_hi - (x.k_lo + j * KB);
+        const uint8_t* src = (key ? k_src : v_src) + (long long)j * (KB * C::RB);
         if (Q8) {
-          uint8_t* p = gen + dst + (c >> 2) * (KB * 128) + r * 128;
+          const uint32_t dst = sRaw + slot * C::RAW;
+#pragma unroll
+          for (int i = 0; i < VPT; ++i) {
+            const bool there = (i * LOADERS + lt) / NC < rows;            // behind the last slot: what a hidden row holds is not read
+            copy16(dst + (i * LOADERS + lt) * 16, src + (there ? i * LOADERS * 16 : -lt * 16), there);
+          }
+          if (key && lt < 2 * KB) {
+            const bool there = lt % KB < rows;
+            copy4(dst + KB * HD + lt * 4, (lt < KB ? a.k_scale : a.v_scale) + scale_at + j * KB + (there ? lt % KB : 0), there);
+          }
+          what |= key ? 1u : 0u;
+        } else {
+          const int n = key ? issued_k++ : issued_v++, s = n % STAGES;
+          if (n >= STAGES) ok = mbar_wait(bar((key ? K_EMPTY : V_EMPTY) + s), (n / STAGES - 1) & 1, abort_smem, a.status, SITE_SMEM_EMPTY);
+          if (ok) {
+            const uint32_t dst = (key ? sK : sV) + s * C::TILE;
+#pragma unroll
+            for (int i = 0; i < VPT; ++i) {
+              const int idx = i * LOADERS + lt, r = idx / NC, c = idx % NC;
+              copy16(dst + (c >> 3) * (KB * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4), src + (r < rows ? i * LOADERS * 16 : -lt * 16), r < rows);
+            }
+          }
+          what |= (key ? 1u : 0u) | (!key && masked_block(a, x, x.k_lo + j * KB) ? 2u : 0u) | (uint32_t)(stretch & 63) << 2;
+        }
+        ++under_way;
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    auto finish = [&](int slot) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(C::LAG - 1) : "memory");
+      const uint32_t kind = (uint32_t)(what >> (8 * (C::LAG - 1))) & 255u;
+      const bool key = kind & 1u;
+      const int n = key ? done_k++ : done_v++, s = n % STAGES;
+      if (Q8) {
+        if (n >= STAGES) ok = mbar_wait(bar((key ? K_EMPTY : V_EMPTY) + s), (n / STAGES - 1) & 1, abort_smem, a.status, SITE_SMEM_EMPTY);
+        if (!ok) return;
+        const uint8_t* raw = gen + (sRaw - base) + slot * C::RAW;
+        uint8_t* dst = gen + ((key ? sK : sV) + s * C::TILE - base);
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+          const int idx = i * LOADERS + lt, r = idx / NC, c = idx % NC;
+          const uint4 v = *reinterpret_cast<const uint4*>(raw + idx * 16);
+          uint8_t* p = dst + (c >> 2) * (KB * 128) + r * 128;
           const uint32_t w[4] = {v.x ^ 0x80808080u, v.y ^ 0x80808080u, v.z ^ 0x80808080u, v.w ^ 0x80808080u};
           const uint4 lo = make_uint4(codes2(w[0], 0x4140), codes2(w[0], 0x4342), codes2(w[1], 0x4140), codes2(w[1], 0x4342));
           const uint4 hi = make_uint4(codes2(w[2], 0x4140), codes2(w[2], 0x4342), codes2(w[3], 0x4140), codes2(w[3], 0x4342));
@@ -184,39 +220,49 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
           const int odd = c >> 2 & 1, c0 = 2 * (c & 3);
           *reinterpret_cast<uint4*>(p + (((c0 + odd) ^ (r & 7)) << 4)) = odd ? hi : lo;
           *reinterpret_cast<uint4*>(p + (((c0 + 1 - odd) ^ (r & 7)) << 4)) = odd ? lo : hi;
-        } else {
-          if (what[d] == 3 && (not_finite(v.x) || not_finite(v.y) || not_finite(v.z) || not_finite(v.w))) {
-            // zero times a NaN or an infinity is not zero: hidden keys must not hold any.  Rows that see them get them at the end.
-            v = make_uint4(finite_or_zero(v.x), finite_or_zero(v.y), finite_or_zero(v.z), finite_or_zero(v.w));
+        }
+        if (key) {
+          if (lt < 2 * KB) {
+            const float f = *reinterpret_cast<const float*>(raw + KB * HD + lt * 4);
+            float* sc = scale_s + (n % SCALES) * 3 * KB + lt % KB;
+            if (lt < KB) {
+              sc[0] = f;
+            } else {
+              sc[KB] = fmaxf(lg2(f), -60.f);
+              sc[2 * KB] = f;
+            }
+          }
+          mbar_arrive(bar(SC_FULL + n % SCALES));
+        }
+      } else if (kind & 2u) {
+        // zero times a NaN or an infinity is not zero: hidden keys must not hold any.  Rows that see them get them at the end.
+        uint8_t* dst = gen + (sV + s * C::TILE - base);
+        bool spoilt = false;
+#pragma unroll 1
+        for (int i = 0; i < VPT; ++i) {
+          const int idx = i * LOADERS + lt, r = idx / NC, c = idx % NC;
+          uint4* p = reinterpret_cast<uint4*>(dst + (c >> 3) * (KB * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+          const uint4 v = *p;
+          if (not_finite(v.x) || not_finite(v.y) || not_finite(v.z) || not_finite(v.w)) {
+            *p = make_uint4(finite_or_zero(v.x), finite_or_zero(v.y), finite_or_zero(v.z), finite_or_zero(v.w));
             spoilt = true;
           }
-          *reinterpret_cast<uint4*>(gen + dst + (c >> 3) * (KB * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
         }
-      }
-      if (!Q8 && spoilt) spoilt_s[stretch_of[d] & 3] = stretch_of[d] + 1;
-      if (Q8 && key) {
-        float* sc = scale_s + (n % SCALES) * 3 * KB + lt % KB;
-        if (lt < KB) {
-          sc[0] = scale[d];
-        } else if (lt < 2 * KB) {
-          sc[KB] = fmaxf(lg2(scale[d]), -60.f);
-          sc[2 * KB] = scale[d];
-        }
-        mbar_arrive(bar(SC_FULL + n % SCALES));
+        if (spoilt) spoilt_s[kind >> 2 & 3] = (int)(kind >> 2) + 1;
       }
       fence_proxy_async_smem();
       mbar_arrive(bar((key ? K_FULL : V_FULL) + s));
     };
-#pragma unroll
-    for (int d = 0; d < C::DEPTH; ++d) load(d);
-    while (ok && what[0]) {
-#pragma unroll
-      for (int d = 0; d < C::DEPTH; ++d) {
-        if (ok && what[d]) {
-          store(d);
-          if (ok) load(d);
-        }
+    for (int o = 0; ok; ++o) {
+      issue();
+      if (!ok) break;
+      const int oldest = slot + 1 == C::LAG ? 0 : slot + 1;              // the place of the tile LAG - 1 before
+      if (o >= C::LAG - 1) {
+        if (under_way == 0) break;
+        finish(oldest);
+        --under_way;
       }
+      slot = oldest;
     }
   } else if (warp == PRODUCT_WARP) {
     // ------------------------------------------------------------------ products (warp-uniform, one elected lane issues)
@@ -449,7 +495,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
         tc_fence_after();
       }
       if (!works) continue;
-      const bool spoilt = !Q8 && spoilt_s[stretch & 3] == stretch + 1;
+      const bool spoilt = !Q8 && spoilt_s[stretch & 3] == (stretch & 63) + 1;
       const float inv = !x.whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
       __nv_bfloat16* dst = a.out + x.b * a.o_sb + t * a.o_st + (long long)h * HD;
       const bool vec = (reinterpret_cast<uintptr_t>(dst) & 15) == 0;
@@ -571,7 +617,7 @@ __global__ void __launch_bounds__(GROUPS * TT) wide_join_kernel(const __grid_con
 template <int HD, bool Q8>
 int run(const Args& p, void* stream) {
   using C = Wide<HD, Q8>;
-  static_assert(C::SMEM <= 226 * 1024 && KB * C::NC % LOADERS == 0 && C::Q_COL + HD / 2 <= 512 && SCALES >= C::STAGES + 2, "shared memory of a CTA");
+  static_assert(C::SMEM <= 226 * 1024 && KB * C::NC % LOADERS == 0 && C::Q_COL + HD / 2 <= 512 && SCALES >= C::STAGES + 2 && C::LAG <= 8, "shared memory of a CTA");
   static std::atomic<unsigned long long> configured{0};   // a bit per device
   int dev = 0;
   MESH_CUDA_OK(cudaGetDevice(&dev));
