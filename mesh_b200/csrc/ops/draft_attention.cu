@@ -105,8 +105,8 @@ __global__ void __launch_bounds__(Cfg<HD, Q8>::WARPS * 32, 1) attention_kernel(c
   if (warp == 0) begin_walk(a, &walk_s);
   __syncthreads();
   Walk walk = walk_s;
-  Stretch x;
-  while (next(a, walk, x)) {
+  for (Stretch y; next(a, walk, y);) {
+  const Stretch x = y;
   const Seq s = x.s;
   const int b = x.b, hk = x.hk, tile = x.tile, n_rows = x.n_rows, k_lo = x.k_lo, k_hi = x.k_hi;
   const int blocks = (k_hi - k_lo + KEYS - 1) / KEYS;

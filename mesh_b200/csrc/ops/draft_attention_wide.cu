@@ -1,19 +1,20 @@
 // Attention of drafts with many query rows (more than 16 drafts times heads of a group) on the 5th-generation tensor cores.
 //
 // A tile is 128 query rows of one (sequence, KV head); a CTA goes through its stretches of 64-key blocks (how the work is cut and
-// the formulas: draft_attention.cuh, draft_attention.cu).  Warps 0-3: softmax, a thread per query row.  Warps 4-11: keys and
-// values, in the 128-byte swizzle of the operands: bf16 rows copied to their place by cp.async, 8-bit codes copied to a
-// staging ring and widened to fp16 from there, every thread the pieces that it has copied itself.  Warp 12: the products
+// the formulas: draft_attention.cuh, draft_attention.cu).  Warps 0-7: softmax, two threads per query row with half of the block's keys
+// each.  Warps 8-14: keys and values, a warp per 4 KB of a tile, into the 128-byte swizzle of the operands: bf16 rows by
+// cp.async; 8-bit codes copied in bulk to places of the warp's own and widened to fp16 from there.  Warp 15: the products
 // S = Q K^T and O += P V by one elected lane, S of the next block before P V of this one.  Tensor memory holds the queries
 // (operand A of the first product, 16 bits), S twice, of which P (16 bits, operand A of the second) overwrites the first
 // half, and O, which is rescaled only when a row's maximum has grown by more than 2^8.
 //
 // Codes are widened once per 128 rows: as operands of a product in 8 bits the queries and probabilities would have to be rounded to 8
-// bits too.  Queries in tensor memory leave shared memory to the rings and its bandwidth to their stores and reads.  What
-// was slower, at 64 drafts x 4 heads over four contexts of 20000-32704 keys of 256 in 8 bits: tiles held in registers ahead
-// of their turn, whose unrolled code did not stay in the instruction cache, 138 us (a tile took 1400 cycles to store, one
-// of 16-bit rows hardly fewer); blocks of 128 keys with the queries in shared memory, 126 us; the same with scores read
-// twice from tensor memory, 165 us.
+// bits too.  Queries in tensor memory leave shared memory to the rings and its bandwidth to their stores and reads.  The
+// roles run different code on the same SM, so it is kept short: with the waits' error paths and the cutting of the work
+// inlined everywhere (112 KB) and tiles held in registers (unrolled twice), one instruction fetch in six missed the cache.
+// What was slower, at 64 drafts x 4 heads over four contexts of 20000-32704 keys of 256 in 8 bits: that, 125 us; all loader
+// threads at every tile through cp.async, with one softmax thread per row, 117; blocks of 128 keys with the queries in
+// shared memory, 126; scores read twice from tensor memory, 165.
 #include "draft_attention.cuh"
 
 namespace mesh {
@@ -21,32 +22,43 @@ namespace draft {
 namespace {
 
 constexpr int TT = WIDE_ROWS, KB = WIDE_UNIT;               // rows of a tile, keys of a block
-constexpr int SOFT = 128, LOADERS = 256, THREADS = SOFT + LOADERS + 32;
-constexpr int LOAD_WARP = SOFT / 32, PRODUCT_WARP = (SOFT + LOADERS) / 32;
+constexpr int SOFT = 256, LOAD_WARPS = 7, THREADS = SOFT + 32 * LOAD_WARPS + 32;
+constexpr int LOAD_WARP = SOFT / 32, PRODUCT_WARP = LOAD_WARP + LOAD_WARPS;
 constexpr int SCALES = 8;                                   // blocks whose scales are kept: two more than there are stages, at least
+constexpr int CHUNK = 4096, PIECES = CHUNK / (32 * 16);     // bytes of stored rows a warp takes at a time; 16-byte pieces of a lane
 
 template <int HD, bool Q8>
 struct Wide {
   static constexpr int TILE = KB * HD * 2;
   static constexpr int STAGES = HD < 256 ? 4 : Q8 ? 2 : 3;
   static constexpr int RB = Q8 ? HD : 2 * HD, NC = RB / 16;           // bytes and 16-byte pieces of a stored row
-  static constexpr int VPT = KB * NC / LOADERS;             // pieces of a loader thread per tile
-  // Tiles under way.  A copy into a ring's place waits for the product that reads it, which may need any tile up to LAG ones before:
-  // at most two fewer than both rings hold, or the loaders would wait for what they have not handed over.
-  static constexpr int LAG = Q8 ? (HD < 256 ? 8 : 4) : 2 * STAGES - 2;
-  static constexpr int RAW = Q8 ? KB * HD + 2 * KB * 4 : 0, STAGING = LAG * RAW;     // codes, and for keys both scales
-  static constexpr int N_BARS = 1 + 4 * STAGES + 2 + 2 + 2 + SCALES;
+  static constexpr int CPT = KB * RB / CHUNK;               // chunks of a tile
+  // Chunks of bf16 rows that a warp has under way beside the newest, which may wait for a product that needs any tile up to
+  // 2 STAGES - 1 before its own: the oldest must lie further back no more than that.
+  static constexpr int BEHIND = CPT >= 4 ? 2 : 1;
+  static_assert(Q8 || BEHIND * LOAD_WARPS < (2 * STAGES - 1) * CPT, "a loader would wait for what it has not handed over");
+  static constexpr int RAWS = Q8 ? 3 : 0;                   // chunks of codes that a warp has under way
+  static constexpr int N_BARS = 1 + 4 * STAGES + 2 + 2 + 2 + SCALES + RAWS * LOAD_WARPS;
   static constexpr int SCALE_BYTES = Q8 ? SCALES * 3 * KB * 4 : 0;
-  static constexpr int SMEM = 2 * STAGES * TILE + STAGING + SCALE_BYTES + 8 * N_BARS + 64 + 1024;
+  static constexpr int SMEM = 2 * STAGES * TILE + RAWS * LOAD_WARPS * CHUNK + SCALE_BYTES + 8 * N_BARS + 64 + 1024;
   static constexpr int S_COL = 0, O_COL = 2 * KB, Q_COL = O_COL + HD;  // columns of tensor memory
 };
 
-// 16 bytes, or zeros where `there` is false; 4 bytes.
+// Once, not in every role: its divisions are long.
+__device__ __noinline__ bool next_stretch(const Args& a, Walk& w, Stretch& x) { return next(a, w, x); }
+
+// The waits' slow path, once: a bounded wait, see mbar_wait.
+__device__ __noinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile int* abort_smem, Status* st, int site) {
+  return mbar_wait(bar, parity, abort_smem, st, site);
+}
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_smem, Status* st, int site) {
+  bool ok = mbar_try_wait(bar, parity);
+  if (!__all_sync(0xffffffffu, ok)) ok = __all_sync(0xffffffffu, wait_on(bar, parity, abort_smem, st, site));
+  return ok;
+}
+// 16 bytes, or zeros where `there` is false.
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void copy4(uint32_t dst, const void* src, bool there) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
 }
 
 // two fp32 at a time
@@ -91,29 +103,61 @@ __device__ __forceinline__ uint32_t finite_or_zero(uint32_t w) {
   return ((w & 0x7f80u) == 0x7f80u ? 0u : w & 0xffffu) | ((w & 0x7f800000u) == 0x7f800000u ? 0u : w & 0xffff0000u);
 }
 
+// Where the tiles of keys and values lie.  Per stretch they come in the order the products take them: K0 K1 V0 K2 V1 ... V(last).
+struct Tiles {
+  Walk walk;
+  Stretch x;
+  int first = 0, blocks = 0, n0 = 0, stretch = -1;        // tiles before this stretch, its blocks, blocks before it
+  long long at = 0;                                       // row of its first slot
+  bool key = false;
+  int j = 0;                                              // block within the stretch
+  // Tile o of all, not before the last one asked for; false behind the last.
+  __device__ __forceinline__ bool find(const Args& a, int o) {
+    while (o - first >= 2 * blocks) {
+      first += 2 * blocks;
+      n0 += blocks;
+      blocks = 0;
+      Stretch y;
+      if (!next_stretch(a, walk, y)) return false;
+      x = y;
+      ++stretch;
+      blocks = blocks_of(x);
+      at = ((long long)x.b * a.kv_heads + x.hk) * a.max_seq + x.k_lo;
+    }
+    o -= first;
+    key = o == 0 || ((o & 1) && o < 2 * blocks - 1);
+    j = key ? (o + 1) / 2 : o == 2 * blocks - 1 ? blocks - 1 : o / 2 - 1;
+    return true;
+  }
+  __device__ __forceinline__ int n() const { return n0 + j; }                              // block of all
+  __device__ __forceinline__ int slot() const { return x.k_lo + j * KB; }
+  __device__ __forceinline__ int rows() const { return x.k_hi - slot(); }                  // of the tile, if fewer than KB
+};
+
 template <int HD, bool Q8>
 __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant__ Args a) {
   using C = Wide<HD, Q8>;
-  constexpr int STAGES = C::STAGES, VPT = C::VPT, NC = C::NC;
+  constexpr int STAGES = C::STAGES, NC = C::NC;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
-  const uint32_t sK = base, sV = sK + STAGES * C::TILE, sRaw = sV + STAGES * C::TILE, sScale = sRaw + C::STAGING, bars = sScale + C::SCALE_BYTES;
+  const uint32_t sK = base, sV = sK + STAGES * C::TILE, sRaw = sV + STAGES * C::TILE, sScale = sRaw + C::RAWS * LOAD_WARPS * CHUNK, bars = sScale + C::SCALE_BYTES;
   float* scale_s = reinterpret_cast<float*>(gen + (sScale - base));        // [buffer]{key scale, lg2 of the value scale, value scale}[key]
   auto bar = [&](int i) { return bars + 8u * i; };
   constexpr int Q_FULL = 0, K_FULL = 1, K_EMPTY = K_FULL + STAGES, V_FULL = K_EMPTY + STAGES, V_EMPTY = V_FULL + STAGES,
-                S_FULL = V_EMPTY + STAGES, P_FULL = S_FULL + 2, O_DONE = P_FULL + 2, SC_FULL = O_DONE + 2;
+                S_FULL = V_EMPTY + STAGES, P_FULL = S_FULL + 2, O_DONE = P_FULL + 2, SC_FULL = O_DONE + 2, RAW_FULL = SC_FULL + SCALES;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen + (bars - base) + 8 * C::N_BARS);
   volatile int* abort_smem = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  volatile int* spoilt_s = reinterpret_cast<volatile int*>(tmem_slot + 2);     // [4]: the stretch (of 64 in turn, + 1) whose values had to be cleaned
+  volatile int* spoilt_s = reinterpret_cast<volatile int*>(tmem_slot + 2);     // [8]: stretch + 1 whose values had to be cleaned; loaders are at most 5 stretches ahead
   __shared__ Walk walk_s;
+  __shared__ float top_s[2][2][TT], sum_s[2][TT];           // [block & 1][half][row], [half][row]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = a.q_heads / a.kv_heads;
 
   if (threadIdx.x == 0) {
     mbar_init(bar(Q_FULL), SOFT);
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(bar(K_FULL + s), LOADERS);
-      mbar_init(bar(V_FULL + s), LOADERS);
+      mbar_init(bar(K_FULL + s), C::CPT);
+      mbar_init(bar(V_FULL + s), C::CPT);
       mbar_init(bar(K_EMPTY + s), 1);
       mbar_init(bar(V_EMPTY + s), 1);
     }
@@ -122,9 +166,10 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
       mbar_init(bar(P_FULL + s), SOFT);
       mbar_init(bar(O_DONE + s), 1);
     }
-    for (int s = 0; s < SCALES; ++s) mbar_init(bar(SC_FULL + s), LOADERS);
+    for (int s = 0; s < SCALES; ++s) mbar_init(bar(SC_FULL + s), 1);
+    for (int s = 0; s < C::RAWS * LOAD_WARPS; ++s) mbar_init(bar(RAW_FULL + s), 1);
     *abort_smem = 0;
-    for (int s = 0; s < 4; ++s) spoilt_s[s] = 0;
+    for (int s = 0; s < 8; ++s) spoilt_s[s] = 0;
     fence_mbar_init();
   }
   if (warp == PRODUCT_WARP) {
@@ -144,74 +189,54 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
 
   if (warp >= LOAD_WARP && warp < PRODUCT_WARP) {
     // ------------------------------------------------------------------ keys and values
-    // Per stretch, in the order the products take them: K0 K1 V0 K2 V1 ...  `issue` starts the copies of a tile, `finish` hands over the
-    // one issued LAG - 1 tiles before.
-    const int lt = threadIdx.x - SOFT;
-    int blocks = 0, kj = 0, vj = 0, stretch = -1;
-    int issued_k = 0, issued_v = 0, done_k = 0, done_v = 0, slot = 0, under_way = 0;
-    bool more = true;
-    const uint8_t* k_src = nullptr;
-    const uint8_t* v_src = nullptr;
-    long long scale_at = 0;
-    unsigned long long what = 0;                          // of the tiles under way, 8 bits each: key, to be cleaned, stretch & 63
-    auto issue = [&]() {
-      while (more && kj >= blocks && vj >= blocks) {
-        more = next(a, walk, x);
-        ++stretch;
-        kj = vj = 0;
-        blocks = more ? blocks_of(x) : 0;
-        scale_at = ((long long)x.b * a.kv_heads + x.hk) * a.max_seq + x.k_lo;
-        k_src = a.k + scale_at * C::RB + lt * 16;
-        v_src = a.v + scale_at * C::RB + lt * 16;
-      }
-      what <<= 8;
-      if (more) {
-        const bool key = kj < blocks && kj <= vj + 1;
-        const int j = key ? kj++ : vj++, rows = x.k_hi - (x.k_lo + j * KB);
-        const uint8_t* src = (key ? k_src : v_src) + (long long)j * (KB * C::RB);
-        if (Q8) {
-          const uint32_t dst = sRaw + slot * C::RAW;
-#pragma unroll
-          for (int i = 0; i < VPT; ++i) {
-            const bool there = (i * LOADERS + lt) / NC < rows;            // behind the last slot: what a hidden row holds is not read
-            copy16(dst + (i * LOADERS + lt) * 16, src + (there ? i * LOADERS * 16 : -lt * 16), there);
-          }
-          if (key && lt < 2 * KB) {
-            const bool there = lt % KB < rows;
-            copy4(dst + KB * HD + lt * 4, (lt < KB ? a.k_scale : a.v_scale) + scale_at + j * KB + (there ? lt % KB : 0), there);
-          }
-          what |= key ? 1u : 0u;
-        } else {
-          const int n = key ? issued_k++ : issued_v++, s = n % STAGES;
-          if (n >= STAGES) ok = mbar_wait(bar((key ? K_EMPTY : V_EMPTY) + s), (n / STAGES - 1) & 1, abort_smem, a.status, SITE_SMEM_EMPTY);
-          if (ok) {
-            const uint32_t dst = (key ? sK : sV) + s * C::TILE;
-#pragma unroll
-            for (int i = 0; i < VPT; ++i) {
-              const int idx = i * LOADERS + lt, r = idx / NC, c = idx % NC;
-              copy16(dst + (c >> 3) * (KB * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4), src + (r < rows ? i * LOADERS * 16 : -lt * 16), r < rows);
-            }
-          }
-          what |= (key ? 1u : 0u) | (!key && masked_block(a, x, x.k_lo + j * KB) ? 2u : 0u) | (uint32_t)(stretch & 63) << 2;
-        }
-        ++under_way;
-      }
-      asm volatile("cp.async.commit_group;" ::: "memory");
+    // Chunk q of all is warp q mod LOAD_WARPS's.
+    Tiles t;
+    t.walk = walk;
+    const int w0 = warp - LOAD_WARP;
+    // A warp may pass a place's phases unseen; but its chunk before, LOAD_WARPS chunks back, waited for a product that comes
+    // after the one two phases back, so the phase before cannot answer.
+    auto place_free = [&]() {
+      return t.n() < STAGES ||
+             wait_warp(bar((t.key ? K_EMPTY : V_EMPTY) + t.n() % STAGES), (t.n() / STAGES - 1) & 1, abort_smem, a.status, SITE_SMEM_EMPTY);
     };
-    auto finish = [&](int slot) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(C::LAG - 1) : "memory");
-      const uint32_t kind = (uint32_t)(what >> (8 * (C::LAG - 1))) & 255u;
-      const bool key = kind & 1u;
-      const int n = key ? done_k++ : done_v++, s = n % STAGES;
-      if (Q8) {
-        if (n >= STAGES) ok = mbar_wait(bar((key ? K_EMPTY : V_EMPTY) + s), (n / STAGES - 1) & 1, abort_smem, a.status, SITE_SMEM_EMPTY);
-        if (!ok) return;
-        const uint8_t* raw = gen + (sRaw - base) + slot * C::RAW;
-        uint8_t* dst = gen + ((key ? sK : sV) + s * C::TILE - base);
+    if (Q8) {
+      constexpr int RAWS = C::RAWS ? C::RAWS : 1;
+      Tiles ahead = t;
+      const uint32_t own = sRaw + w0 * (RAWS * CHUNK), own_full = bar(RAW_FULL) + 8 * w0 * RAWS;
+      auto fetch = [&](int q, int place) {                // starts the copy of a chunk; what lies behind the last slot is not read
+        if (!ahead.find(a, q / C::CPT)) return;
+        const int part = q % C::CPT, bytes = min(max(ahead.rows() * C::RB - part * CHUNK, 0), CHUNK);
+        if (lane == 0) {
+          mbar_expect_tx(own_full + 8 * place, bytes);
+          if (bytes)
+            bulk_load_1d(own + place * CHUNK, (ahead.key ? a.k : a.v) + (ahead.at + ahead.j * KB) * C::RB + part * CHUNK, bytes, own_full + 8 * place);
+        }
+      };
+#pragma unroll 1
+      for (int i = 0; i < RAWS; ++i) fetch(w0 + i * LOAD_WARPS, i);
+      int place = 0, phase = 0;
+#pragma unroll 1
+      for (int q = w0; ok && t.find(a, q / C::CPT); q += LOAD_WARPS) {
+        const int part = q % C::CPT, s = t.n() % STAGES, rows = t.rows();
+        const bool scales = t.key && part == 0;
+        float f[4];                                       // scales of keys lane, lane + 32 and their values
+        if (scales) {
+          const long long row = t.at + t.j * KB + lane;
 #pragma unroll
-        for (int i = 0; i < VPT; ++i) {
-          const int idx = i * LOADERS + lt, r = idx / NC, c = idx % NC;
-          const uint4 v = *reinterpret_cast<const uint4*>(raw + idx * 16);
+          for (int i = 0; i < 2; ++i) {
+            f[i] = lane + 32 * i < rows ? __ldcg(a.k_scale + row + 32 * i) : 0.f;
+            f[2 + i] = lane + 32 * i < rows ? __ldcg(a.v_scale + row + 32 * i) : 0.f;
+          }
+        }
+        ok = wait_warp(own_full + 8 * place, phase, abort_smem, a.status, SITE_SMEM_FULL) && place_free();
+        if (!ok) break;
+        const uint8_t* src = gen + (own - base) + place * CHUNK;
+        uint8_t* dst = gen + ((t.key ? sK : sV) + s * C::TILE - base);
+#pragma unroll 4
+        for (int i = 0; i < PIECES; ++i) {
+          const int idx = part * (CHUNK / 16) + i * 32 + lane, r = idx / NC, c = idx % NC;
+          uint4 v = *reinterpret_cast<const uint4*>(src + (i * 32 + lane) * 16);
+          if (r >= rows) v = make_uint4(0, 0, 0, 0);
           uint8_t* p = dst + (c >> 2) * (KB * 128) + r * 128;
           const uint32_t w[4] = {v.x ^ 0x80808080u, v.y ^ 0x80808080u, v.z ^ 0x80808080u, v.w ^ 0x80808080u};
           const uint4 lo = make_uint4(codes2(w[0], 0x4140), codes2(w[0], 0x4342), codes2(w[1], 0x4140), codes2(w[1], 0x4342));
@@ -221,48 +246,82 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
           *reinterpret_cast<uint4*>(p + (((c0 + odd) ^ (r & 7)) << 4)) = odd ? hi : lo;
           *reinterpret_cast<uint4*>(p + (((c0 + 1 - odd) ^ (r & 7)) << 4)) = odd ? lo : hi;
         }
-        if (key) {
-          if (lt < 2 * KB) {
-            const float f = *reinterpret_cast<const float*>(raw + KB * HD + lt * 4);
-            float* sc = scale_s + (n % SCALES) * 3 * KB + lt % KB;
-            if (lt < KB) {
-              sc[0] = f;
-            } else {
-              sc[KB] = fmaxf(lg2(f), -60.f);
-              sc[2 * KB] = f;
-            }
+        if (scales) {
+          float* sc = scale_s + (t.n() % SCALES) * 3 * KB + lane;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            sc[32 * i] = f[i];
+            sc[KB + 32 * i] = fmaxf(lg2(f[2 + i]), -60.f);
+            sc[2 * KB + 32 * i] = f[2 + i];
           }
-          mbar_arrive(bar(SC_FULL + n % SCALES));
         }
-      } else if (kind & 2u) {
-        // zero times a NaN or an infinity is not zero: hidden keys must not hold any.  Rows that see them get them at the end.
-        uint8_t* dst = gen + (sV + s * C::TILE - base);
-        bool spoilt = false;
+        fence_proxy_async_smem();                         // of the stores, for the products; of the reads, for the next copy
+        __syncwarp();
+        if (lane == 0) {
+          if (scales) mbar_arrive(bar(SC_FULL + t.n() % SCALES));
+          mbar_arrive(bar((t.key ? K_FULL : V_FULL) + s));
+        }
+        fetch(q + RAWS * LOAD_WARPS, place);
+        if (++place == RAWS) {
+          place = 0;
+          phase ^= 1;
+        }
+      }
+    } else {
+      // What a chunk under way needs when it is handed over: its barrier, and for values of a masked block where they lie.
+      uint32_t full[C::BEHIND] = {}, clean[C::BEHIND] = {};
+      int of[C::BEHIND] = {};
+      bool more = true;
 #pragma unroll 1
-        for (int i = 0; i < VPT; ++i) {
-          const int idx = i * LOADERS + lt, r = idx / NC, c = idx % NC;
-          uint4* p = reinterpret_cast<uint4*>(dst + (c >> 3) * (KB * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
-          const uint4 v = *p;
-          if (not_finite(v.x) || not_finite(v.y) || not_finite(v.z) || not_finite(v.w)) {
-            *p = make_uint4(finite_or_zero(v.x), finite_or_zero(v.y), finite_or_zero(v.z), finite_or_zero(v.w));
-            spoilt = true;
+      for (int q = w0; ok && (more || full[C::BEHIND - 1]); q += LOAD_WARPS) {
+        uint32_t new_full = 0, new_clean = 0;
+        if (more) more = t.find(a, q / C::CPT);
+        if (more) {
+          const int part = q % C::CPT, s = t.n() % STAGES, rows = t.rows();
+          const uint32_t dst = (t.key ? sK : sV) + s * C::TILE;
+          const uint8_t* src = (t.key ? a.k : a.v) + (t.at + t.j * KB) * C::RB;
+          ok = place_free();
+          if (!ok) break;
+#pragma unroll 4
+          for (int i = 0; i < PIECES; ++i) {
+            const int idx = part * (CHUNK / 16) + i * 32 + lane, r = idx / NC, c = idx % NC;
+            copy16(dst + (c >> 3) * (KB * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4), src + (r < rows ? idx * 16 : 0), r < rows);
           }
+          new_full = bar((t.key ? K_FULL : V_FULL) + s);
+          if (!t.key && masked_block(a, t.x, t.slot())) new_clean = dst + part * (CHUNK / C::RB) * 128;
         }
-        if (spoilt) spoilt_s[kind >> 2 & 3] = (int)(kind >> 2) + 1;
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (full[C::BEHIND - 1]) {
+          asm volatile("cp.async.wait_group %0;" ::"n"(C::BEHIND) : "memory");
+          if (clean[C::BEHIND - 1]) {
+            // zero times a NaN or an infinity is not zero: hidden keys must not hold any.  Rows that see them get them at the end.
+            bool spoilt = false;
+#pragma unroll 1
+            for (int i = 0; i < PIECES; ++i) {
+              const int idx = i * 32 + lane, c = idx % NC, r0 = (clean[C::BEHIND - 1] - base) / 128, r = idx / NC;
+              uint4* p = reinterpret_cast<uint4*>(gen + (clean[C::BEHIND - 1] - base) + (c >> 3) * (KB * 128) + r * 128 + (((c & 7) ^ ((r0 + r) & 7)) << 4));
+              const uint4 v = *p;
+              if (not_finite(v.x) || not_finite(v.y) || not_finite(v.z) || not_finite(v.w)) {
+                *p = make_uint4(finite_or_zero(v.x), finite_or_zero(v.y), finite_or_zero(v.z), finite_or_zero(v.w));
+                spoilt = true;
+              }
+            }
+            if (spoilt) spoilt_s[of[C::BEHIND - 1] & 7] = of[C::BEHIND - 1] + 1;
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(full[C::BEHIND - 1]);
+        }
+#pragma unroll
+        for (int i = C::BEHIND - 1; i > 0; --i) {
+          full[i] = full[i - 1];
+          clean[i] = clean[i - 1];
+          of[i] = of[i - 1];
+        }
+        full[0] = new_full;
+        clean[0] = new_clean;
+        of[0] = t.stretch;
       }
-      fence_proxy_async_smem();
-      mbar_arrive(bar((key ? K_FULL : V_FULL) + s));
-    };
-    for (int o = 0; ok; ++o) {
-      issue();
-      if (!ok) break;
-      const int oldest = slot + 1 == C::LAG ? 0 : slot + 1;              // the place of the tile LAG - 1 before
-      if (o >= C::LAG - 1) {
-        if (under_way == 0) break;
-        finish(oldest);
-        --under_way;
-      }
-      slot = oldest;
     }
   } else if (warp == PRODUCT_WARP) {
     // ------------------------------------------------------------------ products (warp-uniform, one elected lane issues)
@@ -273,7 +332,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
     int n = 0, visit = 0;                                 // blocks and stretches done
     auto issue_s = [&](int n) {
       const int s = n % STAGES;
-      ok = mbar_wait_warp(bar(K_FULL + s), (n / STAGES) & 1, abort_smem, a.status, SITE_SMEM_FULL);
+      ok = wait_warp(bar(K_FULL + s), (n / STAGES) & 1, abort_smem, a.status, SITE_SMEM_FULL);
       if (!ok) return;
       tc_fence_after();
       if (leader) {
@@ -287,10 +346,10 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
       }
       __syncwarp();
     };
-    while (ok && next(a, walk, x)) {
-      const int blocks = blocks_of(x);
+    for (Stretch y; ok && next_stretch(a, walk, y);) {
+      const int blocks = blocks_of(y);
       if (blocks == 0) continue;
-      ok = mbar_wait_warp(bar(Q_FULL), visit++ & 1, abort_smem, a.status, SITE_SMEM_FULL);
+      ok = wait_warp(bar(Q_FULL), visit++ & 1, abort_smem, a.status, SITE_SMEM_FULL);
       if (ok) issue_s(n);
       for (int j = 0; ok && j < blocks; ++j, ++n) {
         if (j + 1 < blocks) {
@@ -298,12 +357,12 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
           // not ordered among themselves: that one's end is waited for.  (So by the time a block's scores are there, the
           // product two blocks back is over: a wait for the end of a product, on one of two barriers in turn, cannot be
           // answered by the phase before.)
-          if (j > 0) ok = mbar_wait_warp(bar(O_DONE + ((n - 1) & 1)), ((n - 1) >> 1) & 1, abort_smem, a.status, SITE_TMEM_EMPTY);
+          if (j > 0) ok = wait_warp(bar(O_DONE + ((n - 1) & 1)), ((n - 1) >> 1) & 1, abort_smem, a.status, SITE_TMEM_EMPTY);
           if (ok) issue_s(n + 1);
         }
         const int s = n % STAGES;
-        if (ok) ok = mbar_wait_warp(bar(V_FULL + s), (n / STAGES) & 1, abort_smem, a.status, SITE_SMEM_FULL);
-        if (ok) ok = mbar_wait_warp(bar(P_FULL + (n & 1)), (n >> 1) & 1, abort_smem, a.status, SITE_TMEM_FULL);
+        if (ok) ok = wait_warp(bar(V_FULL + s), (n / STAGES) & 1, abort_smem, a.status, SITE_SMEM_FULL);
+        if (ok) ok = wait_warp(bar(P_FULL + (n & 1)), (n >> 1) & 1, abort_smem, a.status, SITE_TMEM_FULL);
         if (!ok) break;
         tc_fence_after();
         if (leader) {
@@ -317,18 +376,22 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
       }
     }
   } else if (warp < LOAD_WARP) {
-    // ------------------------------------------------------------------ softmax: thread = query row = TMEM lane
+    // ------------------------------------------------------------------ softmax: two threads per query row = TMEM lane
     constexpr float LIFT = Q8 ? 6.f : 0.f;                // with the 2^8 that a reference may lag behind, w stays below 2^14
-    const int row = threadIdx.x;
-    const uint32_t lane_addr = tmem + ((uint32_t)(warp * 32) << 16);
+    constexpr int HALF = KB / 2;                          // keys of a thread
+    const int row = threadIdx.x & 127, half = threadIdx.x >> 7;
+    const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    auto both = [] { asm volatile("bar.sync 1, %0;" ::"n"(SOFT) : "memory"); };
     int n = 0, stretch = -1;
-    while (ok && next(a, walk, x)) {
+    // Every warp of these passes the same barriers whatever happens: a wait that ran out makes the others run out, it ends no loop.
+    for (Stretch y; next_stretch(a, walk, y);) {
+      x = y;
       ++stretch;
       const int blocks = blocks_of(x), r = x.tile * TT + row, t = min(r / G, a.T - 1), h = x.hk * G + r % G;
       const bool real = row < x.n_rows;
       float unit = 1.f;
-      if (blocks > 0) {                                   // the row of Q into its place
-        const __nv_bfloat16* src = a.q + x.b * a.q_sb + t * a.q_st + (long long)h * HD;
+      if (blocks > 0) {                                   // half a row of Q into its place
+        const __nv_bfloat16* src = a.q + x.b * a.q_sb + t * a.q_st + (long long)h * HD + half * (HD / 2);
         const bool vec = (reinterpret_cast<uintptr_t>(src) & 15) == 0;
         auto piece = [&](int c) {
           uint4 v = make_uint4(0, 0, 0, 0);
@@ -344,17 +407,20 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
         };
         if (Q8) {
           float top = 0.f;
-#pragma unroll 8
-          for (int c = 0; c < HD / 8; ++c) {
+#pragma unroll 4
+          for (int c = 0; c < HD / 16; ++c) {
             const uint4 v = piece(c);
             const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u))));
           }
+          sum_s[half][row] = top;
+          both();
+          top = fmaxf(top, sum_s[half ^ 1][row]);
           unit = ldexpf(1.f, top > 0.f ? min(max(8 - ilogbf(top), -110), 110) : 0);
         }
 #pragma unroll 1
-        for (int c = 0; c < HD / 32; ++c) {
+        for (int c = 0; c < HD / 64; ++c) {
           uint32_t w[16];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -366,7 +432,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
             for (int i = 0; i < 16; ++i) w[i] = pack16(true, __uint_as_float(w[i] << 16) * unit, __uint_as_float(w[i] & 0xffff0000u) * unit);
           }
           __syncwarp();
-          tmem_st_32x16(lane_addr + C::Q_COL + c * 16, w);
+          tmem_st_32x16(lane_addr + C::Q_COL + half * (HD / 4) + c * 16, w);
         }
         tmem_st_wait();
         tc_fence_before();                                // and O of the stretch before has been read
@@ -375,64 +441,59 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
       const float q_unit = a.scale_log2 / unit;
       const unsigned long long vis = a.visible ? (unsigned long long)__ldcg(a.visible + (long long)x.b * a.T + t) : t >= 63 ? ~0ull : (2ull << t) - 1;
       const int row_lo = a.window > 0 ? max(0, x.s.pos + max(__popcll(vis), 1) - a.window) : 0;
-      const bool works = warp * 32 < x.n_rows;            // some row of this warp is real
+      const bool works = (warp & 3) * 32 < x.n_rows;            // some row of this warp is real
       const F2 unit2 = f2(q_unit, q_unit);
       float m = -CUDART_INF_F, l = 0.f;
-      for (int j = 0; ok && j < blocks; ++j, ++n) {
-        ok = mbar_wait_warp(bar(S_FULL + (n & 1)), (n >> 1) & 1, abort_smem, a.status, SITE_TMEM_FULL);
-        if (ok && Q8) ok = mbar_wait_warp(bar(SC_FULL + n % SCALES), (n / SCALES) & 1, abort_smem, a.status, SITE_SMEM_FULL);
-        if (!ok) break;
+      for (int j = 0; j < blocks; ++j, ++n) {
+        ok = ok && wait_warp(bar(S_FULL + (n & 1)), (n >> 1) & 1, abort_smem, a.status, SITE_TMEM_FULL);
+        if (Q8) ok = ok && wait_warp(bar(SC_FULL + n % SCALES), (n / SCALES) & 1, abort_smem, a.status, SITE_SMEM_FULL);
         tc_fence_after();
         const uint32_t s_addr = lane_addr + C::S_COL + (n & 1) * KB;
+        const int slot0 = x.k_lo + j * KB;
+        const bool masked = masked_block(a, x, slot0);
+        const float4* ks = reinterpret_cast<const float4*>(scale_s + (n % SCALES) * 3 * KB + half * HALF);
+        uint32_t v[32], see = ~0u;                        // scores times the keys' scales; the keys that the row sees
         if (works) {
-          const int slot0 = x.k_lo + j * KB;
-          const bool masked = masked_block(a, x, slot0);
-          const float4* ks = reinterpret_cast<const float4*>(scale_s + (n % SCALES) * 3 * KB);
-          uint32_t v[2][32];                              // scores times the keys' scales
-          tmem_ld_32x32(s_addr, v[0]);
-          tmem_ld_32x32(s_addr + 32, v[1]);
+          tmem_ld_32x32(s_addr + half * HALF, v);
           tmem_ld_wait();
           if (Q8) {
 #pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-              for (int i = 0; i < 32; i += 4) {
-                const float4 k4 = ks[(c * 32 + i) / 4];
-                float f0, f1;
-                unpack(mul2(f2(__uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1])), f2(k4.x, k4.y)), f0, f1);
-                v[c][i] = __float_as_uint(f0);
-                v[c][i + 1] = __float_as_uint(f1);
-                unpack(mul2(f2(__uint_as_float(v[c][i + 2]), __uint_as_float(v[c][i + 3])), f2(k4.z, k4.w)), f0, f1);
-                v[c][i + 2] = __float_as_uint(f0);
-                v[c][i + 3] = __float_as_uint(f1);
-              }
-          }
-          uint32_t see[2] = {~0u, ~0u};
-          if (masked) {
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              see[c] = seen(x, row_lo, vis, slot0 + c * 32);
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (!(see[c] >> i & 1u)) v[c][i] = 0xff800000u;          // -inf: exp2 gives an exact zero
+            for (int i = 0; i < 32; i += 4) {
+              const float4 k4 = ks[i / 4];
+              float f0, f1;
+              unpack(mul2(f2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), f2(k4.x, k4.y)), f0, f1);
+              v[i] = __float_as_uint(f0);
+              v[i + 1] = __float_as_uint(f1);
+              unpack(mul2(f2(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])), f2(k4.z, k4.w)), f0, f1);
+              v[i + 2] = __float_as_uint(f0);
+              v[i + 3] = __float_as_uint(f1);
             }
+          }
+          if (masked) {
+            see = seen(x, row_lo, vis, slot0 + half * HALF);
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (!(see >> i & 1u)) v[i] = 0xff800000u;   // -inf: exp2 gives an exact zero
           }
           float part[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              float f[4] = {__uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1]), __uint_as_float(v[c][i + 2]), __uint_as_float(v[c][i + 3])};
-              if (Q8) {
-                const float4 u4 = ks[KB / 4 + (c * 32 + i) / 4];
-                unpack(fma2(f2(f[0], f[1]), unit2, f2(u4.x, u4.y)), f[0], f[1]);
-                unpack(fma2(f2(f[2], f[3]), unit2, f2(u4.z, u4.w)), f[2], f[3]);
-              }
-#pragma unroll
-              for (int e = 0; e < 4; ++e) part[e] = fmaxf(part[e], f[e]);
+          for (int i = 0; i < 32; i += 4) {
+            float f[4] = {__uint_as_float(v[i]), __uint_as_float(v[i + 1]), __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])};
+            if (Q8) {
+              const float4 u4 = ks[KB / 4 + i / 4];
+              unpack(fma2(f2(f[0], f[1]), unit2, f2(u4.x, u4.y)), f[0], f[1]);
+              unpack(fma2(f2(f[2], f[3]), unit2, f2(u4.z, u4.w)), f[2], f[3]);
             }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) part[e] = fmaxf(part[e], f[e]);
+          }
           float top = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
           if (!Q8) top *= q_unit;
+          top_s[n & 1][half][row] = top;
+        }
+        both();                                           // and every score is in registers: P may overwrite them
+        if (works) {
+          const float top = fmaxf(top_s[n & 1][0][row], top_s[n & 1][1][row]);
           float alpha = 1.f;
           if (top - LIFT > m + 8.f) {                     // also the first block with a visible key (m = -inf)
             alpha = ex2(m - (top - LIFT));
@@ -441,44 +502,41 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
           // tcgen05.ld / .st are warp-collective: the decision must be the same for all rows of a warp.  Never for the first
           // block: its product overwrites O.
           if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-            ok = mbar_wait_warp(bar(O_DONE + ((n - 1) & 1)), ((n - 1) >> 1) & 1, abort_smem, a.status, SITE_TMEM_EMPTY);
-            if (!ok) break;
+            ok = ok && wait_warp(bar(O_DONE + ((n - 1) & 1)), ((n - 1) >> 1) & 1, abort_smem, a.status, SITE_TMEM_EMPTY);
             tc_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < HD / 16; ++c) {
+            for (int c = 0; c < HD / 32; ++c) {           // half of the columns each
               uint32_t o[16];
-              tmem_ld_32x16(lane_addr + C::O_COL + c * 16, o);
+              const uint32_t at = lane_addr + C::O_COL + half * (HD / 2) + c * 16;
+              tmem_ld_32x16(at, o);
               tmem_ld_wait();
 #pragma unroll
               for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-              tmem_st_32x16(lane_addr + C::O_COL + c * 16, o);
+              tmem_st_32x16(at, o);
             }
           }
           const float off = m == -CUDART_INF_F ? 0.f : -m;
           const F2 off2 = f2(off, off);
           F2 sum2[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
+          uint32_t w[16];
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            uint32_t w[16];
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              float p0, p1;
-              unpack(fma2(f2(__uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1])), unit2, off2), p0, p1);
-              F2 p = f2(ex2(p0), ex2(p1));
-              sum2[(i / 2) & 1] = add2(sum2[(i / 2) & 1], p);
-              if (Q8) {
-                const float4 v4 = ks[2 * KB / 4 + (c * 32 + i) / 4];
-                p = mul2(p, i & 2 ? f2(v4.z, v4.w) : f2(v4.x, v4.y));
-              }
-              unpack(p, p0, p1);
-              w[i / 2] = pack16(Q8, p0, p1);
+          for (int i = 0; i < 32; i += 2) {
+            float p0, p1;
+            unpack(fma2(f2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), unit2, off2), p0, p1);
+            F2 p = f2(ex2(p0), ex2(p1));
+            sum2[(i / 2) & 1] = add2(sum2[(i / 2) & 1], p);
+            if (Q8) {
+              const float4 v4 = ks[2 * KB / 4 + i / 4];
+              p = mul2(p, i & 2 ? f2(v4.z, v4.w) : f2(v4.x, v4.y));
             }
-            if (Q8 && masked) {                           // a hidden key's scale may be anything
-#pragma unroll
-              for (int i = 0; i < 16; ++i) w[i] &= (see[c] >> (2 * i) & 1u ? 0xffffu : 0u) | (see[c] >> (2 * i + 1) & 1u ? 0xffff0000u : 0u);
-            }
-            tmem_st_32x16(s_addr + c * 16, w);            // every score is in registers by now
+            unpack(p, p0, p1);
+            w[i / 2] = pack16(Q8, p0, p1);
           }
+          if (Q8 && masked) {                             // a hidden key's scale may be anything
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w[i] &= (see >> (2 * i) & 1u ? 0xffffu : 0u) | (see >> (2 * i + 1) & 1u ? 0xffff0000u : 0u);
+          }
+          tmem_st_32x16(s_addr + half * (HALF / 2), w);
           float s0, s1;
           unpack(add2(sum2[0], sum2[1]), s0, s1);
           l = l * alpha + s0 + s1;
@@ -487,20 +545,22 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
         tc_fence_before();
         mbar_arrive(bar(P_FULL + (n & 1)));
       }
-      if (!ok) break;
-      // ---- the stretch's result: final, or a share of it
+      // ---- the stretch's result: final, or a share of it; half of the columns each
       if (blocks > 0) {
-        ok = mbar_wait_warp(bar(O_DONE + ((n - 1) & 1)), ((n - 1) >> 1) & 1, abort_smem, a.status, SITE_TMEM_FULL);
-        if (!ok) break;
+        ok = ok && wait_warp(bar(O_DONE + ((n - 1) & 1)), ((n - 1) >> 1) & 1, abort_smem, a.status, SITE_TMEM_FULL);
         tc_fence_after();
       }
-      if (!works) continue;
-      const bool spoilt = !Q8 && spoilt_s[stretch & 3] == (stretch & 63) + 1;
+      sum_s[half][row] = l;
+      both();
+      l += sum_s[half ^ 1][row];
+      both();                                             // the sums have been read
+      if (!ok || !works) continue;
+      const bool spoilt = !Q8 && spoilt_s[stretch & 7] == stretch + 1;
       const float inv = !x.whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
       __nv_bfloat16* dst = a.out + x.b * a.o_sb + t * a.o_st + (long long)h * HD;
       const bool vec = (reinterpret_cast<uintptr_t>(dst) & 15) == 0;
 #pragma unroll 1
-      for (int c = 0; c < HD / 32; ++c) {
+      for (int c = half * (HD / 64); c < (half + 1) * (HD / 64); ++c) {
         uint32_t o[32];
         if (blocks > 0) {
           tmem_ld_32x32(lane_addr + C::O_COL + c * 32, o);
@@ -517,7 +577,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
               const float f = __bfloat162float(v0[(long long)slot * HD + i]);
-              if (!(fabsf(f) < CUDART_INF_F)) o[i] = __float_as_uint(__uint_as_float(o[i]) + f);
+              o[i] = __float_as_uint(__uint_as_float(o[i]) + (fabsf(f) < CUDART_INF_F ? 0.f : f));
             }
           }
           __syncwarp();
@@ -543,7 +603,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
         }
         __syncwarp();
       }
-      if (!x.whole && real) a.part_ml[x.slot * TT + row] = make_float2(m, l);
+      if (!x.whole && real && half == 0) a.part_ml[x.slot * TT + row] = make_float2(m, l);
       __syncwarp();
     }
   }
@@ -617,7 +677,7 @@ __global__ void __launch_bounds__(GROUPS * TT) wide_join_kernel(const __grid_con
 template <int HD, bool Q8>
 int run(const Args& p, void* stream) {
   using C = Wide<HD, Q8>;
-  static_assert(C::SMEM <= 226 * 1024 && KB * C::NC % LOADERS == 0 && C::Q_COL + HD / 2 <= 512 && SCALES >= C::STAGES + 2 && C::LAG <= 8, "shared memory of a CTA");
+  static_assert(C::SMEM <= 222 * 1024 && C::CPT * CHUNK == KB * C::RB && C::Q_COL + HD / 2 <= 512 && SCALES >= C::STAGES + 2, "shared memory of a CTA");
   static std::atomic<unsigned long long> configured{0};   // a bit per device
   int dev = 0;
   MESH_CUDA_OK(cudaGetDevice(&dev));
