@@ -1,20 +1,21 @@
 // Attention of drafts with many query rows (more than 16 drafts times heads of a group) on the 5th-generation tensor cores.
 //
 // A tile is 128 query rows of one (sequence, KV head); a CTA goes through its stretches of 64-key blocks (how the work is cut and
-// the formulas: draft_attention.cuh, draft_attention.cu).  Warps 0-7: softmax, two threads per query row with half of the block's keys
-// each.  Warps 8-14: keys and values, a warp per 4 KB of a tile, into the 128-byte swizzle of the operands: bf16 rows by
-// cp.async; 8-bit codes copied in bulk to places of the warp's own and widened to fp16 from there.  Warp 15: the products
-// S = Q K^T and O += P V by one elected lane, S of the next block before P V of this one.  Tensor memory holds the queries
-// (operand A of the first product, 16 bits), S twice, of which P (16 bits, operand A of the second) overwrites the first
-// half, and O, which is rescaled only when a row's maximum has grown by more than 2^8.
+// the formulas: draft_attention.cuh, draft_attention.cu).  Warps 0-15: softmax, in two groups that take the blocks in turn, in each
+// two threads per query row with half of the block's keys.  Warps 16-22: keys and values, a warp per 4 KB of a tile, into the 128-byte
+// swizzle of the operands: bf16 rows by cp.async; 8-bit codes copied in bulk to places of the warp's own and widened to
+// fp16 from there.  Warp 23: the products S = Q K^T and O += P V by one elected lane, S up to three blocks ahead of P V.
+// Tensor memory holds the queries (operand A of the first product, 16 bits), S of four blocks (heads of 256: two), of each of
+// which P (16 bits, operand A of the second) overwrites the first half, and O, which is rescaled only when a row's maximum
+// has grown by more than 2^8: the reference point of a row goes from group to group through shared memory.
 //
 // Codes are widened once per 128 rows: as operands of a product in 8 bits the queries and probabilities would have to be rounded to 8
 // bits too.  Queries in tensor memory leave shared memory to the rings and its bandwidth to their stores and reads.  The
-// roles run different code on the same SM, so it is kept short: with the waits' error paths and the cutting of the work
-// inlined everywhere (112 KB) and tiles held in registers (unrolled twice), one instruction fetch in six missed the cache.
-// What was slower, at 64 drafts x 4 heads over four contexts of 20000-32704 keys of 256 in 8 bits: that, 125 us; all loader
-// threads at every tile through cp.async, with one softmax thread per row, 117; blocks of 128 keys with the queries in
-// shared memory, 126; scores read twice from tensor memory, 165.
+// roles are chains of short steps, each a few instructions behind the one before, so there are many warps of few registers; and
+// they run different code on the same SM, so it is kept short.  What was slower, at 64 drafts x 4 heads over four
+// contexts of 20000-32704 keys of 256 in 8 bits: one group of softmax threads, 130 us; tiles held in registers ahead of
+// their turn and everything inlined (112 KB of code, one fetch in six missed the cache), 125; all loader threads at every
+// tile, 117; blocks of 128 keys with the queries in shared memory, 126; scores read twice from tensor memory, 165.
 #include "draft_attention.cuh"
 
 namespace mesh {
@@ -22,26 +23,27 @@ namespace draft {
 namespace {
 
 constexpr int TT = WIDE_ROWS, KB = WIDE_UNIT;               // rows of a tile, keys of a block
-constexpr int SOFT = 256, LOAD_WARPS = 7, THREADS = SOFT + 32 * LOAD_WARPS + 32;
+constexpr int GROUP = 256, SOFT = 2 * GROUP, LOAD_WARPS = 7, THREADS = SOFT + 32 * LOAD_WARPS + 32;
 constexpr int LOAD_WARP = SOFT / 32, PRODUCT_WARP = LOAD_WARP + LOAD_WARPS;
-constexpr int SCALES = 8;                                   // blocks whose scales are kept: two more than there are stages, at least
+constexpr int SCALES = 8;                                   // blocks whose scales are kept: stages and buffers of S together
 constexpr int CHUNK = 4096, PIECES = CHUNK / (32 * 16);     // bytes of stored rows a warp takes at a time; 16-byte pieces of a lane
 
 template <int HD, bool Q8>
 struct Wide {
   static constexpr int TILE = KB * HD * 2;
   static constexpr int STAGES = HD < 256 ? 4 : Q8 ? 2 : 3;
+  static constexpr int NB = HD < 256 ? 4 : 2;               // blocks whose S is in tensor memory
   static constexpr int RB = Q8 ? HD : 2 * HD, NC = RB / 16;           // bytes and 16-byte pieces of a stored row
   static constexpr int CPT = KB * RB / CHUNK;               // chunks of a tile
-  // Chunks of bf16 rows that a warp has under way beside the newest, which may wait for a product that needs any tile up to
-  // 2 STAGES - 1 before its own: the oldest must lie further back no more than that.
+  // Chunks of bf16 rows that a warp has under way.  While it waits for the place of a tile of values the product that frees it waits for
+  // tiles of keys up to 2 STAGES - 2 NB + 4 before that one: what the warp has not handed over must be younger.
   static constexpr int BEHIND = CPT >= 4 ? 2 : 1;
-  static_assert(Q8 || BEHIND * LOAD_WARPS < (2 * STAGES - 1) * CPT, "a loader would wait for what it has not handed over");
+  static_assert(Q8 || (BEHIND - 1) * LOAD_WARPS <= (2 * STAGES - 2 * NB + 3) * CPT, "a loader would wait for what it has not handed over");
   static constexpr int RAWS = Q8 ? 3 : 0;                   // chunks of codes that a warp has under way
-  static constexpr int N_BARS = 1 + 4 * STAGES + 2 + 2 + 2 + SCALES + RAWS * LOAD_WARPS;
+  static constexpr int N_BARS = 1 + 4 * STAGES + 3 * NB + 2 + SCALES + RAWS * LOAD_WARPS;
   static constexpr int SCALE_BYTES = Q8 ? SCALES * 3 * KB * 4 : 0;
   static constexpr int SMEM = 2 * STAGES * TILE + RAWS * LOAD_WARPS * CHUNK + SCALE_BYTES + 8 * N_BARS + 64 + 1024;
-  static constexpr int S_COL = 0, O_COL = 2 * KB, Q_COL = O_COL + HD;  // columns of tensor memory
+  static constexpr int S_COL = 0, O_COL = NB * KB, Q_COL = O_COL + HD;  // columns of tensor memory
 };
 
 // Once, not in every role: its divisions are long.
@@ -104,15 +106,14 @@ __device__ __forceinline__ uint32_t finite_or_zero(uint32_t w) {
 }
 
 // Where the tiles of keys and values lie.  Per stretch they come in the order the products take them: K0 K1 V0 K2 V1 ... V(last).
-struct Tiles {
-  Walk walk;
+struct Tiles {                                             // (the walk apart: what a call takes the address of stays in memory)
   Stretch x;
   int first = 0, blocks = 0, n0 = 0, stretch = -1;        // tiles before this stretch, its blocks, blocks before it
   long long at = 0;                                       // row of its first slot
   bool key = false;
   int j = 0;                                              // block within the stretch
   // Tile o of all, not before the last one asked for; false behind the last.
-  __device__ __forceinline__ bool find(const Args& a, int o) {
+  __device__ __forceinline__ bool find(const Args& a, Walk& walk, int o) {
     while (o - first >= 2 * blocks) {
       first += 2 * blocks;
       n0 += blocks;
@@ -137,7 +138,7 @@ struct Tiles {
 template <int HD, bool Q8>
 __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant__ Args a) {
   using C = Wide<HD, Q8>;
-  constexpr int STAGES = C::STAGES, NC = C::NC;
+  constexpr int STAGES = C::STAGES, NC = C::NC, NB = C::NB;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
@@ -145,12 +146,14 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
   float* scale_s = reinterpret_cast<float*>(gen + (sScale - base));        // [buffer]{key scale, lg2 of the value scale, value scale}[key]
   auto bar = [&](int i) { return bars + 8u * i; };
   constexpr int Q_FULL = 0, K_FULL = 1, K_EMPTY = K_FULL + STAGES, V_FULL = K_EMPTY + STAGES, V_EMPTY = V_FULL + STAGES,
-                S_FULL = V_EMPTY + STAGES, P_FULL = S_FULL + 2, O_DONE = P_FULL + 2, SC_FULL = O_DONE + 2, RAW_FULL = SC_FULL + SCALES;
+                S_FULL = V_EMPTY + STAGES, P_FULL = S_FULL + NB, O_DONE = P_FULL + NB, M_READY = O_DONE + NB, SC_FULL = M_READY + 2, RAW_FULL = SC_FULL + SCALES;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen + (bars - base) + 8 * C::N_BARS);
   volatile int* abort_smem = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* spoilt_s = reinterpret_cast<volatile int*>(tmem_slot + 2);     // [8]: stretch + 1 whose values had to be cleaned; loaders are at most 5 stretches ahead
   __shared__ Walk walk_s;
-  __shared__ float top_s[2][2][TT], sum_s[2][TT];           // [block & 1][half][row], [half][row]
+  __shared__ float top_s[2][2][2][TT];                      // [group][its block & 1][half][row]
+  __shared__ float m_s[2][TT], sum_s[4][TT];                // [group][row]: reference points; [group, half][row]
+  __shared__ volatile int over_s;                           // blocks whose second product is over
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = a.q_heads / a.kv_heads;
 
   if (threadIdx.x == 0) {
@@ -161,11 +164,13 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
       mbar_init(bar(K_EMPTY + s), 1);
       mbar_init(bar(V_EMPTY + s), 1);
     }
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < NB; ++s) {
       mbar_init(bar(S_FULL + s), 1);
-      mbar_init(bar(P_FULL + s), SOFT);
+      mbar_init(bar(P_FULL + s), GROUP);
       mbar_init(bar(O_DONE + s), 1);
     }
+    for (int s = 0; s < 2; ++s) mbar_init(bar(M_READY + s), TT);
+    over_s = 0;
     for (int s = 0; s < SCALES; ++s) mbar_init(bar(SC_FULL + s), 1);
     for (int s = 0; s < C::RAWS * LOAD_WARPS; ++s) mbar_init(bar(RAW_FULL + s), 1);
     *abort_smem = 0;
@@ -191,20 +196,32 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
     // ------------------------------------------------------------------ keys and values
     // Chunk q of all is warp q mod LOAD_WARPS's.
     Tiles t;
-    t.walk = walk;
     const int w0 = warp - LOAD_WARP;
-    // A warp may pass a place's phases unseen; but its chunk before, LOAD_WARPS chunks back, waited for a product that comes
-    // after the one two phases back, so the phase before cannot answer.
+    // A warp may pass a place's phases unseen, and a wait could be answered by the phase before the one it means: so the one two phases
+    // back must be known to be over, which it nearly always is.
     auto place_free = [&]() {
-      return t.n() < STAGES ||
-             wait_warp(bar((t.key ? K_EMPTY : V_EMPTY) + t.n() % STAGES), (t.n() / STAGES - 1) & 1, abort_smem, a.status, SITE_SMEM_EMPTY);
+      const int n = t.n();
+      if (n < STAGES) return true;
+      if (n >= 2 * STAGES && over_s <= n - 2 * STAGES) {
+        const unsigned long long t0 = globaltimer_ns();
+        while (over_s <= n - 2 * STAGES) {
+          if (*abort_smem) return false;
+          if (globaltimer_ns() - t0 > MESH_WAIT_LIMIT_NS || status_aborted(a.status)) {
+            *abort_smem = 1;
+            status_record(a.status, MESH_TIMEOUT, SITE_SMEM_EMPTY, n, over_s, 0);
+            return false;
+          }
+        }
+      }
+      return wait_warp(bar((t.key ? K_EMPTY : V_EMPTY) + n % STAGES), (n / STAGES - 1) & 1, abort_smem, a.status, SITE_SMEM_EMPTY);
     };
     if (Q8) {
       constexpr int RAWS = C::RAWS ? C::RAWS : 1;
-      Tiles ahead = t;
+      Tiles ahead;
+      Walk ahead_walk = walk;
       const uint32_t own = sRaw + w0 * (RAWS * CHUNK), own_full = bar(RAW_FULL) + 8 * w0 * RAWS;
       auto fetch = [&](int q, int place) {                // starts the copy of a chunk; what lies behind the last slot is not read
-        if (!ahead.find(a, q / C::CPT)) return;
+        if (!ahead.find(a, ahead_walk, q / C::CPT)) return;
         const int part = q % C::CPT, bytes = min(max(ahead.rows() * C::RB - part * CHUNK, 0), CHUNK);
         if (lane == 0) {
           mbar_expect_tx(own_full + 8 * place, bytes);
@@ -216,7 +233,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
       for (int i = 0; i < RAWS; ++i) fetch(w0 + i * LOAD_WARPS, i);
       int place = 0, phase = 0;
 #pragma unroll 1
-      for (int q = w0; ok && t.find(a, q / C::CPT); q += LOAD_WARPS) {
+      for (int q = w0; ok && t.find(a, walk, q / C::CPT); q += LOAD_WARPS) {
         const int part = q % C::CPT, s = t.n() % STAGES, rows = t.rows();
         const bool scales = t.key && part == 0;
         float f[4];                                       // scales of keys lane, lane + 32 and their values
@@ -229,6 +246,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
           }
         }
         ok = wait_warp(own_full + 8 * place, phase, abort_smem, a.status, SITE_SMEM_FULL) && place_free();
+        ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         const uint8_t* src = gen + (own - base) + place * CHUNK;
         uint8_t* dst = gen + ((t.key ? sK : sV) + s * C::TILE - base);
@@ -274,25 +292,8 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
       bool more = true;
 #pragma unroll 1
       for (int q = w0; ok && (more || full[C::BEHIND - 1]); q += LOAD_WARPS) {
-        uint32_t new_full = 0, new_clean = 0;
-        if (more) more = t.find(a, q / C::CPT);
-        if (more) {
-          const int part = q % C::CPT, s = t.n() % STAGES, rows = t.rows();
-          const uint32_t dst = (t.key ? sK : sV) + s * C::TILE;
-          const uint8_t* src = (t.key ? a.k : a.v) + (t.at + t.j * KB) * C::RB;
-          ok = place_free();
-          if (!ok) break;
-#pragma unroll 4
-          for (int i = 0; i < PIECES; ++i) {
-            const int idx = part * (CHUNK / 16) + i * 32 + lane, r = idx / NC, c = idx % NC;
-            copy16(dst + (c >> 3) * (KB * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4), src + (r < rows ? idx * 16 : 0), r < rows);
-          }
-          new_full = bar((t.key ? K_FULL : V_FULL) + s);
-          if (!t.key && masked_block(a, t.x, t.slot())) new_clean = dst + part * (CHUNK / C::RB) * 128;
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
         if (full[C::BEHIND - 1]) {
-          asm volatile("cp.async.wait_group %0;" ::"n"(C::BEHIND) : "memory");
+          asm volatile("cp.async.wait_group %0;" ::"n"(C::BEHIND - 1) : "memory");
           if (clean[C::BEHIND - 1]) {
             // zero times a NaN or an infinity is not zero: hidden keys must not hold any.  Rows that see them get them at the end.
             bool spoilt = false;
@@ -312,6 +313,23 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
           __syncwarp();
           if (lane == 0) mbar_arrive(full[C::BEHIND - 1]);
         }
+        uint32_t new_full = 0, new_clean = 0;
+        if (more) more = t.find(a, walk, q / C::CPT);
+        if (more) {
+          const int part = q % C::CPT, s = t.n() % STAGES, rows = t.rows();
+          const uint32_t dst = (t.key ? sK : sV) + s * C::TILE;
+          const uint8_t* src = (t.key ? a.k : a.v) + (t.at + t.j * KB) * C::RB;
+          ok = __all_sync(0xffffffffu, place_free());
+          if (!ok) break;
+#pragma unroll 4
+          for (int i = 0; i < PIECES; ++i) {
+            const int idx = part * (CHUNK / 16) + i * 32 + lane, r = idx / NC, c = idx % NC;
+            copy16(dst + (c >> 3) * (KB * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4), src + (r < rows ? idx * 16 : 0), r < rows);
+          }
+          new_full = bar((t.key ? K_FULL : V_FULL) + s);
+          if (!t.key && masked_block(a, t.x, t.slot())) new_clean = dst + part * (CHUNK / C::RB) * 128;
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
 #pragma unroll
         for (int i = C::BEHIND - 1; i > 0; --i) {
           full[i] = full[i - 1];
@@ -339,10 +357,10 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k) {
           const int off = ((k / 4) * (KB * 128) + (k % 4) * 32) / 16;
-          umma_f16_ts(tmem + C::S_COL + (n & 1) * KB, tmem + C::Q_COL + k * 8, dk0 + (uint32_t)(s * (C::TILE >> 4)) + off, idesc_s, k ? 1u : 0u);
+          umma_f16_ts(tmem + C::S_COL + n % NB * KB, tmem + C::Q_COL + k * 8, dk0 + (uint32_t)(s * (C::TILE >> 4)) + off, idesc_s, k ? 1u : 0u);
         }
         umma_commit(bar(K_EMPTY + s));
-        umma_commit(bar(S_FULL + (n & 1)));
+        umma_commit(bar(S_FULL + n % NB));
       }
       __syncwarp();
     };
@@ -350,27 +368,28 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
       const int blocks = blocks_of(y);
       if (blocks == 0) continue;
       ok = wait_warp(bar(Q_FULL), visit++ & 1, abort_smem, a.status, SITE_SMEM_FULL);
-      if (ok) issue_s(n);
+      if (lane == 0) over_s = n;
+      for (int i = 0; ok && i < NB - 1 && i < blocks; ++i) issue_s(n + i);
       for (int j = 0; ok && j < blocks; ++j, ++n) {
-        if (j + 1 < blocks) {
-          // S of the next block overwrites the P that the product before the last one reads, and products of different shapes are
-          // not ordered among themselves: that one's end is waited for.  (So by the time a block's scores are there, the
-          // product two blocks back is over: a wait for the end of a product, on one of two barriers in turn, cannot be
-          // answered by the phase before.)
-          if (j > 0) ok = wait_warp(bar(O_DONE + ((n - 1) & 1)), ((n - 1) >> 1) & 1, abort_smem, a.status, SITE_TMEM_EMPTY);
-          if (ok) issue_s(n + 1);
+        // The S issued next overwrites the P that the product before reads, and products of different shapes are not ordered among
+        // themselves: that one's end is waited for.  (So by the time a block's scores are there, the product NB blocks back
+        // is over: a wait for the end of a product, on one of NB barriers in turn, cannot be answered by the phase before.)
+        if (j > 0) {
+          ok = wait_warp(bar(O_DONE + (n - 1) % NB), (n - 1) / NB & 1, abort_smem, a.status, SITE_TMEM_EMPTY);
+          if (lane == 0) over_s = n;
         }
+        if (ok && j + NB - 1 < blocks) issue_s(n + NB - 1);
         const int s = n % STAGES;
         if (ok) ok = wait_warp(bar(V_FULL + s), (n / STAGES) & 1, abort_smem, a.status, SITE_SMEM_FULL);
-        if (ok) ok = wait_warp(bar(P_FULL + (n & 1)), (n >> 1) & 1, abort_smem, a.status, SITE_TMEM_FULL);
+        if (ok) ok = wait_warp(bar(P_FULL + n % NB), n / NB & 1, abort_smem, a.status, SITE_TMEM_FULL);
         if (!ok) break;
         tc_fence_after();
         if (leader) {
 #pragma unroll
           for (int k = 0; k < KB / 16; ++k)
-            umma_f16_ts(tmem + C::O_COL, tmem + C::S_COL + (n & 1) * KB + k * 8, dv0 + (uint32_t)(s * (C::TILE >> 4)) + k * 128, idesc_o, (j | k) ? 1u : 0u);
+            umma_f16_ts(tmem + C::O_COL, tmem + C::S_COL + n % NB * KB + k * 8, dv0 + (uint32_t)(s * (C::TILE >> 4)) + k * 128, idesc_o, (j | k) ? 1u : 0u);
           umma_commit(bar(V_EMPTY + s));
-          umma_commit(bar(O_DONE + (n & 1)));
+          umma_commit(bar(O_DONE + n % NB));
         }
         __syncwarp();
       }
@@ -379,10 +398,11 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
     // ------------------------------------------------------------------ softmax: two threads per query row = TMEM lane
     constexpr float LIFT = Q8 ? 6.f : 0.f;                // with the 2^8 that a reference may lag behind, w stays below 2^14
     constexpr int HALF = KB / 2;                          // keys of a thread
-    const int row = threadIdx.x & 127, half = threadIdx.x >> 7;
+    const int row = threadIdx.x & 127, half = threadIdx.x >> 7 & 1, group = threadIdx.x / GROUP, quarter = threadIdx.x >> 7;
     const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    auto both = [] { asm volatile("bar.sync 1, %0;" ::"n"(SOFT) : "memory"); };
-    int n = 0, stretch = -1;
+    auto both = [&] { asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(GROUP) : "memory"); };      // halves of a group
+    auto all = [] { asm volatile("bar.sync 3, %0;" ::"n"(SOFT) : "memory"); };
+    int n = 0, stretch = -1;                              // blocks of the stretches before
     // Every warp of these passes the same barriers whatever happens: a wait that ran out makes the others run out, it ends no loop.
     for (Stretch y; next_stretch(a, walk, y);) {
       x = y;
@@ -390,8 +410,8 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
       const int blocks = blocks_of(x), r = x.tile * TT + row, t = min(r / G, a.T - 1), h = x.hk * G + r % G;
       const bool real = row < x.n_rows;
       float unit = 1.f;
-      if (blocks > 0) {                                   // half a row of Q into its place
-        const __nv_bfloat16* src = a.q + x.b * a.q_sb + t * a.q_st + (long long)h * HD + half * (HD / 2);
+      if (blocks > 0) {                                   // a quarter of a row of Q into its place
+        const __nv_bfloat16* src = a.q + x.b * a.q_sb + t * a.q_st + (long long)h * HD + quarter * (HD / 4);
         const bool vec = (reinterpret_cast<uintptr_t>(src) & 15) == 0;
         auto piece = [&](int c) {
           uint4 v = make_uint4(0, 0, 0, 0);
@@ -407,32 +427,29 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
         };
         if (Q8) {
           float top = 0.f;
-#pragma unroll 4
-          for (int c = 0; c < HD / 16; ++c) {
+#pragma unroll 2
+          for (int c = 0; c < HD / 32; ++c) {
             const uint4 v = piece(c);
             const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u))));
           }
-          sum_s[half][row] = top;
-          both();
-          top = fmaxf(top, sum_s[half ^ 1][row]);
+          sum_s[quarter][row] = top;
+          all();
+          top = fmaxf(fmaxf(sum_s[0][row], sum_s[1][row]), fmaxf(sum_s[2][row], sum_s[3][row]));
           unit = ldexpf(1.f, top > 0.f ? min(max(8 - ilogbf(top), -110), 110) : 0);
         }
 #pragma unroll 1
-        for (int c = 0; c < HD / 64; ++c) {
-          uint32_t w[16];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint4 v = piece(c * 4 + i);
-            w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
-          }
+        for (int c = 0; c < HD / 32; ++c) {
+          const uint4 v = piece(c);
+          uint32_t w[4] = {v.x, v.y, v.z, v.w};
           if (Q8) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) w[i] = pack16(true, __uint_as_float(w[i] << 16) * unit, __uint_as_float(w[i] & 0xffff0000u) * unit);
+            for (int i = 0; i < 4; ++i) w[i] = pack16(true, __uint_as_float(w[i] << 16) * unit, __uint_as_float(w[i] & 0xffff0000u) * unit);
           }
           __syncwarp();
-          tmem_st_32x16(lane_addr + C::Q_COL + half * (HD / 4) + c * 16, w);
+          asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(lane_addr + C::Q_COL + quarter * (HD / 8) + c * 4),
+                       "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
         }
         tmem_st_wait();
         tc_fence_before();                                // and O of the stretch before has been read
@@ -443,12 +460,14 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
       const int row_lo = a.window > 0 ? max(0, x.s.pos + max(__popcll(vis), 1) - a.window) : 0;
       const bool works = (warp & 3) * 32 < x.n_rows;            // some row of this warp is real
       const F2 unit2 = f2(q_unit, q_unit);
-      float m = -CUDART_INF_F, l = 0.f;
-      for (int j = 0; j < blocks; ++j, ++n) {
-        ok = ok && wait_warp(bar(S_FULL + (n & 1)), (n >> 1) & 1, abort_smem, a.status, SITE_TMEM_FULL);
+      const int before = n;
+      float m = -CUDART_INF_F, l = 0.f;                   // the point that l is relative to
+      for (int j = (n & 1) ^ group; j < blocks; j += 2) {
+        const int n = before + j;
+        ok = ok && wait_warp(bar(S_FULL + n % NB), n / NB & 1, abort_smem, a.status, SITE_TMEM_FULL);
         if (Q8) ok = ok && wait_warp(bar(SC_FULL + n % SCALES), (n / SCALES) & 1, abort_smem, a.status, SITE_SMEM_FULL);
         tc_fence_after();
-        const uint32_t s_addr = lane_addr + C::S_COL + (n & 1) * KB;
+        const uint32_t s_addr = lane_addr + C::S_COL + n % NB * KB;
         const int slot0 = x.k_lo + j * KB;
         const bool masked = masked_block(a, x, slot0);
         const float4* ks = reinterpret_cast<const float4*>(scale_s + (n % SCALES) * 3 * KB + half * HALF);
@@ -489,20 +508,33 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
           }
           float top = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
           if (!Q8) top *= q_unit;
-          top_s[n & 1][half][row] = top;
+          top_s[group][n >> 1 & 1][half][row] = top;
         }
         both();                                           // and every score is in registers: P may overwrite them
+        if (!works && half == 0) mbar_arrive(bar(M_READY + group));
         if (works) {
-          const float top = fmaxf(top_s[n & 1][0][row], top_s[n & 1][1][row]);
-          float alpha = 1.f;
-          if (top - LIFT > m + 8.f) {                     // also the first block with a visible key (m = -inf)
-            alpha = ex2(m - (top - LIFT));
-            m = top - LIFT;
+          const float top = fmaxf(top_s[group][n >> 1 & 1][0][row], top_s[group][n >> 1 & 1][1][row]);
+          float alpha = 1.f, now = -CUDART_INF_F;         // the point that the other group left for the block before
+          if (j > 0) {
+            ok = ok && wait_warp(bar(M_READY + (group ^ 1)), (n - 1) >> 1 & 1, abort_smem, a.status, SITE_SMEM_FULL);
+            now = m_s[group ^ 1][row];
+          }
+          if (top - LIFT > now + 8.f) {                   // also the first block with a visible key (now = -inf)
+            alpha = ex2(now - (top - LIFT));
+            now = top - LIFT;
+          }
+          if (half == 0) {
+            m_s[group][row] = now;
+            mbar_arrive(bar(M_READY + group));
+          }
+          if (m != now) {
+            l *= ex2(m - now);                            // nothing summed yet: 0
+            m = now;
           }
           // tcgen05.ld / .st are warp-collective: the decision must be the same for all rows of a warp.  Never for the first
           // block: its product overwrites O.
           if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-            ok = ok && wait_warp(bar(O_DONE + ((n - 1) & 1)), ((n - 1) >> 1) & 1, abort_smem, a.status, SITE_TMEM_EMPTY);
+            ok = ok && wait_warp(bar(O_DONE + (n - 1) % NB), (n - 1) / NB & 1, abort_smem, a.status, SITE_TMEM_EMPTY);
             tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < HD / 32; ++c) {           // half of the columns each
@@ -539,43 +571,50 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
           tmem_st_32x16(s_addr + half * (HALF / 2), w);
           float s0, s1;
           unpack(add2(sum2[0], sum2[1]), s0, s1);
-          l = l * alpha + s0 + s1;
+          l += s0 + s1;
           tmem_st_wait();
         }
         tc_fence_before();
-        mbar_arrive(bar(P_FULL + (n & 1)));
+        mbar_arrive(bar(P_FULL + n % NB));
       }
-      // ---- the stretch's result: final, or a share of it; half of the columns each
+      n += blocks;
+      // ---- the stretch's result: final, or a share of it; a quarter of the columns each
       if (blocks > 0) {
-        ok = ok && wait_warp(bar(O_DONE + ((n - 1) & 1)), ((n - 1) >> 1) & 1, abort_smem, a.status, SITE_TMEM_FULL);
+        ok = ok && wait_warp(bar(O_DONE + (n - 1) % NB), (n - 1) / NB & 1, abort_smem, a.status, SITE_TMEM_FULL);
         tc_fence_after();
       }
-      sum_s[half][row] = l;
-      both();
-      l += sum_s[half ^ 1][row];
-      both();                                             // the sums have been read
+      all();                                              // every point that is waited for has been read
+      if (half == 0) m_s[group][row] = m;
+      sum_s[quarter][row] = l;
+      all();
+      {                                                   // the later point of the two; sums of both groups brought to it
+        const float m0 = m_s[0][row], m1 = m_s[1][row], ref = fmaxf(m0, m1), at = ref == -CUDART_INF_F ? 0.f : ref;
+        l = (sum_s[0][row] + sum_s[1][row]) * ex2(m0 - at) + (sum_s[2][row] + sum_s[3][row]) * ex2(m1 - at);
+        m = ref;
+      }
+      all();                                              // they have been read
       if (!ok || !works) continue;
       const bool spoilt = !Q8 && spoilt_s[stretch & 7] == stretch + 1;
       const float inv = !x.whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
       __nv_bfloat16* dst = a.out + x.b * a.o_sb + t * a.o_st + (long long)h * HD;
       const bool vec = (reinterpret_cast<uintptr_t>(dst) & 15) == 0;
 #pragma unroll 1
-      for (int c = half * (HD / 64); c < (half + 1) * (HD / 64); ++c) {
-        uint32_t o[32];
+      for (int c = quarter * (HD / 64); c < (quarter + 1) * (HD / 64); ++c) {
+        uint32_t o[16];
         if (blocks > 0) {
-          tmem_ld_32x32(lane_addr + C::O_COL + c * 32, o);
+          tmem_ld_32x16(lane_addr + C::O_COL + c * 16, o);
           tmem_ld_wait();
         } else {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = 0;
+          for (int i = 0; i < 16; ++i) o[i] = 0;
         }
         if (spoilt) {                                     // seldom: values of the masked blocks that are not finite
-          const __nv_bfloat16* v0 = reinterpret_cast<const __nv_bfloat16*>(a.v) + ((long long)x.b * a.kv_heads + x.hk) * a.max_seq * HD + c * 32;
+          const __nv_bfloat16* v0 = reinterpret_cast<const __nv_bfloat16*>(a.v) + ((long long)x.b * a.kv_heads + x.hk) * a.max_seq * HD + c * 16;
           for (int slot = x.k_lo; slot < x.k_hi; ++slot) {
             if (!masked_block(a, x, x.k_lo + (slot - x.k_lo) / KB * KB)) continue;
             if (!(seen(x, row_lo, vis, slot) & 1u)) continue;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
+            for (int i = 0; i < 16; ++i) {
               const float f = __bfloat162float(v0[(long long)slot * HD + i]);
               o[i] = __float_as_uint(__uint_as_float(o[i]) + (fabsf(f) < CUDART_INF_F ? 0.f : f));
             }
@@ -584,26 +623,26 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
         }
         // the loads above are warp-collective: every lane takes part, only the stores depend on the row being real
         if (real && x.whole) {
-          uint32_t w[16];
+          uint32_t w[8];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) w[i] = pack16(false, __uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
-          uint32_t* p = reinterpret_cast<uint32_t*>(dst + c * 32);
+          for (int i = 0; i < 8; ++i) w[i] = pack16(false, __uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+          uint32_t* p = reinterpret_cast<uint32_t*>(dst + c * 16);
           if (vec) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) reinterpret_cast<uint4*>(p)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+            reinterpret_cast<uint4*>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+            reinterpret_cast<uint4*>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
           } else {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) p[i] = w[i];
+            for (int i = 0; i < 8; ++i) p[i] = w[i];
           }
         } else if (real) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            a.part[(x.slot * (HD / 4) + c * 8 + i) * TT + row] =
+          for (int i = 0; i < 4; ++i)
+            a.part[(x.slot * (HD / 4) + c * 4 + i) * TT + row] =
                 make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
         }
         __syncwarp();
       }
-      if (!x.whole && real && half == 0) a.part_ml[x.slot * TT + row] = make_float2(m, l);
+      if (!x.whole && real && quarter == 0) a.part_ml[x.slot * TT + row] = make_float2(m, l);
       __syncwarp();
     }
   }
@@ -677,7 +716,7 @@ __global__ void __launch_bounds__(GROUPS * TT) wide_join_kernel(const __grid_con
 template <int HD, bool Q8>
 int run(const Args& p, void* stream) {
   using C = Wide<HD, Q8>;
-  static_assert(C::SMEM <= 222 * 1024 && C::CPT * CHUNK == KB * C::RB && C::Q_COL + HD / 2 <= 512 && SCALES >= C::STAGES + 2, "shared memory of a CTA");
+  static_assert(C::SMEM <= 222 * 1024 && C::CPT * CHUNK == KB * C::RB && C::Q_COL + HD / 2 <= 512 && SCALES >= C::STAGES + C::NB, "shared memory of a CTA");
   static std::atomic<unsigned long long> configured{0};   // a bit per device
   int dev = 0;
   MESH_CUDA_OK(cudaGetDevice(&dev));
