@@ -2,9 +2,9 @@
 //
 // A tile is 128 query rows of one (sequence, KV head); a CTA goes through its stretches of 64-key blocks (how the work is cut and
 // the formulas: draft_attention.cuh, draft_attention.cu).  Warps 0-15: softmax, in two groups that take the blocks in turn, in each
-// two threads per query row with half of the block's keys.  Warps 16-22: keys and values, a warp per 4 KB of a tile, into the 128-byte
+// two threads per query row with half of the block's keys.  Warps 16-21: keys and values, a warp per 4 KB of a tile, into the 128-byte
 // swizzle of the operands: bf16 rows by cp.async; 8-bit codes copied in bulk to places of the warp's own and widened to
-// fp16 from there.  Warp 23: the products S = Q K^T and O += P V by one elected lane, S up to three blocks ahead of P V.
+// fp16 from there.  Warps 22 and 23: the products S = Q K^T, up to three blocks ahead, and O += P V, by one elected lane each.
 // Tensor memory holds the queries (operand A of the first product, 16 bits), S of four blocks (heads of 256: two), of each of
 // which P (16 bits, operand A of the second) overwrites the first half, and O, which is rescaled only when a row's maximum
 // has grown by more than 2^8: the reference point of a row goes from group to group through shared memory.
@@ -23,8 +23,8 @@ namespace draft {
 namespace {
 
 constexpr int TT = WIDE_ROWS, KB = WIDE_UNIT;               // rows of a tile, keys of a block
-constexpr int GROUP = 256, SOFT = 2 * GROUP, LOAD_WARPS = 7, THREADS = SOFT + 32 * LOAD_WARPS + 32;
-constexpr int LOAD_WARP = SOFT / 32, PRODUCT_WARP = LOAD_WARP + LOAD_WARPS;
+constexpr int GROUP = 256, SOFT = 2 * GROUP, LOAD_WARPS = 6, THREADS = SOFT + 32 * LOAD_WARPS + 64;
+constexpr int LOAD_WARP = SOFT / 32, S_WARP = LOAD_WARP + LOAD_WARPS, O_WARP = S_WARP + 1;
 constexpr int SCALES = 8;                                   // blocks whose scales are kept: stages and buffers of S together
 constexpr int CHUNK = 4096, PIECES = CHUNK / (32 * 16);     // bytes of stored rows a warp takes at a time; 16-byte pieces of a lane
 
@@ -35,10 +35,10 @@ struct Wide {
   static constexpr int NB = HD < 256 ? 4 : 2;               // blocks whose S is in tensor memory
   static constexpr int RB = Q8 ? HD : 2 * HD, NC = RB / 16;           // bytes and 16-byte pieces of a stored row
   static constexpr int CPT = KB * RB / CHUNK;               // chunks of a tile
-  // Chunks of bf16 rows that a warp has under way.  While it waits for the place of a tile of values the product that frees it waits for
-  // tiles of keys up to 2 STAGES - 2 NB + 4 before that one: what the warp has not handed over must be younger.
-  static constexpr int BEHIND = CPT >= 4 ? 2 : 1;
-  static_assert(Q8 || (BEHIND - 1) * LOAD_WARPS <= (2 * STAGES - 2 * NB + 3) * CPT, "a loader would wait for what it has not handed over");
+  // Chunks of bf16 rows that a warp has under way.  While it waits for a place, the product that frees it waits for tiles of at least
+  // 2 STAGES - 1 before: what the warp has not handed over must be younger.
+  static constexpr int BEHIND = CPT >= 4 ? 3 : 2;
+  static_assert(Q8 || (BEHIND - 1) * LOAD_WARPS <= (2 * STAGES - 2) * CPT, "a loader would wait for what it has not handed over");
   static constexpr int RAWS = Q8 ? 3 : 0;                   // chunks of codes that a warp has under way
   static constexpr int N_BARS = 1 + 4 * STAGES + 3 * NB + 2 + SCALES + RAWS * LOAD_WARPS;
   static constexpr int SCALE_BYTES = Q8 ? SCALES * 3 * KB * 4 : 0;
@@ -138,6 +138,7 @@ struct Tiles {                                             // (the walk apart: w
 template <int HD, bool Q8>
 __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant__ Args a) {
   using C = Wide<HD, Q8>;
+  constexpr uint32_t FP16 = Q8 ? (1u << 7) | (1u << 10) : 0u;              // operands in fp16 instead of bf16
   constexpr int STAGES = C::STAGES, NC = C::NC, NB = C::NB;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -177,7 +178,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
     for (int s = 0; s < 8; ++s) spoilt_s[s] = 0;
     fence_mbar_init();
   }
-  if (warp == PRODUCT_WARP) {
+  if (warp == O_WARP) {
     tmem_alloc<1>(smem_u32(tmem_slot), 512);
     tmem_relinquish<1>();
   }
@@ -192,7 +193,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
   Stretch x;
   bool ok = true;
 
-  if (warp >= LOAD_WARP && warp < PRODUCT_WARP) {
+  if (warp >= LOAD_WARP && warp < S_WARP) {
     // ------------------------------------------------------------------ keys and values
     // Chunk q of all is warp q mod LOAD_WARPS's.
     Tiles t;
@@ -252,17 +253,18 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
         uint8_t* dst = gen + ((t.key ? sK : sV) + s * C::TILE - base);
 #pragma unroll 4
         for (int i = 0; i < PIECES; ++i) {
-          const int idx = part * (CHUNK / 16) + i * 32 + lane, r = idx / NC, c = idx % NC;
-          uint4 v = *reinterpret_cast<const uint4*>(src + (i * 32 + lane) * 16);
+          // the eight lanes of a phase store to eight different 16-byte banks: four pieces of each of two rows that follow one another
+          const int at = NC == 4 ? lane : NC == 8 ? (lane & 19) | (lane & 4) << 1 | (lane & 8) >> 1 : (lane & 3) | (lane & 4) << 2 | (lane & 24) >> 1;
+          const int idx = part * (CHUNK / 16) + i * 32 + at, r = idx / NC, c = idx % NC;
+          uint4 v = *reinterpret_cast<const uint4*>(src + (i * 32 + at) * 16);
           if (r >= rows) v = make_uint4(0, 0, 0, 0);
           uint8_t* p = dst + (c >> 2) * (KB * 128) + r * 128;
           const uint32_t w[4] = {v.x ^ 0x80808080u, v.y ^ 0x80808080u, v.z ^ 0x80808080u, v.w ^ 0x80808080u};
           const uint4 lo = make_uint4(codes2(w[0], 0x4140), codes2(w[0], 0x4342), codes2(w[1], 0x4140), codes2(w[1], 0x4342));
           const uint4 hi = make_uint4(codes2(w[2], 0x4140), codes2(w[2], 0x4342), codes2(w[3], 0x4140), codes2(w[3], 0x4342));
-          // the eight lanes of a phase on eight different 16-byte banks: every other group of columns begins with its odd piece
-          const int odd = c >> 2 & 1, c0 = 2 * (c & 3);
-          *reinterpret_cast<uint4*>(p + (((c0 + odd) ^ (r & 7)) << 4)) = odd ? hi : lo;
-          *reinterpret_cast<uint4*>(p + (((c0 + 1 - odd) ^ (r & 7)) << 4)) = odd ? lo : hi;
+          const int c0 = 2 * (c & 3);
+          *reinterpret_cast<uint4*>(p + ((c0 ^ (r & 7)) << 4)) = lo;
+          *reinterpret_cast<uint4*>(p + (((c0 + 1) ^ (r & 7)) << 4)) = hi;
         }
         if (scales) {
           float* sc = scale_s + (t.n() % SCALES) * 3 * KB + lane;
@@ -290,8 +292,9 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
       uint32_t full[C::BEHIND] = {}, clean[C::BEHIND] = {};
       int of[C::BEHIND] = {};
       bool more = true;
+      int under_way = 0;
 #pragma unroll 1
-      for (int q = w0; ok && (more || full[C::BEHIND - 1]); q += LOAD_WARPS) {
+      for (int q = w0; ok && (more || under_way > 0); q += LOAD_WARPS) {
         if (full[C::BEHIND - 1]) {
           asm volatile("cp.async.wait_group %0;" ::"n"(C::BEHIND - 1) : "memory");
           if (clean[C::BEHIND - 1]) {
@@ -312,6 +315,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) mbar_arrive(full[C::BEHIND - 1]);
+          --under_way;
         }
         uint32_t new_full = 0, new_clean = 0;
         if (more) more = t.find(a, walk, q / C::CPT);
@@ -327,6 +331,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
             copy16(dst + (c >> 3) * (KB * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4), src + (r < rows ? idx * 16 : 0), r < rows);
           }
           new_full = bar((t.key ? K_FULL : V_FULL) + s);
+          ++under_way;
           if (!t.key && masked_block(a, t.x, t.slot())) new_clean = dst + part * (CHUNK / C::RB) * 128;
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -341,53 +346,63 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
         of[0] = t.stretch;
       }
     }
-  } else if (warp == PRODUCT_WARP) {
-    // ------------------------------------------------------------------ products (warp-uniform, one elected lane issues)
-    constexpr uint32_t half = Q8 ? (1u << 7) | (1u << 10) : 0u;              // operands in fp16 instead of bf16
-    constexpr uint32_t idesc_s = umma_idesc_bf16(TT, KB, 0, 0) & ~half, idesc_o = umma_idesc_bf16(TT, HD, 0, 1) & ~half;
+  } else if (warp == S_WARP) {
+    // ------------------------------------------------------------------ S = Q K^T (warp-uniform, one elected lane issues)
+    constexpr uint32_t idesc = umma_idesc_bf16(TT, KB, 0, 0) & ~FP16;
     const bool leader = elect_one();
-    const uint64_t dk0 = umma_smem_desc(sK, 16, 1024), dv0 = umma_smem_desc(sV, KB * 128, 1024);
+    const uint64_t dk0 = umma_smem_desc(sK, 16, 1024);
     int n = 0, visit = 0;                                 // blocks and stretches done
-    auto issue_s = [&](int n) {
-      const int s = n % STAGES;
-      ok = wait_warp(bar(K_FULL + s), (n / STAGES) & 1, abort_smem, a.status, SITE_SMEM_FULL);
-      if (!ok) return;
-      tc_fence_after();
-      if (leader) {
-#pragma unroll
-        for (int k = 0; k < HD / 16; ++k) {
-          const int off = ((k / 4) * (KB * 128) + (k % 4) * 32) / 16;
-          umma_f16_ts(tmem + C::S_COL + n % NB * KB, tmem + C::Q_COL + k * 8, dk0 + (uint32_t)(s * (C::TILE >> 4)) + off, idesc_s, k ? 1u : 0u);
-        }
-        umma_commit(bar(K_EMPTY + s));
-        umma_commit(bar(S_FULL + n % NB));
-      }
-      __syncwarp();
-    };
     for (Stretch y; ok && next_stretch(a, walk, y);) {
       const int blocks = blocks_of(y);
       if (blocks == 0) continue;
       ok = wait_warp(bar(Q_FULL), visit++ & 1, abort_smem, a.status, SITE_SMEM_FULL);
+      const int first = n;
       if (lane == 0) over_s = n;
-      for (int i = 0; ok && i < NB - 1 && i < blocks; ++i) issue_s(n + i);
-      for (int j = 0; ok && j < blocks; ++j, ++n) {
-        // The S issued next overwrites the P that the product before reads, and products of different shapes are not ordered among
-        // themselves: that one's end is waited for.  (So by the time a block's scores are there, the product NB blocks back
-        // is over: a wait for the end of a product, on one of NB barriers in turn, cannot be answered by the phase before.)
-        if (j > 0) {
-          ok = wait_warp(bar(O_DONE + (n - 1) % NB), (n - 1) / NB & 1, abort_smem, a.status, SITE_TMEM_EMPTY);
-          if (lane == 0) over_s = n;
+#pragma unroll 1
+      for (; ok && n < first + blocks; ++n) {
+        // This S overwrites the P that the product NB blocks back reads: that one's end is waited for.  (So by the time a block's
+        // scores are there, that product is over: a wait for the end of a product, on one of NB barriers in turn, cannot be
+        // answered by the phase before.)
+        if (n >= first + NB) {
+          ok = wait_warp(bar(O_DONE + n % NB), (n / NB - 1) & 1, abort_smem, a.status, SITE_TMEM_EMPTY);
+          if (lane == 0) over_s = n - NB + 1;
         }
-        if (ok && j + NB - 1 < blocks) issue_s(n + NB - 1);
         const int s = n % STAGES;
-        if (ok) ok = wait_warp(bar(V_FULL + s), (n / STAGES) & 1, abort_smem, a.status, SITE_SMEM_FULL);
-        if (ok) ok = wait_warp(bar(P_FULL + n % NB), n / NB & 1, abort_smem, a.status, SITE_TMEM_FULL);
+        ok = ok && wait_warp(bar(K_FULL + s), (n / STAGES) & 1, abort_smem, a.status, SITE_SMEM_FULL);
         if (!ok) break;
         tc_fence_after();
         if (leader) {
+          const uint32_t d = tmem + C::S_COL + n % NB * KB;
+          const uint64_t dk = dk0 + (uint32_t)(s * (C::TILE >> 4));
 #pragma unroll
-          for (int k = 0; k < KB / 16; ++k)
-            umma_f16_ts(tmem + C::O_COL, tmem + C::S_COL + n % NB * KB + k * 8, dv0 + (uint32_t)(s * (C::TILE >> 4)) + k * 128, idesc_o, (j | k) ? 1u : 0u);
+          for (int k = 0; k < HD / 16; ++k)
+            umma_f16_ts(d, tmem + C::Q_COL + k * 8, dk + ((k / 4) * (KB * 128) + (k % 4) * 32) / 16, idesc, k ? 1u : 0u);
+          umma_commit(bar(K_EMPTY + s));
+          umma_commit(bar(S_FULL + n % NB));
+        }
+        __syncwarp();
+      }
+    }
+  } else if (warp == O_WARP) {
+    // ------------------------------------------------------------------ O += P V
+    constexpr uint32_t idesc = umma_idesc_bf16(TT, HD, 0, 1) & ~FP16;                       // B = V is MN-major
+    const bool leader = elect_one();
+    const uint64_t dv0 = umma_smem_desc(sV, KB * 128, 1024);
+    int n = 0;
+    for (Stretch y; ok && next_stretch(a, walk, y);) {
+      const int first = n, blocks = blocks_of(y);
+#pragma unroll 1
+      for (; ok && n < first + blocks; ++n) {
+        const int s = n % STAGES;
+        ok = wait_warp(bar(V_FULL + s), (n / STAGES) & 1, abort_smem, a.status, SITE_SMEM_FULL);
+        ok = ok && wait_warp(bar(P_FULL + n % NB), n / NB & 1, abort_smem, a.status, SITE_TMEM_FULL);
+        if (!ok) break;
+        tc_fence_after();
+        if (leader) {
+          const uint32_t p = tmem + C::S_COL + n % NB * KB;
+          const uint64_t dv = dv0 + (uint32_t)(s * (C::TILE >> 4));
+#pragma unroll
+          for (int k = 0; k < KB / 16; ++k) umma_f16_ts(tmem + C::O_COL, p + k * 8, dv + k * 128, idesc, k ? 1u : n > first ? 1u : 0u);
           umma_commit(bar(V_EMPTY + s));
           umma_commit(bar(O_DONE + n % NB));
         }
@@ -648,7 +663,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == PRODUCT_WARP) {
+  if (warp == O_WARP) {
     tc_fence_after();
     tmem_dealloc<1>(tmem, 512);
   }
