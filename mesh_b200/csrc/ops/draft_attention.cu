@@ -45,11 +45,13 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
 
 template <int HD, bool Q8>
 struct Cfg {
-  static constexpr int RB = Q8 ? HD : 2 * HD;             // bytes of a row
-  static constexpr int NC = RB / 16;                      // 16-byte chunks of a row
+  static constexpr int NT = HD / 8;                       // column tiles of the output
+  static constexpr int RB = Q8 ? HD : 2 * HD, NC = RB / 16;           // bytes and 16-byte chunks of a row
   static constexpr int STAGE = 2 * KEYS * RB + (Q8 ? 2 * KEYS * 4 : 0);
-  static constexpr int WARPS = STAGE > 9000 ? 4 : 8;
-  static constexpr int STAGES = (200 * 1024 / WARPS) / STAGE > 8 ? 8 : (200 * 1024 / WARPS) / STAGE;
+  // As many warps as their registers allow (half of a warp's are the output's), four where a block is 16 KB.  Heads of 128 in 8 bits:
+  // 151 us with 12 warps, 162 with 8; two warps to a block with half of the columns each, 16 in all, 185.
+  static constexpr int WARPS = STAGE > 9000 ? 4 : HD == 256 ? 8 : HD == 128 ? 12 : 16;
+  static constexpr int ROOM = 200 * 1024 / WARPS, STAGES = ROOM / STAGE > 8 ? 8 : ROOM / STAGE;
   static constexpr int RING = WARPS * STAGES * STAGE;
   static constexpr int QB = ROWS * HD * 2;
   static constexpr int UNIT = WARPS * KEYS;               // keys of a unit of work
@@ -80,16 +82,15 @@ __device__ __forceinline__ bool finite_rows(const uint8_t* rows, int lane) {
   return !__any_sync(0xffffffffu, bad);
 }
 
-// Values i % VW of column group n' = 0..7 of group i / VW: the column that tile i's n' is.
+// The column that n' = 0..7 of output tile i is: the tiles are values i % VW of the column groups n' of group i / VW.
 template <int VW>
 __device__ __forceinline__ int column(int i, int n) { return ((i / VW) * 8 + n) * VW + i % VW; }
 
 template <int HD, bool Q8>
 __global__ void __launch_bounds__(Cfg<HD, Q8>::WARPS * 32, 1) attention_kernel(const __grid_constant__ Args a) {
   using C = Cfg<HD, Q8>;
-  constexpr int RB = C::RB, NC = C::NC, STAGES = C::STAGES, PER = C::PER, VW = C::VW;
+  constexpr int RB = C::RB, NC = C::NC, STAGES = C::STAGES, PER = C::PER, VW = C::VW, NT = C::NT;
   constexpr int KI = HD / (4 * PER);                      // chunks of a key per lane
-  constexpr int NT = HD / 8;                              // column tiles of the output
   extern __shared__ __align__(128) uint8_t smem[];
   uint4* q_s = reinterpret_cast<uint4*>(smem);            // [k step][lane]: operand A of the scores
   __shared__ float unit_s[ROWS], weight_s[C::WARPS][ROWS], m_s[ROWS], l_s[ROWS];
@@ -397,21 +398,24 @@ __global__ void __launch_bounds__(Cfg<HD, Q8>::WARPS * 32, 1) attention_kernel(c
   }
   __syncthreads();
   const bool whole = x.whole;
-  const long long slot = x.slot;
+  const int slot = x.slot;
   __nv_bfloat16* row_s = reinterpret_cast<__nv_bfloat16*>(smem);          // the queries' memory and, after a barrier, more
-  float4 sum[(NT * 32 + C::WARPS * 32 - 1) / (C::WARPS * 32)];
+  constexpr int TURNS = (NT + C::WARPS - 1) / C::WARPS;   // tiles of the output that a warp sums
+  float4 sum[TURNS];
 #pragma unroll
-  for (int y = 0; y < NT / C::WARPS; ++y) {
+  for (int y = 0; y < TURNS; ++y) {
     const int i = y * C::WARPS + warp;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (i < NT) {
 #pragma unroll
-    for (int w = 0; w < C::WARPS; ++w) {
-      const float w0 = weight_s[w][n], w1 = weight_s[w][n + 8];
-      const float4 v = o_s[(w * NT + i) * 32 + lane];
-      acc.x += w0 * v.x; acc.y += w0 * v.y; acc.z += w1 * v.z; acc.w += w1 * v.w;
+      for (int w = 0; w < C::WARPS; ++w) {
+        const float w0 = weight_s[w][n], w1 = weight_s[w][n + 8];
+        const float4 v = o_s[(w * NT + i) * 32 + lane];
+        acc.x += w0 * v.x; acc.y += w0 * v.y; acc.z += w1 * v.z; acc.w += w1 * v.w;
+      }
+      if (!whole) a.part[((long long)slot * NT + i) * 32 + lane] = acc;
     }
     sum[y] = acc;
-    if (!whole) a.part[(slot * NT + i) * 32 + lane] = acc;
   }
   if (!whole) {
     if (threadIdx.x < ROWS) a.part_ml[slot * ROWS + threadIdx.x] = make_float2(m_s[threadIdx.x], l_s[threadIdx.x]);
@@ -419,11 +423,12 @@ __global__ void __launch_bounds__(Cfg<HD, Q8>::WARPS * 32, 1) attention_kernel(c
     __syncthreads();
     const float i0 = l_s[n] == 0.f ? 0.f : 1.f / l_s[n], i1 = l_s[n + 8] == 0.f ? 0.f : 1.f / l_s[n + 8];
 #pragma unroll
-    for (int y = 0; y < NT / C::WARPS; ++y) {
+    for (int y = 0; y < TURNS; ++y) {
       const int i = y * C::WARPS + warp;
+      if (i >= NT) continue;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int col = column<VW>(i, 2 * t4 + e);
+        const int col = column<C::VW>(i, 2 * t4 + e);
         row_s[n * C::OUT_PITCH + col] = __float2bfloat16_rn((e ? sum[y].y : sum[y].x) * i0);
         row_s[(n + 8) * C::OUT_PITCH + col] = __float2bfloat16_rn((e ? sum[y].w : sum[y].z) * i1);
       }
@@ -439,78 +444,84 @@ __global__ void __launch_bounds__(Cfg<HD, Q8>::WARPS * 32, 1) attention_kernel(c
   }
 }
 
-// Joins the shares of the items that were cut: a CTA per item and tile of 8 columns, whose warps take the shares in turn.
-template <int HD, bool Q8>
+// Joins the shares of the items that were cut.  SPLIT: a CTA per item and tile of 8 columns, whose warps take the shares in turn (few items
+// in many shares); else a CTA per item, whose warps take the tiles of columns.
+template <int HD, bool Q8, bool SPLIT>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args a) {
   using C = Cfg<HD, Q8>;
-  constexpr int NT = HD / 8;
-  __shared__ long long c_s[3];
+  constexpr int NT = HD / 8, EACH = SPLIT ? 8 : 1;        // warps among which an item's shares are dealt
+  __shared__ int c_s[3];
   __shared__ float m_s[8][ROWS], l_s[8][ROWS];
   __shared__ float4 o_s[8][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = lane >> 2, t4 = lane & 3, G = a.q_heads / a.kv_heads;
-  const int i = blockIdx.y, tile = blockIdx.x % a.tiles, hk = blockIdx.x / a.tiles % a.kv_heads, b = blockIdx.x / a.tiles / a.kv_heads;
+  const int tile = blockIdx.x % a.tiles, hk = blockIdx.x / a.tiles % a.kv_heads, b = blockIdx.x / a.tiles / a.kv_heads;
   // All wait: what comes after this kernel relies on the one before it.  And none looks at the lengths before: they are older than
   // that kernel, but only the wait keeps a read from finding what its line held before them.
   griddep_wait();
   if (warp == 0) shares_of_item(a, b, hk, tile, c_s);
   __syncthreads();
-  const long long c0 = c_s[0], c1 = c_s[1];
-  const int odd = (int)c_s[2];
+  const int c0 = c_s[0], c1 = c_s[1], odd = c_s[2];
   if (c0 == c1) return;                                   // whole in one CTA, or not there
-  float m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.f, 0.f};
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (long long c = c0 + warp; c <= c1; c += 8 * 4) {
-    float2 x[4][2];
-    float4 v[4];
-#pragma unroll
-    for (int y = 0; y < 4; ++y) {
-      const long long cc = c + 8 * y, slot = 2 * cc + (cc == c0 ? odd : 0);
-      x[y][0] = x[y][1] = make_float2(-CUDART_INF_F, 0.f);
-      v[y] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (cc <= c1) {
-        x[y][0] = __ldcg(a.part_ml + slot * ROWS + n);
-        x[y][1] = __ldcg(a.part_ml + slot * ROWS + n + 8);
-        v[y] = __ldcg(a.part + (slot * NT + i) * 32 + lane);
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      float now = m[j];
-#pragma unroll
-      for (int y = 0; y < 4; ++y) now = fmaxf(now, x[y][j].x);
-      const float ref = now == -CUDART_INF_F ? 0.f : now, old = ex2(m[j] - ref);
-      m[j] = now;
-      l[j] *= old;
-      if (j == 0) { acc.x *= old; acc.y *= old; } else { acc.z *= old; acc.w *= old; }
+  const int n_rows = sequence(a, b).count * G - tile * ROWS;
+  for (int i = SPLIT ? blockIdx.y : warp; i < NT; i += SPLIT ? NT : 8) {
+    float m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.f, 0.f};
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c = c0 + (SPLIT ? warp : 0); c <= c1; c += EACH * 4) {
+      float2 x[4][2];
+      float4 v[4];
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
-        const float wt = ex2(x[y][j].x - ref);
-        l[j] += wt * x[y][j].y;
-        if (j == 0) { acc.x += wt * v[y].x; acc.y += wt * v[y].y; } else { acc.z += wt * v[y].z; acc.w += wt * v[y].w; }
+        const int cc = c + EACH * y;
+        const long long slot = 2 * cc + (cc == c0 ? odd : 0);
+        x[y][0] = x[y][1] = make_float2(-CUDART_INF_F, 0.f);
+        v[y] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (cc <= c1) {
+          x[y][0] = __ldcg(a.part_ml + slot * ROWS + n);
+          x[y][1] = __ldcg(a.part_ml + slot * ROWS + n + 8);
+          v[y] = __ldcg(a.part + (slot * NT + i) * 32 + lane);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float now = m[j];
+#pragma unroll
+        for (int y = 0; y < 4; ++y) now = fmaxf(now, x[y][j].x);
+        const float ref = now == -CUDART_INF_F ? 0.f : now, old = ex2(m[j] - ref);
+        m[j] = now;
+        l[j] *= old;
+        if (j == 0) { acc.x *= old; acc.y *= old; } else { acc.z *= old; acc.w *= old; }
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const float wt = ex2(x[y][j].x - ref);
+          l[j] += wt * x[y][j].y;
+          if (j == 0) { acc.x += wt * v[y].x; acc.y += wt * v[y].y; } else { acc.z += wt * v[y].z; acc.w += wt * v[y].w; }
+        }
       }
     }
+    o_s[warp][lane] = acc;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      if (t4 == 0) { m_s[warp][n + 8 * j] = m[j]; l_s[warp][n + 8 * j] = l[j]; }
+    if (SPLIT) __syncthreads();
+    else __syncwarp();
+    // 16 rows x 8 columns; of a whole CTA or of this warp's own sums
+    for (int e = SPLIT ? threadIdx.x : lane; e < ROWS * 8; e += SPLIT ? 256 : 32) {
+      const int row = e >> 3, c = e & 7, r = tile * ROWS + row, w0 = SPLIT ? 0 : warp;
+      if (row >= n_rows) continue;
+      float mm = -CUDART_INF_F, ll = 0.f, sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < EACH; ++w) mm = fmaxf(mm, m_s[w0 + w][row]);
+      const float ref = mm == -CUDART_INF_F ? 0.f : mm;
+#pragma unroll
+      for (int w = 0; w < EACH; ++w) {
+        const float wt = ex2(m_s[w0 + w][row] - ref);
+        ll += wt * l_s[w0 + w][row];
+        sum += wt * reinterpret_cast<const float*>(&o_s[w0 + w][(row & 7) * 4 + (c >> 1)])[2 * (row >> 3) + (c & 1)];
+      }
+      a.out[b * a.o_sb + (r / G) * a.o_st + (long long)(hk * G + r % G) * HD + column<C::VW>(i, c)] = __float2bfloat16_rn(ll == 0.f ? 0.f : sum / ll);
+    }
+    __syncwarp();
   }
-  o_s[warp][lane] = acc;
-#pragma unroll
-  for (int j = 0; j < 2; ++j)
-    if (t4 == 0) { m_s[warp][n + 8 * j] = m[j]; l_s[warp][n + 8 * j] = l[j]; }
-  __syncthreads();
-  // 16 rows x 8 columns: thread -> row, column
-  if (threadIdx.x >= ROWS * 8) return;
-  const int row = threadIdx.x >> 3, c = threadIdx.x & 7, r = tile * ROWS + row;
-  float mm = -CUDART_INF_F, ll = 0.f, sum = 0.f;
-#pragma unroll
-  for (int w = 0; w < 8; ++w) mm = fmaxf(mm, m_s[w][row]);
-  const float ref = mm == -CUDART_INF_F ? 0.f : mm;
-#pragma unroll
-  for (int w = 0; w < 8; ++w) {
-    const float wt = ex2(m_s[w][row] - ref);
-    ll += wt * l_s[w][row];
-    sum += wt * reinterpret_cast<const float*>(&o_s[w][(row & 7) * 4 + (c >> 1)])[2 * (row >> 3) + (c & 1)];
-  }
-  const Seq s = sequence(a, b);
-  if (r < s.count * G)
-    a.out[b * a.o_sb + (r / G) * a.o_st + (long long)(hk * G + r % G) * HD + column<C::VW>(i, c)] = __float2bfloat16_rn(ll == 0.f ? 0.f : sum / ll);
 }
 
 // The kernel for many rows, with tiles of 128, from 17 query rows per KV head on.
@@ -529,6 +540,7 @@ static void cut(const MeshKvCache* c, const MeshDraftAttention* a, Args& p) {
   const long long units = (long long)c->B * c->kv_heads * p.tiles * ((keys + p.unit - 1) / p.unit);
   const long long most = a->splits > 0 ? a->splits : sm_count();
   p.shares = (int)(units < most ? units : most);
+  p.few = a->splits > 0 ? 0 : w ? 32 : 16;
 }
 
 static int check(const MeshKvCache* c, const MeshDraftAttention* a) {
@@ -544,11 +556,10 @@ static int check(const MeshKvCache* c, const MeshDraftAttention* a) {
   return 0;
 }
 
-template <int HD, bool Q8> constexpr bool NT_OK = HD / 8 % Cfg<HD, Q8>::WARPS == 0 && ROWS * Cfg<HD, Q8>::OUT_PITCH * 2 <= Cfg<HD, Q8>::SMEM;
 template <int HD, bool Q8>
 static int run(const Args& p, void* stream) {
   using C = Cfg<HD, Q8>;
-  static_assert(C::STAGES >= 3 && C::SMEM <= 226 * 1024 && NT_OK<HD, Q8>, "ring of a warp");
+  static_assert(C::STAGES >= 2 && C::SMEM <= 224 * 1024 && ROWS * C::OUT_PITCH * 2 <= C::SMEM, "ring of a warp");
   static std::atomic<unsigned long long> configured{0};   // a bit per device
   int dev = 0;
   MESH_CUDA_OK(cudaGetDevice(&dev));
@@ -557,7 +568,11 @@ static int run(const Args& p, void* stream) {
     configured.fetch_or(1ull << (dev & 63));
   }
   MESH_CUDA_OK(launch(attention_kernel<HD, Q8>, dim3(p.shares), C::WARPS * 32, C::SMEM, stream, p));
-  if (p.part) MESH_CUDA_OK(launch(join_kernel<HD, Q8>, dim3((unsigned)(p.B * p.kv_heads * p.tiles), HD / 8), 256, 0, stream, p));
+  if (p.part) {
+    const unsigned items = (unsigned)(p.B * p.kv_heads * p.tiles);
+    if (p.shares > 2ll * items) MESH_CUDA_OK(launch(join_kernel<HD, Q8, true>, dim3(items, HD / 8), 256, 0, stream, p));
+    else MESH_CUDA_OK(launch(join_kernel<HD, Q8, false>, dim3(items), 256, 0, stream, p));
+  }
   return 0;
 }
 
@@ -588,7 +603,8 @@ extern "C" int mesh_draft_attention(const MeshKvCache* c, const MeshDraftAttenti
   p.B = c->B; p.T = a->T; p.q_heads = a->q_heads; p.kv_heads = c->kv_heads; p.max_seq = c->max_seq; p.window = a->window;
   p.status = (Status*)a->status;
   cut(c, a, p);
-  if ((long long)c->B * c->kv_heads * p.tiles > 0x7fffffff) return set_error(-2, "draft_attention: too many rows for one call");
+  if ((long long)c->B * c->kv_heads * p.tiles * ((c->max_seq + p.unit - 1) / p.unit + 1) > 0x7fffffff || p.shares > 0x3fffffff)
+    return set_error(-2, "draft_attention: too many rows and keys for one call");
   p.scale_log2 = a->scale * 1.4426950408889634f;
   if (p.shares > 1) {
     if (!a->scratch || (uintptr_t)a->scratch % 16) return set_error(-2, "draft_attention: scratch memory must be given and start on a multiple of 16 bytes");

@@ -23,6 +23,7 @@ struct Args {
   float scale_log2;                   // scale * log2(e): exponentials are powers of two
   float4* part; float2* part_ml;      // two slots per CTA: the output as its threads hold it, and {m, l} of the rows
   int shares;                         // CTAs of the attention kernel
+  int few;                            // see cut_work; 0: as many shares as CTAs
   Status* status;
 };
 
@@ -65,10 +66,10 @@ __device__ __forceinline__ Seq sequence(const Args& a, int b) {
   return s;
 }
 
-// How the work is cut.  Sequence b has `rows` query rows per KV head in `tiles` tiles and `units` units of keys; its items follow
-// one another, KV head by KV head, tile by tile.
+// How the work is cut.  Sequence b has `tiles` tiles of query rows per KV head and `units` units of keys; its items follow one
+// another, KV head by KV head, tile by tile.  All units together are fewer than 2^31 (checked before the launch).
 struct Load {
-  Seq s; int tiles, units; long long work;
+  Seq s; int tiles, units, work;
 };
 __device__ __forceinline__ Load load_of(const Args& a, int b) {
   Load l;
@@ -76,36 +77,58 @@ __device__ __forceinline__ Load load_of(const Args& a, int b) {
   const int rows = max(l.s.count, 0) * (a.q_heads / a.kv_heads);
   l.tiles = (rows + a.rows - 1) / a.rows;
   l.units = max(1, (l.s.hi - l.s.lo + a.unit - 1) / a.unit);   // rows that see nothing are written too
-  l.work = (long long)l.tiles * l.units * a.kv_heads;
+  l.work = l.tiles * l.units * a.kv_heads;
   return l;
 }
-// Work of all sequences before b, and of all; by a whole warp.
-__device__ __forceinline__ void work_before(const Args& a, int b, long long& before, long long& total) {
+// Work of all sequences before b, and how all of it is shared out; by a whole warp.
+struct Cut {
+  int total, shares, per, more;       // shares of per units, the first `more` of one more
+};
+__device__ __forceinline__ int share_begin(const Cut& c, int i) { return i * c.per + min(i, c.more); }
+__device__ __forceinline__ int share_of(const Cut& c, int w) {
+  const int edge = c.more * (c.per + 1);
+  return w < edge ? w / (c.per + 1) : c.more + (w - edge) / c.per;
+}
+// A share that ends inside an item costs a partial result, written, read and joined, and the next one a new start: some six units'
+// time.  So where shares are short (at most `few` units a CTA), they are whole items or, if these are alike, equal pieces of them.
+__device__ __forceinline__ Cut cut_work(const Args& a, int total, int items) {
+  Cut c;
+  c.total = total;
+  c.shares = min(a.shares, total);
+  if (total <= a.few * a.shares && items < a.shares) c.shares = min(items * (a.shares / max(items, 1)), total);
+  c.shares = max(c.shares, 1);
+  c.per = total / c.shares;
+  c.more = total - c.per * c.shares;
+  return c;
+}
+__device__ __forceinline__ Cut work_before(const Args& a, int b, int& before) {
   const int lane = threadIdx.x & 31;
-  long long lo = 0, all = 0;
+  int lo = 0, all = 0, items = 0;
   for (int i = lane; i < a.B; i += 32) {
-    const long long w = load_of(a, i).work;
-    all += w;
-    if (i < b) lo += w;
+    const Load l = load_of(a, i);
+    all += l.work;
+    items += l.tiles * a.kv_heads;
+    if (i < b) lo += l.work;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     lo += __shfl_xor_sync(0xffffffffu, lo, o);
     all += __shfl_xor_sync(0xffffffffu, all, o);
+    items += __shfl_xor_sync(0xffffffffu, items, o);
   }
   before = lo;
-  total = all;
+  return cut_work(a, all, items);
 }
 // The sequence that unit w of the work belongs to, and the work before it; by a whole warp.  w < total.
-__device__ __forceinline__ int sequence_of(const Args& a, long long w, long long& before) {
+__device__ __forceinline__ int sequence_of(const Args& a, int w, int& before) {
   const int lane = threadIdx.x & 31;
   before = 0;
   for (int i0 = 0; i0 < a.B; i0 += 32) {
-    const long long mine = i0 + lane < a.B ? load_of(a, i0 + lane).work : 0;
-    long long upto = mine;
+    const int mine = i0 + lane < a.B ? load_of(a, i0 + lane).work : 0;
+    int upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+      const int v = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += v;
     }
     const uint32_t past = __ballot_sync(0xffffffffu, before + upto > w);
@@ -118,28 +141,24 @@ __device__ __forceinline__ int sequence_of(const Args& a, long long w, long long
   }
   return a.B;
 }
-// CTA c of n has units [c total / n, (c + 1) total / n).
-__device__ __forceinline__ long long share_begin(long long c, long long n, long long total) { return c * total / n; }
-__device__ __forceinline__ long long share_of(long long w, long long n, long long total) { return ((w + 1) * n - 1) / total; }
 
 // The stretches of a CTA's share, each within one item.  `begin` by warp 0, then a barrier; `next` by any thread that keeps a Walk.
 struct Stretch {
   Seq s; int b, hk, tile, n_rows;     // n_rows: query rows of the tile that exist
   int k_lo, k_hi;                     // slots
   bool whole;                         // all of the item: its result is final
-  long long slot;                     // where it goes otherwise
+  int slot;                           // where it goes otherwise
 };
 struct Walk {
-  long long at, stop;                 // units, relative to the first of sequence b
+  int at, stop;                       // units, relative to the first of sequence b
   int b; bool first;
 };
 __device__ __forceinline__ void begin_walk(const Args& a, Walk* w) {
-  long long before, total, none;
-  work_before(a, 0, none, total);
-  const long long shares = min((long long)a.shares, total);
+  int before;
+  const Cut c = work_before(a, 0, before);
   if ((threadIdx.x & 31) == 0) { w->at = w->stop = 0; w->b = 0; w->first = true; }
-  if (blockIdx.x < shares) {
-    const long long w0 = share_begin(blockIdx.x, shares, total), w1 = share_begin(blockIdx.x + 1, shares, total);
+  if ((int)blockIdx.x < min(c.shares, c.total)) {
+    const int w0 = share_begin(c, blockIdx.x), w1 = share_begin(c, blockIdx.x + 1);
     const int b = sequence_of(a, w0, before);
     if ((threadIdx.x & 31) == 0) { w->at = w0 - before; w->stop = w1 - before; w->b = b; }
   }
@@ -152,8 +171,7 @@ __device__ __forceinline__ bool next(const Args& a, Walk& w, Stretch& x) {
     w.stop -= load.work;
     load = load_of(a, ++w.b);
   }
-  const int item = (int)(w.at / load.units);              // the items of a sequence are fewer than 2^31
-  const int u0 = (int)(w.at - (long long)item * load.units), u1 = (int)min((long long)load.units, u0 + w.stop - w.at);
+  const int item = w.at / load.units, u0 = w.at - item * load.units, u1 = min(load.units, u0 + w.stop - w.at);
   x.s = load.s;
   x.b = w.b;
   x.hk = item / load.tiles;
@@ -162,7 +180,7 @@ __device__ __forceinline__ bool next(const Args& a, Walk& w, Stretch& x) {
   x.k_lo = min(load.s.lo + u0 * a.unit, load.s.hi);
   x.k_hi = min(load.s.lo + u1 * a.unit, load.s.hi);
   x.whole = u1 - u0 == load.units;
-  x.slot = 2 * (long long)blockIdx.x + (w.first ? 0 : 1);
+  x.slot = 2 * blockIdx.x + (w.first ? 0 : 1);
   w.at += u1 - u0;
   w.first = false;
   return true;
@@ -170,17 +188,17 @@ __device__ __forceinline__ bool next(const Args& a, Walk& w, Stretch& x) {
 
 // The shares that an item was cut into, by warp 0: c[0] .. c[1], and whether it is not the first stretch of the first of them
 // (equal shares: not cut, or there is no such item).
-__device__ __forceinline__ void shares_of_item(const Args& a, int b, int hk, int tile, long long (&c)[3]) {
+__device__ __forceinline__ void shares_of_item(const Args& a, int b, int hk, int tile, int (&c)[3]) {
   const Load load = load_of(a, b);
-  long long before, total;
-  work_before(a, b, before, total);
+  int before;
+  const Cut cut = work_before(a, b, before);
   if ((threadIdx.x & 31) == 0) {
     c[0] = c[1] = c[2] = 0;
     if (tile < load.tiles) {
-      const long long shares = min((long long)a.shares, total), w = before + ((long long)hk * load.tiles + tile) * load.units;
-      c[0] = share_of(w, shares, total);
-      c[1] = share_of(w + load.units - 1, shares, total);
-      c[2] = share_begin(c[0], shares, total) >= w ? 0 : 1;
+      const int w = before + (hk * load.tiles + tile) * load.units;
+      c[0] = share_of(cut, w);
+      c[1] = share_of(cut, w + load.units - 1);
+      c[2] = share_begin(cut, c[0]) >= w ? 0 : 1;
     }
   }
 }

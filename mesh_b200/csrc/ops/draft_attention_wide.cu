@@ -652,12 +652,12 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
         } else if (real) {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            a.part[(x.slot * (HD / 4) + c * 4 + i) * TT + row] =
+            a.part[((long long)x.slot * (HD / 4) + c * 4 + i) * TT + row] =
                 make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
         }
         __syncwarp();
       }
-      if (!x.whole && real && quarter == 0) a.part_ml[x.slot * TT + row] = make_float2(m, l);
+      if (!x.whole && real && quarter == 0) a.part_ml[(long long)x.slot * TT + row] = make_float2(m, l);
       __syncwarp();
     }
   }
@@ -669,30 +669,31 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
   }
 }
 
-// Joins the shares of the items that were cut: a CTA per item and 8 columns, four groups of threads that take the shares in
-// turn, a thread per row.
+// Joins the shares of the items that were cut, a thread per row and 8 columns.  SPLIT: a CTA per item and 8 columns, four groups of threads
+// that take the shares in turn (few items in many shares); else one per item and 32 columns, a group for 8 of them.
 constexpr int GROUPS = 4;
-template <int HD>
+template <int HD, bool SPLIT>
 __global__ void __launch_bounds__(GROUPS * TT) wide_join_kernel(const __grid_constant__ Args a) {
-  __shared__ long long c_s[3];
+  constexpr int EACH = SPLIT ? GROUPS : 1;                // groups among which an item's shares are dealt
+  __shared__ int c_s[3];
   __shared__ float2 ml_s[GROUPS][TT];
   __shared__ float4 o_s[GROUPS][2][TT];
   const int warp = threadIdx.x >> 5, row = threadIdx.x % TT, group = threadIdx.x / TT, G = a.q_heads / a.kv_heads;
-  const int i = blockIdx.y * 2, tile = blockIdx.x % a.tiles, hk = blockIdx.x / a.tiles % a.kv_heads, b = blockIdx.x / a.tiles / a.kv_heads;
+  const int tile = blockIdx.x % a.tiles, hk = blockIdx.x / a.tiles % a.kv_heads, b = blockIdx.x / a.tiles / a.kv_heads;
+  const int i = SPLIT ? blockIdx.y * 2 : blockIdx.y * 8 + group * 2;       // group of 4 columns
   // All wait: what comes after this kernel relies on the one before it.  And none looks at the lengths before: they are older than
   // that kernel, but only the wait keeps a read from finding what its line held before them.
   griddep_wait();
   if (warp == 0) shares_of_item(a, b, hk, tile, c_s);
   __syncthreads();
-  const long long c0 = c_s[0], c1 = c_s[1];
-  const int odd = (int)c_s[2];
-  const int n_rows = min(sequence(a, b).count * G - tile * TT, TT);
+  const int c0 = c_s[0], c1 = c_s[1], odd = c_s[2];
   if (c0 == c1) return;                                   // whole in one CTA, or not there
+  const int n_rows = min(sequence(a, b).count * G - tile * TT, TT);
   float m = -CUDART_INF_F, l = 0.f;
   float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   if (row < n_rows) {
 #pragma unroll 4
-    for (long long c = c0 + group; c <= c1; c += GROUPS) {
+    for (int c = c0 + (SPLIT ? group : 0); c <= c1; c += EACH) {
       const long long slot = 2 * c + (c == c0 ? odd : 0);
       const float2 x = __ldcg(a.part_ml + slot * TT + row);
       const float4 u = __ldcg(a.part + (slot * (HD / 4) + i) * TT + row), v = __ldcg(a.part + (slot * (HD / 4) + i + 1) * TT + row);
@@ -707,25 +708,27 @@ __global__ void __launch_bounds__(GROUPS * TT) wide_join_kernel(const __grid_con
   o_s[group][0][row] = make_float4(acc[0], acc[1], acc[2], acc[3]);
   o_s[group][1][row] = make_float4(acc[4], acc[5], acc[6], acc[7]);
   __syncthreads();
-  // a thread per row and pair of columns
-  const int out_row = threadIdx.x / 4, pair = threadIdx.x % 4;
-  if (out_row >= n_rows) return;
-  float mm = -CUDART_INF_F, ll = 0.f, s0 = 0.f, s1 = 0.f;
+  // pairs of columns, those of a row by neighbouring threads
+  constexpr int PAIRS = SPLIT ? 4 : 16;
+  for (int e = threadIdx.x; e < TT * PAIRS; e += GROUPS * TT) {
+    const int out_row = e / PAIRS, pair = e % 4, g0 = SPLIT ? 0 : e % PAIRS / 4, r = tile * TT + out_row;
+    if (out_row >= n_rows) continue;
+    float mm = -CUDART_INF_F, ll = 0.f, s0 = 0.f, s1 = 0.f;
 #pragma unroll
-  for (int g = 0; g < GROUPS; ++g) mm = fmaxf(mm, ml_s[g][out_row].x);
-  const float ref = mm == -CUDART_INF_F ? 0.f : mm;
+    for (int g = 0; g < EACH; ++g) mm = fmaxf(mm, ml_s[g0 + g][out_row].x);
+    const float ref = mm == -CUDART_INF_F ? 0.f : mm;
 #pragma unroll
-  for (int g = 0; g < GROUPS; ++g) {
-    const float wt = ex2(ml_s[g][out_row].x - ref);
-    const float2 v = reinterpret_cast<const float2*>(&o_s[g][pair >> 1][out_row])[pair & 1];
-    ll += wt * ml_s[g][out_row].y;
-    s0 += wt * v.x;
-    s1 += wt * v.y;
+    for (int g = 0; g < EACH; ++g) {
+      const float wt = ex2(ml_s[g0 + g][out_row].x - ref);
+      const float2 v = reinterpret_cast<const float2*>(&o_s[g0 + g][pair >> 1][out_row])[pair & 1];
+      ll += wt * ml_s[g0 + g][out_row].y;
+      s0 += wt * v.x;
+      s1 += wt * v.y;
+    }
+    const float inv = ll == 0.f ? 0.f : 1.f / ll;
+    *reinterpret_cast<uint32_t*>(a.out + b * a.o_sb + (r / G) * a.o_st + (long long)(hk * G + r % G) * HD + blockIdx.y * (SPLIT ? 8 : 32) + (g0 * 4 + pair) * 2) =
+        pack16(false, s0 * inv, s1 * inv);
   }
-  const float inv = ll == 0.f ? 0.f : 1.f / ll;
-  const int r = tile * TT + out_row;
-  *reinterpret_cast<uint32_t*>(a.out + b * a.o_sb + (r / G) * a.o_st + (long long)(hk * G + r % G) * HD + blockIdx.y * 8 + pair * 2) =
-      pack16(false, s0 * inv, s1 * inv);
 }
 
 template <int HD, bool Q8>
@@ -740,7 +743,11 @@ int run(const Args& p, void* stream) {
     configured.fetch_or(1ull << (dev & 63));
   }
   MESH_CUDA_OK(launch(wide_kernel<HD, Q8>, dim3(p.shares), THREADS, C::SMEM, stream, p));
-  if (p.part) MESH_CUDA_OK(launch(wide_join_kernel<HD>, dim3((unsigned)(p.B * p.kv_heads * p.tiles), HD / 8), GROUPS * TT, 0, stream, p));
+  if (p.part) {
+    const unsigned items = (unsigned)(p.B * p.kv_heads * p.tiles);
+    if (p.shares > 8ll * items) MESH_CUDA_OK(launch(wide_join_kernel<HD, true>, dim3(items, HD / 8), GROUPS * TT, 0, stream, p));
+    else MESH_CUDA_OK(launch(wide_join_kernel<HD, false>, dim3(items, HD / 32), GROUPS * TT, 0, stream, p));
+  }
   return 0;
 }
 
