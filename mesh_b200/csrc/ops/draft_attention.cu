@@ -3,18 +3,25 @@
 // The T drafts of a sequence and the G query heads that share a KV head are T * G query rows over the same keys: rows
 // t * G + g.  An item is 16 of them (one tile of the matrix instruction) with all keys that any of them sees.  The items' keys, in
 // units of 16 a warp, are laid end to end and cut into one share per CTA, all alike: lengths differ from sequence to sequence,
-// and whole items (or equal slices of each) left most SMs waiting for the longest (282 us of a case that now takes MEASURED).  Only
+// and whole items (or equal slices of each) left most SMs waiting for the longest (282 us of a case that now takes 143).  Only
 // the device knows the lengths, so every CTA finds its share itself.  A CTA's warps take blocks of 16 keys in turn, each
 // with a ring of its own that cp.async fills, so that nothing but the end of an item joins them.  Items that were cut are
 // joined by a second kernel.
 //
 // Formulas.  A score is s = scale q.k; with 8-bit rows k = ks kc and v = vs vc, where kc, vc are the codes: s = (scale ks) (q.kc),
-// and the weight of a value's codes is w = exp(s - m) vs.  The running reference m of a row is the maximum of s + log vs, so
-// w <= 1 whatever the scales; the sum of exp(s - m) is kept beside it in fp32.  Codes go through the products as fp16, which
-// holds them exactly; so do the queries, after a row is multiplied by the power of two that brings its largest value to
-// 2^8..2^9 (what is smaller than 2^-32 of that is lost, less than the products' own rounding in fp32).  w is multiplied
-// by 2^14 first (in m), so that fp16 holds it down to 2^-38; its rounding to 11 bits is an eighth of bf16's.  With a bf16 cache
-// queries and values are bf16 as they are and w is rounded to bf16, half a step of the result's own type.
+// and the weight of a value's codes is w = exp(s - m) vs; the sum of exp(s - m) is kept beside it in fp32.  The reference m of a
+// row follows the maximum of s + log vs, whatever the scales are, and is moved, and the output with it, only when that has
+// grown by more than 2^8: with every new maximum most blocks of 16 rows rescaled their output (59 us now, 68 then, 4 drafts).
+// Codes go through the products as fp16, which holds them exactly; so do the queries, after a row is multiplied by the power of two
+// that brings its largest value to 2^8..2^9 (what is smaller than 2^-32 of that is lost, less than the products' own rounding
+// in fp32).  w is multiplied by 2^6 first (in m), so it stays below 2^14 and fp16 holds it in full down to 2^-20, in part down to
+// 2^-30, of the largest; its rounding to 11 bits is an eighth of bf16's.  With a bf16 cache queries and values are bf16 as they are
+// and w is rounded to bf16, half a step of the result's own type.
+//
+// Measured: 16 sequences of 4000 to 32767 keys, 8 KV heads of 128 in 8 bits, 4 query heads each, one token: 142 us, 4.4 TB/s of keys
+// and values.  What bounds it is the issue of instructions (2.4 a clock and SM): a code has to be widened for either product, and
+// the tile's 16 rows hold 4 queries.  32 keys a block took the same time, with a few registers spilled.  With bf16 rows (8 x 12000
+// keys) 72 us, 5.6 TB/s: memory.
 #include "draft_attention.cuh"
 
 namespace mesh {
@@ -49,7 +56,7 @@ struct Cfg {
   static constexpr int RB = Q8 ? HD : 2 * HD, NC = RB / 16;           // bytes and 16-byte chunks of a row
   static constexpr int STAGE = 2 * KEYS * RB + (Q8 ? 2 * KEYS * 4 : 0);
   // As many warps as their registers allow (half of a warp's are the output's), four where a block is 16 KB.  Heads of 128 in 8 bits:
-  // 151 us with 12 warps, 162 with 8; two warps to a block with half of the columns each, 16 in all, 185.
+  // With 12 warps 151 us, with 8 162; two warps to a block with half of the columns each, 16 in all, 185.
   static constexpr int WARPS = STAGE > 9000 ? 4 : HD == 256 ? 8 : HD == 128 ? 12 : 16;
   static constexpr int ROOM = 200 * 1024 / WARPS, STAGES = ROOM / STAGE > 8 ? 8 : ROOM / STAGE;
   static constexpr int RING = WARPS * STAGES * STAGE;
@@ -194,7 +201,7 @@ __global__ void __launch_bounds__(Cfg<HD, Q8>::WARPS * 32, 1) attention_kernel(c
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const int t = min((tile * ROWS + n + 8 * j) / G, a.T - 1);
-    vis[j] = a.visible ? (unsigned long long)__ldg(a.visible + (long long)b * a.T + t) : t >= 63 ? ~0ull : (2ull << t) - 1;
+    vis[j] = a.visible ? (unsigned long long)__ldcg(a.visible + (long long)b * a.T + t) : t >= 63 ? ~0ull : (2ull << t) - 1;
     row_lo[j] = a.window > 0 ? max(0, s.pos + max(__popcll(vis[j]), 1) - a.window) : 0;
   }
   const int free_lo = a.window > 0 ? max(0, s.pos + 64 - a.window) : 0;      // from here to pos every row sees every key
@@ -205,7 +212,7 @@ __global__ void __launch_bounds__(Cfg<HD, Q8>::WARPS * 32, 1) attention_kernel(c
   for (int i = 0; i < NT; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
-  constexpr float LIFT = Q8 ? 14.f : 0.f;
+  constexpr float LIFT = Q8 ? 6.f : 0.f, LAG = 8.f;
 
   for (int block = 0; block * C::WARPS + warp < blocks; ++block) {
     cp_async_wait<STAGES - 2>();
@@ -268,16 +275,17 @@ __global__ void __launch_bounds__(Cfg<HD, Q8>::WARPS * 32, 1) attention_kernel(c
           top[j] = fmaxf(top[j], v + up);
         }
       }
-    float alpha[2];
+    // The reference moves only when some score has grown by more than 2^LAG (also at the first key that is seen)
+    if (__any_sync(0xffffffffu, top[0] - LIFT > m[0] + LAG || top[1] - LIFT > m[1] + LAG)) {
+      float alpha[2];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], 1));
-      top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], 2));
-      const float now = fmaxf(m[j], top[j] - LIFT);
-      alpha[j] = m[j] == now ? 1.f : ex2(m[j] - now);     // nothing seen before: 0
-      m[j] = now;
-    }
-    if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+      for (int j = 0; j < 2; ++j) {
+        top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], 1));
+        top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], 2));
+        const float now = top[j] - LIFT > m[j] + LAG ? top[j] - LIFT : m[j];
+        alpha[j] = m[j] == now ? 1.f : ex2(m[j] - now);   // nothing seen before: 0
+        m[j] = now;
+      }
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
         o[i][0] *= alpha[0]; o[i][1] *= alpha[0];
@@ -524,8 +532,15 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args 
   }
 }
 
-// The kernel for many rows, with tiles of 128, from 17 query rows per KV head on.
-static bool wide(const MeshKvCache* c, const MeshDraftAttention* a) { return a->T * (a->q_heads / c->kv_heads) > ROWS; }
+// Units that a share may be longer for the sake of whole pieces: of 128 to 256 keys, and of 64 of the other kernel.  KV heads of 128 in 8
+// bits, 4 heads a group, 8 sequences: single tokens over 12000 keys 57.7 us cut equally, 60.4 in pieces 5 longer; 64 drafts over 4000
+// keys 99.2 us and, in pieces 9 longer, 92.6.
+constexpr int FEW = 4, WIDE_FEW = 12;
+
+// The kernel for many rows, with tiles of 128, from three tiles of 16 on: it has a longer start and end, and this one fetches the
+// keys once per tile.  Eight sequences, 8 KV heads of 128 in 8 bits, 4 heads a group, this kernel and the other one: 8 drafts over
+// 500 keys 14 and 21 us, over 12000 keys 100 and 119 us (bf16: 112 and 102); 12 drafts 25 and 22, 142 and 120 us.
+static bool wide(const MeshKvCache* c, const MeshDraftAttention* a) { return a->T * (a->q_heads / c->kv_heads) > 2 * ROWS; }
 
 static void cut(const MeshKvCache* c, const MeshDraftAttention* a, Args& p) {
   const bool w = wide(c, a), q8 = c->bits == 8;
@@ -540,7 +555,7 @@ static void cut(const MeshKvCache* c, const MeshDraftAttention* a, Args& p) {
   const long long units = (long long)c->B * c->kv_heads * p.tiles * ((keys + p.unit - 1) / p.unit);
   const long long most = a->splits > 0 ? a->splits : sm_count();
   p.shares = (int)(units < most ? units : most);
-  p.few = a->splits > 0 ? 0 : w ? 32 : 16;
+  p.few = a->splits > 0 ? 0 : w ? WIDE_FEW : FEW;
 }
 
 static int check(const MeshKvCache* c, const MeshDraftAttention* a) {

@@ -19,11 +19,11 @@ constexpr int THREADS = 256;
 // 8 consecutive bf16.  ALIGNED: the address is a multiple of 16 bytes.
 template <bool ALIGNED>
 __device__ __forceinline__ uint4 load8(const __nv_bfloat16* p) {
-  if (ALIGNED) return __ldg(reinterpret_cast<const uint4*>(p));
+  if (ALIGNED) return __ldcg(reinterpret_cast<const uint4*>(p));
   uint4 r;
   unsigned short* h = reinterpret_cast<unsigned short*>(&r);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) h[i] = __ldg(reinterpret_cast<const unsigned short*>(p) + i);
+  for (int i = 0; i < 8; ++i) h[i] = __ldcg(reinterpret_cast<const unsigned short*>(p) + i);
   return r;
 }
 
@@ -85,8 +85,8 @@ __global__ void __launch_bounds__(THREADS) append_kernel(MeshKvCache c, const __
   bool there = b < c.B;
   long long slot = 0;
   if (there) {
-    slot = (long long)__ldg(pos + b) + t;
-    there = t < (counts ? __ldg(counts + b) : T) && slot >= 0 && slot < c.max_seq;
+    slot = (long long)__ldcg(pos + b) + t;
+    there = t < (counts ? __ldcg(counts + b) : T) && slot >= 0 && slot < c.max_seq;
   }
   uint4 kx = make_uint4(0, 0, 0, 0), vx = kx;
   if (there) {
@@ -141,18 +141,18 @@ __global__ void __launch_bounds__(THREADS) read_kernel(MeshKvCache c, uint4* __r
   const int t = (int)(bt % T);
   const long long b = bt / T;
   if (b >= c.B) return;
-  const long long slot = (long long)__ldg(start + b) + t;
+  const long long slot = (long long)__ldcg(start + b) + t;
   uint4 kx = make_uint4(0, 0, 0, 0), vx = kx;
-  if (t < (counts ? __ldg(counts + b) : T) && slot >= 0 && slot < c.max_seq) {
+  if (t < (counts ? __ldcg(counts + b) : T) && slot >= 0 && slot < c.max_seq) {
     const long long at = (b * c.kv_heads + h) * c.max_seq + slot;
     if (Q8) {
-      const uint2 kc = __ldg(reinterpret_cast<const uint2*>(c.k) + at * LANES + lane);
-      const uint2 vc = __ldg(reinterpret_cast<const uint2*>(c.v) + at * LANES + lane);
-      kx = decode8(kc, __ldg(c.k_scale + at));
-      vx = decode8(vc, __ldg(c.v_scale + at));
+      const uint2 kc = __ldcg(reinterpret_cast<const uint2*>(c.k) + at * LANES + lane);
+      const uint2 vc = __ldcg(reinterpret_cast<const uint2*>(c.v) + at * LANES + lane);
+      kx = decode8(kc, __ldcg(c.k_scale + at));
+      vx = decode8(vc, __ldcg(c.v_scale + at));
     } else {
-      kx = __ldg(reinterpret_cast<const uint4*>(c.k) + at * LANES + lane);
-      vx = __ldg(reinterpret_cast<const uint4*>(c.v) + at * LANES + lane);
+      kx = __ldcg(reinterpret_cast<const uint4*>(c.k) + at * LANES + lane);
+      vx = __ldcg(reinterpret_cast<const uint4*>(c.v) + at * LANES + lane);
     }
   }
   k_out[row * LANES + lane] = kx;
@@ -175,8 +175,8 @@ __global__ void __launch_bounds__(THREADS) keep_kernel(const __grid_constant__ K
   griddep_launch_dependents();
   griddep_wait();
   const int h = blockIdx.x % kv_heads, b = blockIdx.x / kv_heads, which = blockIdx.y & 1, layer = blockIdx.y >> 1;
-  const long long p = __ldg(pos + b);
-  const int n = min(N, counts ? __ldg(counts + b) : N);
+  const long long p = __ldcg(pos + b);
+  const int n = min(N, counts ? __ldcg(counts + b) : N);
   const long long base = ((long long)b * kv_heads + h) * max_seq;
   uint4* data = reinterpret_cast<uint4*>(a.data[layer][which]) + base * LANES;
   uint4 r[PER];
@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(THREADS) keep_kernel(const __grid_constant__ K
     const int j = i * THREADS + threadIdx.x, e = j / LANES;
     to[i] = -1;
     if (e >= n) continue;
-    const int from = __ldg(path + (long long)b * N + e);
+    const int from = __ldcg(path + (long long)b * N + e);
     const long long src = p + from, dst = p + e;
     if (from < 0 || from == e || p < 0 || src >= max_seq || dst >= max_seq) continue;
     r[i] = data[src * LANES + j % LANES];
@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(THREADS) keep_kernel(const __grid_constant__ K
   float s = 0.f;
   long long s_to = -1;
   if (scale && (int)threadIdx.x < n) {
-    const int from = __ldg(path + (long long)b * N + threadIdx.x);
+    const int from = __ldcg(path + (long long)b * N + threadIdx.x);
     const long long src = p + from, dst = p + threadIdx.x;
     if (from >= 0 && p >= 0 && src < max_seq && dst < max_seq) {
       s = scale[base + src];
