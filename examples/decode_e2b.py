@@ -22,12 +22,13 @@ def main(argv=None):
     ap.add_argument("--prompt", type=int, default=128)
     ap.add_argument("--tokens", type=int, default=64)
     ap.add_argument("--layers", type=int, default=30)
+    ap.add_argument("--cache-bits", type=int, default=16, choices=[8, 16])
     a = ap.parse_args(argv)
     from mesh_b200.distributed import init, shutdown
     from mesh_b200.models.e2b import E2BConfig, E2BDecoder
     ctx = init(backend="nccl")
     cfg = E2BConfig(layers=a.layers)
-    m = E2BDecoder(cfg, ctx, a.batch, a.weights)
+    m = E2BDecoder(cfg, ctx, a.batch, a.weights, cache_bits=a.cache_bits)
     g = torch.Generator().manual_seed(11)
     prompt = torch.randint(0, cfg.vocab, (a.batch, a.prompt), generator=g, dtype=torch.int32).to(ctx.device)
     m.prefill(prompt)

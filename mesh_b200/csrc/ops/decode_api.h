@@ -20,7 +20,7 @@ typedef struct MeshDecodeLinear {
   void* out; long long ldo; int out_f32;
   int q_heads, kv_heads, head_dim;
   const int* pos; const float* cos_t; const float* sin_t;
-  void* q_out; void* k_cache; void* v_cache; int max_seq;
+  void* q_out; void* k_cache; void* v_cache; int max_seq;   // max_seq 0: this token's rows alone, [B, kv_heads, head_dim]
   int rank, world;
   void* ar_recv[MESH_DEC_MAX_RANKS];
   const uint32_t* step_ptr; uint32_t calls_per_step, call_index;   // all-reduce sequence = *step_ptr * calls + index + 1

@@ -47,7 +47,7 @@ struct LinArgs {
   const int* pos; const float* cos_t; const float* sin_t;
   __nv_bfloat16* q_out;                               // [B, q_heads * head_dim]
   __nv_bfloat16* k_cache; __nv_bfloat16* v_cache;     // [B, kv_heads, max_seq, head_dim]
-  int max_seq;
+  int max_seq;                                        // 0: the rows of this token alone, [B, kv_heads, head_dim]
   // all-reduce + residual
   int rank, world;
   uint2* ar_recv[MESH_DEC_MAX_RANKS];                 // ar_recv[d]: rank d's slots [world][N * 8]
@@ -385,13 +385,14 @@ __device__ __forceinline__ void finish_group(const LinArgs& a, int grp, const fl
             o_lo = lo * cs - hi * sn;
             o_hi = hi * cs + lo * sn;
           }
+          const long long slots = a.max_seq ? a.max_seq : 1, slot = a.max_seq ? p : 0;
           __nv_bfloat16* dst;
           if (h < a.q_heads) {
             dst = a.q_out + (long long)n * a.q_heads * hd + h * hd;
           } else if (h < a.q_heads + a.kv_heads) {
-            dst = a.k_cache + (((long long)n * a.kv_heads + (h - a.q_heads)) * a.max_seq + p) * hd;
+            dst = a.k_cache + (((long long)n * a.kv_heads + (h - a.q_heads)) * slots + slot) * hd;
           } else {
-            dst = a.v_cache + (((long long)n * a.kv_heads + (h - a.q_heads - a.kv_heads)) * a.max_seq + p) * hd;
+            dst = a.v_cache + (((long long)n * a.kv_heads + (h - a.q_heads - a.kv_heads)) * slots + slot) * hd;
           }
           dst[i] = __float2bfloat16_rn(o_lo);
           dst[i + half] = __float2bfloat16_rn(o_hi);

@@ -11,6 +11,10 @@ cheap compute is free"), vocabulary-parallel LM head with a MAXLOC exchange of 8
 A decode step is 5 kernels per layer — [norm+QKV+RoPE+cache], [attention], [o-proj+all-reduce+residual],
 [norm+gate/up+GeGLU], [down+all-reduce+residual] — plus LM head and argmax, captured once in a CUDA graph and
 replayed: no host round trip between tokens (design/e2b-crossover-2026-09-16.md:73-84).
+
+With ``cache_bits=8`` the key/value cache is kept in 8-bit codes (``ops/cache.py``): half of the bytes that a long context costs, and room
+for twice the tokens.  ``draft_step`` runs a tree of drafted tokens through the model at once and ``accept`` keeps the branch
+that the model itself would have taken.
 """
 from __future__ import annotations
 
@@ -20,7 +24,10 @@ import time
 import torch
 
 from ..ops import decode as D
+from ..ops.cache import CacheGroup, KVCache
+from ..ops.draft import draft_attention, tree_depth
 from ..ops.gemm import gemm, glu_fwd
+from ..ops.logits import constrain_logits
 from ..ops.norm import rmsnorm_fwd
 from ..ops.rope import rope_, rope_tables
 
@@ -53,7 +60,10 @@ def _rand(shape, std, seed, device):
 class E2BDecoder:
     """Holds this rank's weight shards, KV caches and workspaces; ``prefill`` then ``decode``."""
 
-    def __init__(self, cfg: E2BConfig, ctx, batch: int, quant: str = "bf16", seed: int = 0):
+    def __init__(self, cfg: E2BConfig, ctx, batch: int, quant: str = "bf16", seed: int = 0, cache_bits: int = 16):
+        if cache_bits not in (8, 16):
+            raise ValueError(f"cache_bits must be 8 or 16, got {cache_bits}")
+        self.cache_bits = cache_bits
         self.cfg, self.ctx, self.B, self.quant = cfg, ctx, batch, quant
         self.rank, self.world, dev = ctx.rank, ctx.world, ctx.device
         self.dev = dev
@@ -93,8 +103,11 @@ class E2BDecoder:
                     codes, scales = quantize(L[k])
                     L[k + "_q"], L[k + "_s"] = codes, scales
                     L[k] = dequantize(codes, scales)          # prefill GEMMs use the dequantised values (same numbers)
-            L["kc"] = torch.zeros((batch, self.kvh, c.max_seq, hd), dtype=torch.bfloat16, device=dev)
-            L["vc"] = torch.zeros_like(L["kc"])
+            if cache_bits == 8:
+                L["cache"] = KVCache.empty(batch, self.kvh, c.max_seq, hd, device=dev)
+            else:
+                L["kc"] = torch.zeros((batch, self.kvh, c.max_seq, hd), dtype=torch.bfloat16, device=dev)
+                L["vc"] = torch.zeros_like(L["kc"])
             self.layers.append(L)
         # tied embedding: every rank keeps the whole table for lookups; its LM-head shard is a row view
         chunks = []
@@ -117,7 +130,11 @@ class E2BDecoder:
         self.att_out = torch.zeros((B, self.qh * hd), dtype=torch.bfloat16, device=dev)
         self.h = torch.zeros((B, self.Fl), dtype=torch.bfloat16, device=dev)
         self.logits = torch.zeros((B, self.Vl), dtype=torch.float32, device=dev)
-        self.att = D.DecodeAttention(B, self.qh, self.kvh, hd, splits=16, device=dev)
+        if cache_bits == 8:
+            self.kv_rows = torch.zeros((2, B, self.kvh, hd), dtype=torch.bfloat16, device=dev)     # a token's, before they are coded
+        else:
+            self.att = D.DecodeAttention(B, self.qh, self.kvh, hd, splits=16, device=dev)
+        self._group = None
         self.out_tokens = torch.zeros((c.max_seq, B), dtype=torch.int32, device=dev)
         self.calls_per_step = 2 * c.layers
         if P > 1:
@@ -162,10 +179,18 @@ class E2BDecoder:
             return self._w(self.layers[l], name)[0]
         for l, L in enumerate(self.layers):
             w, s = self._w(L, "wqkv")
+            coded = self.cache_bits == 8
+            kc, vc, slots = (*self.kv_rows, 0) if coded else (L["kc"], L["vc"], c.max_seq)
             D.decode_linear(x, w, scales=s, norm_w=L["n1"], eps=c.eps, mode=D.QKV, next_weights=nxt(l, "wo"),
                             qkv=dict(q_heads=self.qh, kv_heads=self.kvh, head_dim=c.head_dim, pos=self.pos, cos=self.cos,
-                                     sin=self.sin, q_out=self.q, k_cache=L["kc"], v_cache=L["vc"], max_seq=c.max_seq))
-            self.att(self.q, L["kc"], L["vc"], self.pos, self.att_out, window=c.window if c.is_local(l) else 0)
+                                     sin=self.sin, q_out=self.q, k_cache=kc, v_cache=vc, max_seq=slots))
+            window = c.window if c.is_local(l) else 0
+            if coded:
+                heads = (self.B, 1, self.qh, c.head_dim)
+                L["cache"].append(kc[:, None], vc[:, None], self.pos)
+                draft_attention(self.q.view(heads), L["cache"], self.pos, window=window, out=self.att_out.view(heads))
+            else:
+                self.att(self.q, kc, vc, self.pos, self.att_out, window=window)
             w, s = self._w(L, "wo")
             if self.world > 1:
                 D.decode_linear(self.att_out, w, scales=s, mode=D.ALLREDUCE, out=x1, residual=x, ar=self._ar(2 * l),
@@ -215,8 +240,11 @@ class E2BDecoder:
             rope_(qv, positions, self.cos, self.sin)
             rope_(kv, positions, self.cos, self.sin)
             vv = qkv[:, (self.qh + self.kvh) * hd:].view(B * T, self.kvh, hd)
-            L["kc"][:, :, :T].copy_(kv.view(B, T, self.kvh, hd).transpose(1, 2))
-            L["vc"][:, :, :T].copy_(vv.view(B, T, self.kvh, hd).transpose(1, 2))
+            if self.cache_bits == 8:
+                L["cache"].append(kv.view(B, T, self.kvh, hd), vv.view(B, T, self.kvh, hd), positions.view(B, T)[:, 0].contiguous())
+            else:
+                L["kc"][:, :, :T].copy_(kv.view(B, T, self.kvh, hd).transpose(1, 2))
+                L["vc"][:, :, :T].copy_(vv.view(B, T, self.kvh, hd).transpose(1, 2))
             # prefill attention straight from the fused qkv matrix (tcgen05 flash attention; no copies of q, k, v)
             flash_attention(qv.view(B, T, self.qh, hd), kv.view(B, T, self.kvh, hd), vv.view(B, T, self.kvh, hd), causal=True,
                             window=c.window if c.is_local(l) else 0, out=att_out.view(B, T, self.qh, hd))
@@ -239,6 +267,89 @@ class E2BDecoder:
         D.decode_argmax(self.logits, self.tok, self.pos, vocab_offset=self.rank * self.Vl, rank=self.rank, world=self.world,
                         xchg_ptrs=self.xchg.ptrs() if self.world > 1 else None, step=self.step)
         return self.tok.clone()
+
+    # ------------------------------------------------------------------ drafts
+    def caches(self) -> CacheGroup:
+        """The layers' caches as one group (``ops/cache.py``); heads of 64, 128 or 256."""
+        if self._group is None:
+            if self.cache_bits == 16:
+                for L in self.layers:
+                    L["cache"] = KVCache(L["kc"], L["vc"])
+            self._group = CacheGroup([L["cache"] for L in self.layers])
+        return self._group
+
+    def draft_step(self, drafts: torch.Tensor, visible: torch.Tensor | None = None, counts: torch.Tensor | None = None,
+                   constraints: dict | None = None) -> torch.Tensor:
+        """Run a tree of drafts of every sequence through the model at once: ``drafts`` int32 ``[B, T]``, T <= 64, whose first is the
+        sequence's last token (``self.tok``), with ``visible`` (``ops/draft.py::tree_visible``; ``None``: a chain) and ``counts``
+        (drafts of each sequence; ``None``: T) -> int32 ``[B, T]``, the token that the model chooses after each of them.  Their rows lie in
+        slots ``pos .. pos + T`` of the caches, which must be there, until ``accept`` or the next step; ``pos`` and ``tok`` stay.
+        ``constraints``: arguments of ``ops/logits.py::constrain_logits`` for the ``B * T`` rows of logits.
+
+        Up to 8 rows the logits are fp32 (as in ``decode``), beyond that they come from the bf16 product: equal ones are
+        likelier there, and the lowest id is taken.  One rank: each holds a part of the vocabulary, and the choice among the
+        ranks' best is made for a token per sequence only."""
+        c = self.cfg
+        if self.world > 1:
+            raise ValueError("draft_step: one rank only")
+        if drafts.dim() != 2 or drafts.shape[0] != self.B or not 1 <= drafts.shape[1] <= 64 or drafts.dtype != torch.int32 or drafts.device != self.pos.device:
+            raise ValueError(f"draft_step: drafts must be int32 [{self.B}, 1..64] on {self.pos.device}, got {drafts.dtype} {list(drafts.shape)} on {drafts.device}")
+        self.caches()
+        B, T = drafts.shape
+        hd, qh, kvh = c.head_dim, self.qh, self.kvh
+        depth = torch.arange(T, dtype=torch.int32, device=self.dev) if visible is None else tree_depth(visible)
+        positions = (self.pos[:, None] + depth).clamp_(max=c.max_seq - 1).reshape(-1).to(torch.int32)
+        x = self.emb[drafts.reshape(-1).long()]
+        att = torch.zeros((B, T, qh, hd), dtype=torch.bfloat16, device=self.dev)       # rows behind counts are not written
+        for l, L in enumerate(self.layers):
+            h, _, _ = rmsnorm_fwd(x, L["n1"], c.eps)
+            qkv = self._mm(h, L, "wqkv")
+            rope_(qkv[:, :(qh + kvh) * hd].view(B * T, qh + kvh, hd), positions, self.cos, self.sin)
+            heads = qkv.view(B, T, qh + 2 * kvh, hd)
+            L["cache"].append(heads[:, :, qh:qh + kvh], heads[:, :, qh + kvh:], self.pos, counts)
+            draft_attention(heads[:, :, :qh], L["cache"], self.pos, counts=counts, visible=visible, window=c.window if c.is_local(l) else 0, out=att)
+            x = x + self._mm(att.view(B * T, qh * hd), L, "wo")
+            h, _, _ = rmsnorm_fwd(x, L["n2"], c.eps)
+            a, _ = glu_fwd(h, L["wgu"], act="gelu_tanh", save_gu=False)
+            x = x + self._mm(a, L, "wd")
+        codes = dict(w=self.lm_q, scales=self.lm_s) if self.quant in ("w4", "w8") else dict(w=self.lm_head)
+        if B * T <= 8:
+            logits = D.decode_linear(x, **codes, norm_w=self.nf, eps=c.eps, out_f32=True)
+        else:
+            h, _, _ = rmsnorm_fwd(x, self.nf, c.eps)
+            if self.quant in ("w4", "w8"):
+                from ..ops.gemm import gemm_q
+                logits = gemm_q(h, self.lm_q, self.lm_s)
+            else:
+                logits = gemm(h, self.lm_head)
+        chosen = torch.empty(B * T, dtype=torch.int32, device=self.dev)
+        constrain_logits(logits, tokens=chosen, **(constraints or {}))
+        return chosen.view(B, T)
+
+    def accept(self, drafts: torch.Tensor, chosen: torch.Tensor, parents=None, counts: torch.Tensor | None = None) -> list[list[int]]:
+        """Keep the branch of the last ``draft_step`` that follows the model's own choices: from the root on, a child that is the
+        token chosen after its parent (the first of equal ones).  ``parents [B][T]`` as in ``tree_visible`` (``None``: a chain).  Its rows
+        move to the front in every layer, ``pos`` moves past them, ``tok`` becomes the token chosen at its end.  Returns
+        each sequence's new tokens: the accepted drafts and that one, at least one."""
+        B, T = drafts.shape
+        d, m = drafts.tolist(), chosen.tolist()
+        rows = parents.tolist() if isinstance(parents, torch.Tensor) else parents
+        most = counts.tolist() if counts is not None else [T] * B
+        paths, new = [], []
+        for b in range(B):
+            path = [0] if most[b] > 0 else []
+            for t in range(1, min(T, most[b])):
+                if (rows[b][t] if rows is not None else t - 1) == path[-1] and d[b][t] == m[b][path[-1]]:
+                    path.append(t)
+            new.append([d[b][t] for t in path[1:]] + [m[b][t] for t in path[-1:]])
+            paths.append(path)
+        n = max(map(len, paths))
+        ints = dict(dtype=torch.int32, device=self.dev)
+        kept = torch.tensor([len(p) for p in paths], **ints)
+        self.caches().keep(self.pos, torch.tensor([p + [-1] * (n - len(p)) for p in paths], **ints), kept)
+        self.pos += kept
+        self.tok.copy_(torch.tensor([t[-1] if t else old for t, old in zip(new, self.tok.tolist())], **ints))
+        return new
 
     # ------------------------------------------------------------------ decode
     def weight_bytes(self) -> int:
@@ -266,6 +377,8 @@ class E2BDecoder:
         Default: ``MESH_DECODE_MODE``, else ``"graph"``."""
         import os
         mode = mode or os.environ.get("MESH_DECODE_MODE") or "graph"
+        if mode == "step" and self.cache_bits == 8:
+            raise ValueError("the step kernel reads caches of bf16 rows: with cache_bits=8 capture the step as a graph")
         if mode == "step" and not self.step_kernel_fits():
             raise ValueError("the step kernel takes groups of at most 4 query heads per KV head")
         if mode not in ("step", "graph"):
@@ -311,7 +424,7 @@ class E2BDecoder:
 
 
 def bench_decode(ctx, steps: int = 256, prompt_len: int = 512, configs=(("bf16", 1), ("bf16", 8), ("w4", 1), ("w4", 8), ("w8", 1), ("w8", 8)),
-                 cfg: E2BConfig | None = None, mode: str | None = None) -> dict:
+                 cfg: E2BConfig | None = None, mode: str | None = None, cache_bits: int = 16) -> dict:
     """Decode tokens/s (whole job: batch * steps / time), device-timed, max over ranks.  ``mode``: how the step is
     replayed (``E2BDecoder.capture``)."""
     import torch.distributed as dist
@@ -326,7 +439,7 @@ def bench_decode(ctx, steps: int = 256, prompt_len: int = 512, configs=(("bf16",
     for quant, B in configs:
         mark = ctx.heap.mark() if ctx.world > 1 else None
         try:
-            m = E2BDecoder(cfg, ctx, B, quant)
+            m = E2BDecoder(cfg, ctx, B, quant, cache_bits=cache_bits)
         except Exception as e:      # a configuration that cannot be built is reported, the others still run
             res["runs"].append({"weights": quant, "batch": B, "error": f"{type(e).__name__}: {e}"[:200]})
             if mark is not None:
