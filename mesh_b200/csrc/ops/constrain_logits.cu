@@ -83,7 +83,7 @@ __device__ __forceinline__ float adjust(float x, uint32_t word, const Row& r) {
   const uint32_t n = word & COUNT;
   if (r.repeats && (n || (word & SEEN))) x = x > 0.f ? __fdiv_rn(x, r.repetition) : __fmul_rn(x, r.repetition);
   if (n) x = __fsub_rn(__fsub_rn(x, __fmul_rn(r.frequency, (float)n)), r.presence);
-  if (word >> BIAS_SHIFT) x = __fadd_rn(x, __ldcg(r.bias + (word >> BIAS_SHIFT) - 1));
+  if (word >> BIAS_SHIFT) x = __fadd_rn(x, r.bias[(word >> BIAS_SHIFT) - 1]);
   return x;
 }
 
@@ -94,11 +94,11 @@ __device__ __forceinline__ int number_of(const uint32_t* listed, const uint16_t*
 // f(i, place in the piece) for the entries of a list that lie in the piece, by threads thread of threads: several loads at a
 // time, a trip to L2 for all of them and not for each.
 template <class F>
-__device__ __forceinline__ void each(const int* __restrict__ list, int n, unsigned first, unsigned size, int thread, int threads, F f) {
+__device__ __forceinline__ void each(const int* list, int n, unsigned first, unsigned size, int thread, int threads, F f) {
   for (int i0 = thread; i0 < n; i0 += 4 * threads) {
     unsigned id[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) id[i] = i0 + i * threads < n ? (unsigned)__ldcg(list + i0 + i * threads) - first : ~0u;
+    for (int i = 0; i < 4; ++i) id[i] = i0 + i * threads < n ? (unsigned)list[i0 + i * threads] - first : ~0u;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (id[i] < size) f(i0 + i * threads, id[i]);
@@ -122,16 +122,16 @@ __global__ void __launch_bounds__(THREADS, 6) constrain_kernel(const __grid_cons
   griddep_wait();
   const int row = blockIdx.x / CTAS, part = blockIdx.x % CTAS;
   Row r;
-  r.hist = a.history ? (a.history_len ? min(max(__ldcg(a.history_len + row), 0), a.hist) : a.hist) : 0;
+  r.hist = a.history ? (a.history_len ? min(max(a.history_len[row], 0), a.hist) : a.hist) : 0;
   r.history = a.history + (long long)row * a.ldh;
-  r.prompt = a.prompt_len ? __ldcg(a.prompt_len + row) : 0;
-  r.nbias = a.bias_ids ? (a.bias_len ? min(max(__ldcg(a.bias_len + row), 0), a.nbias) : a.nbias) : 0;
+  r.prompt = a.prompt_len ? a.prompt_len[row] : 0;
+  r.nbias = a.bias_ids ? (a.bias_len ? min(max(a.bias_len[row], 0), a.nbias) : a.nbias) : 0;
   r.bias_ids = a.bias_ids + (long long)row * a.ldb;
   r.bias = a.bias + (long long)row * a.ldb;
   r.repeats = a.repetition != nullptr;
-  r.repetition = a.repetition ? __ldcg(a.repetition + row) : 1.f;
-  r.presence = a.presence ? __ldcg(a.presence + row) : 0.f;
-  r.frequency = a.frequency ? __ldcg(a.frequency + row) : 0.f;
+  r.repetition = a.repetition ? a.repetition[row] : 1.f;
+  r.presence = a.presence ? a.presence[row] : 0.f;
+  r.frequency = a.frequency ? a.frequency[row] : 0.f;
   const uint8_t* in = reinterpret_cast<const uint8_t*>(a.logits) + (long long)row * a.ldl * (HALF ? 2 : 4);
   uint8_t* out = reinterpret_cast<uint8_t*>(a.out) + (long long)row * a.ldo * (HALF ? 2 : 4);
   const uint32_t* allowed = a.allowed ? a.allowed + (long long)row * a.ldw : nullptr;
@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(THREADS, 6) constrain_kernel(const __grid_cons
 #pragma unroll
         for (int i = 0; i < AT_ONCE; ++i) {
           x[i] = src[i * STREAM];
-          ok[i] = allowed ? __ldcg(allow + i * (STEP / 32)) : ~0u;
+          ok[i] = allowed ? allow[i * (STEP / 32)] : ~0u;
         }
 #pragma unroll
         for (int i = 0; i < AT_ONCE; ++i) {
@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(THREADS, 6) constrain_kernel(const __grid_cons
       for (int at = whole + st; at < hi - lo; at += STREAM) {            // the rest, and rows at any address
         const int c = lo + at;
         float f = load1<HALF>(in, c);
-        if ((allowed && !(__ldcg(allowed + (c >> 5)) >> (c & 31) & 1u)) || (lists && (listed[at >> 5] >> (at & 31) & 1u))) f = -CUDART_INF_F;
+        if ((allowed && !(allowed[c >> 5] >> (c & 31) & 1u)) || (lists && (listed[at >> 5] >> (at & 31) & 1u))) f = -CUDART_INF_F;
         if (f > best) { best = f; bi = c; }
         if (keeps) store1<HALF>(out, c, f);
       }
@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(THREADS, 6) constrain_kernel(const __grid_cons
       __syncthreads();                                    // the words are whole, and the stream has written -inf there
       for (int k = threadIdx.x; k < n_listed; k += THREADS) {
         const int id = ids[k], c = lo + id;
-        if (allowed && !(__ldcg(allowed + (c >> 5)) >> (c & 31) & 1u)) continue;
+        if (allowed && !(allowed[c >> 5] >> (c & 31) & 1u)) continue;
         const float v = adjust(raw[k], table[number_of(listed, number, id)], r);
         better(best, bi, v, c);
         if (keeps) store1<HALF>(out, c, v);

@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(Cfg<HD, Q8>::WARPS * 32, 1) attention_kernel(c
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const int t = min((tile * ROWS + n + 8 * j) / G, a.T - 1);
-    vis[j] = a.visible ? (unsigned long long)__ldcg(a.visible + (long long)b * a.T + t) : t >= 63 ? ~0ull : (2ull << t) - 1;
+    vis[j] = a.visible ? (unsigned long long)a.visible[(long long)b * a.T + t] : t >= 63 ? ~0ull : (2ull << t) - 1;
     row_lo[j] = a.window > 0 ? max(0, s.pos + max(__popcll(vis[j]), 1) - a.window) : 0;
   }
   const int free_lo = a.window > 0 ? max(0, s.pos + 64 - a.window) : 0;      // from here to pos every row sees every key

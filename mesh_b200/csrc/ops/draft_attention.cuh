@@ -59,8 +59,8 @@ struct Seq {
 };
 __device__ __forceinline__ Seq sequence(const Args& a, int b) {
   Seq s;
-  s.pos = min(max(__ldcg(a.pos + b), 0), a.max_seq);
-  s.count = a.counts ? min(__ldcg(a.counts + b), a.T) : a.T;
+  s.pos = min(max(a.pos[b], 0), a.max_seq);
+  s.count = a.counts ? min(a.counts[b], a.T) : a.T;
   s.hi = min(s.pos + max(s.count, 0), a.max_seq);
   s.lo = a.window > 0 ? max(0, s.pos - a.window + 1) : 0;          // the root's; its descendants see less
   return s;

@@ -16,14 +16,17 @@ namespace kv {
 
 constexpr int THREADS = 256;
 
+// Everything that is read here may have been written by the kernel before, which may still run when this one starts: plain loads behind
+// the wait, and no __restrict__, with which the compiler would take the read-only path, that knows no such order.
+
 // 8 consecutive bf16.  ALIGNED: the address is a multiple of 16 bytes.
 template <bool ALIGNED>
 __device__ __forceinline__ uint4 load8(const __nv_bfloat16* p) {
-  if (ALIGNED) return __ldcg(reinterpret_cast<const uint4*>(p));
+  if (ALIGNED) return *reinterpret_cast<const uint4*>(p);
   uint4 r;
   unsigned short* h = reinterpret_cast<unsigned short*>(&r);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) h[i] = __ldcg(reinterpret_cast<const unsigned short*>(p) + i);
+  for (int i = 0; i < 8; ++i) h[i] = reinterpret_cast<const unsigned short*>(p)[i];
   return r;
 }
 
@@ -70,9 +73,9 @@ struct Strides { long long b, t, h; };
 
 // HD / 8 lanes share a row: 16 bytes of the key and 16 of the value each.
 template <int HD, bool Q8, bool ALIGNED>
-__global__ void __launch_bounds__(THREADS) append_kernel(MeshKvCache c, const __nv_bfloat16* __restrict__ k, const __nv_bfloat16* __restrict__ v,
-                                                         Strides ks, Strides vs, const int* __restrict__ pos,
-                                                         const int* __restrict__ counts, int T) {
+__global__ void __launch_bounds__(THREADS) append_kernel(MeshKvCache c, const __nv_bfloat16* k, const __nv_bfloat16* v,
+                                                         Strides ks, Strides vs, const int* pos,
+                                                         const int* counts, int T) {
   constexpr int LANES = HD / 8;
   griddep_launch_dependents();
   griddep_wait();
@@ -85,8 +88,8 @@ __global__ void __launch_bounds__(THREADS) append_kernel(MeshKvCache c, const __
   bool there = b < c.B;
   long long slot = 0;
   if (there) {
-    slot = (long long)__ldcg(pos + b) + t;
-    there = t < (counts ? __ldcg(counts + b) : T) && slot >= 0 && slot < c.max_seq;
+    slot = (long long)pos[b] + t;
+    there = t < (counts ? counts[b] : T) && slot >= 0 && slot < c.max_seq;
   }
   uint4 kx = make_uint4(0, 0, 0, 0), vx = kx;
   if (there) {
@@ -129,8 +132,8 @@ __device__ __forceinline__ uint4 decode8(const uint2& x, float scale) {
 }
 
 template <int HD, bool Q8>
-__global__ void __launch_bounds__(THREADS) read_kernel(MeshKvCache c, uint4* __restrict__ k_out, uint4* __restrict__ v_out,
-                                                       const int* __restrict__ start, const int* __restrict__ counts, int T) {
+__global__ void __launch_bounds__(THREADS) read_kernel(MeshKvCache c, uint4* k_out, uint4* v_out,
+                                                       const int* start, const int* counts, int T) {
   constexpr int LANES = HD / 8;
   griddep_launch_dependents();
   griddep_wait();
@@ -141,18 +144,18 @@ __global__ void __launch_bounds__(THREADS) read_kernel(MeshKvCache c, uint4* __r
   const int t = (int)(bt % T);
   const long long b = bt / T;
   if (b >= c.B) return;
-  const long long slot = (long long)__ldcg(start + b) + t;
+  const long long slot = (long long)start[b] + t;
   uint4 kx = make_uint4(0, 0, 0, 0), vx = kx;
-  if (t < (counts ? __ldcg(counts + b) : T) && slot >= 0 && slot < c.max_seq) {
+  if (t < (counts ? counts[b] : T) && slot >= 0 && slot < c.max_seq) {
     const long long at = (b * c.kv_heads + h) * c.max_seq + slot;
     if (Q8) {
-      const uint2 kc = __ldcg(reinterpret_cast<const uint2*>(c.k) + at * LANES + lane);
-      const uint2 vc = __ldcg(reinterpret_cast<const uint2*>(c.v) + at * LANES + lane);
-      kx = decode8(kc, __ldcg(c.k_scale + at));
-      vx = decode8(vc, __ldcg(c.v_scale + at));
+      const uint2 kc = reinterpret_cast<const uint2*>(c.k)[at * LANES + lane];
+      const uint2 vc = reinterpret_cast<const uint2*>(c.v)[at * LANES + lane];
+      kx = decode8(kc, c.k_scale[at]);
+      vx = decode8(vc, c.v_scale[at]);
     } else {
-      kx = __ldcg(reinterpret_cast<const uint4*>(c.k) + at * LANES + lane);
-      vx = __ldcg(reinterpret_cast<const uint4*>(c.v) + at * LANES + lane);
+      kx = reinterpret_cast<const uint4*>(c.k)[at * LANES + lane];
+      vx = reinterpret_cast<const uint4*>(c.v)[at * LANES + lane];
     }
   }
   k_out[row * LANES + lane] = kx;
@@ -168,15 +171,15 @@ struct KeepArgs {
 // One CTA moves the rows of one (layer, key or value, sequence, head): all of them into registers, a barrier, all out again,
 // so an entry may read a slot that another one writes.  At most 64 rows of 512 bytes: 8 x 16 bytes a thread.
 template <int ROW>                                       // bytes of a row
-__global__ void __launch_bounds__(THREADS) keep_kernel(const __grid_constant__ KeepArgs a, const int* __restrict__ pos,
-                                                       const int* __restrict__ path, const int* __restrict__ counts, int N,
+__global__ void __launch_bounds__(THREADS) keep_kernel(const __grid_constant__ KeepArgs a, const int* pos,
+                                                       const int* path, const int* counts, int N,
                                                        int kv_heads, int max_seq) {
   constexpr int LANES = ROW / 16, PER = KEEP_MOST * LANES / THREADS > 0 ? KEEP_MOST * LANES / THREADS : 1;
   griddep_launch_dependents();
   griddep_wait();
   const int h = blockIdx.x % kv_heads, b = blockIdx.x / kv_heads, which = blockIdx.y & 1, layer = blockIdx.y >> 1;
-  const long long p = __ldcg(pos + b);
-  const int n = min(N, counts ? __ldcg(counts + b) : N);
+  const long long p = pos[b];
+  const int n = min(N, counts ? counts[b] : N);
   const long long base = ((long long)b * kv_heads + h) * max_seq;
   uint4* data = reinterpret_cast<uint4*>(a.data[layer][which]) + base * LANES;
   uint4 r[PER];
@@ -186,7 +189,7 @@ __global__ void __launch_bounds__(THREADS) keep_kernel(const __grid_constant__ K
     const int j = i * THREADS + threadIdx.x, e = j / LANES;
     to[i] = -1;
     if (e >= n) continue;
-    const int from = __ldcg(path + (long long)b * N + e);
+    const int from = path[(long long)b * N + e];
     const long long src = p + from, dst = p + e;
     if (from < 0 || from == e || p < 0 || src >= max_seq || dst >= max_seq) continue;
     r[i] = data[src * LANES + j % LANES];
@@ -196,7 +199,7 @@ __global__ void __launch_bounds__(THREADS) keep_kernel(const __grid_constant__ K
   float s = 0.f;
   long long s_to = -1;
   if (scale && (int)threadIdx.x < n) {
-    const int from = __ldcg(path + (long long)b * N + threadIdx.x);
+    const int from = path[(long long)b * N + threadIdx.x];
     const long long src = p + from, dst = p + threadIdx.x;
     if (from >= 0 && p >= 0 && src < max_seq && dst < max_seq) {
       s = scale[base + src];

@@ -285,6 +285,7 @@ class E2BDecoder:
         (drafts of each sequence; ``None``: T) -> int32 ``[B, T]``, the token that the model chooses after each of them.  Their rows lie in
         slots ``pos .. pos + T`` of the caches, which must be there, until ``accept`` or the next step; ``pos`` and ``tok`` stay.
         ``constraints``: arguments of ``ops/logits.py::constrain_logits`` for the ``B * T`` rows of logits.
+        After a first call the step may be captured in a CUDA graph.
 
         Up to 8 rows the logits are fp32 (as in ``decode``), beyond that they come from the bf16 product: equal ones are
         likelier there, and the lowest id is taken.  One rank: each holds a part of the vocabulary, and the choice among the

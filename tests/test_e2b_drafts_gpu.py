@@ -123,6 +123,25 @@ def test_drafts_under_a_grammar_and_a_chain():
     check_status()
 
 
+def test_captured_step_of_drafts_follows_its_inputs():
+    from mesh_b200.ops.draft import tree_visible
+    from mesh_b200.utils.status import check_status
+    B, T, n = 2, 24, len(PARENTS)
+    m, _, g = _model(B, "w4", 8, T)
+    drafts = torch.zeros((B, n), dtype=torch.int32, device="cuda")
+    visible = tree_visible([PARENTS] * B).cuda()
+    m.draft_step(drafts, visible)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        chosen = m.draft_step(drafts, visible)
+    for at in (T, T + 9, 1):
+        drafts.copy_(torch.randint(0, m.cfg.vocab, (B, n), generator=g, dtype=torch.int32))
+        m.pos.fill_(at)
+        graph.replay()
+        assert torch.equal(chosen, m.draft_step(drafts, visible))
+    check_status()
+
+
 def test_refusals():
     from mesh_b200.models.e2b import E2BDecoder
     with pytest.raises(ValueError, match="cache_bits"):
