@@ -30,32 +30,52 @@ __device__ __forceinline__ uint4 load8(const __nv_bfloat16* p) {
   return r;
 }
 
-// Codes of eight values of a row whose largest magnitude has the bf16 bits `top`, and the row's scale.
+// A row's scale, from the bf16 bits of its largest magnitude.
+__device__ __forceinline__ float scale_of(uint32_t top) { return top >= 0x7f80u ? __int_as_float(0x7fc00000) : __uint_as_float(top << 16) / 127.f; }
+
+__device__ __forceinline__ unsigned long long pair(float lo, float hi) {
+  unsigned long long r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// Codes of eight values of a row whose largest magnitude has the bf16 bits `top`.
 //
 // The quotient 127 x / a has a numerator of 15 bits and a denominator of 8, so it is either exactly half way between two
-// integers or further than 2^-17 of its size from there: a product with the rounded reciprocal (off by 2^-24 of its size) falls
-// on the right side of every border except on the border itself.  There the remainder, which is exact in fp32, is half of a / 128
-// and the odd code goes to its even neighbour.  This costs 6 operations a value; a division would cost more than the memory does.
-__device__ __forceinline__ uint2 encode8(const uint4& x, uint32_t top, float& scale) {
+// integers or further than 2^-17 of its size from there.  A product q with the rounded reciprocal is off by 2^-23 of its size, which
+// is good enough except half way.  The remainder v - q a is exact, and q plus remainder times reciprocal is then the quotient itself,
+// which fp32 holds, so the sum with 1.5 2^23 goes to the even neighbour.  Five operations for two values; a division, or a
+// comparison for the half way ones, costs more than the memory does (16000 rows: 127 us).
+__device__ __forceinline__ uint2 encode8(const uint4& x, uint32_t top) {
+  if (top >= 0x7f80u || top == 0) return make_uint2(0, 0);              // a NaN or an infinity in the row
   const float a0 = __uint_as_float(top << 16);
-  if (top >= 0x7f80u) {                                  // a NaN or an infinity in the row
-    scale = __int_as_float(0x7fc00000);
-    return make_uint2(0, 0);
-  }
-  scale = a0 / 127.f;
-  if (top == 0) return make_uint2(0, 0);
-  const float lift = a0 < 1e-18f ? 0x1p66f : 1.f;        // keeps 1 / a finite; exact
-  const float a = a0 * lift, a7 = a * 0x1p-7f, inv = 128.f / a, f = lift * (127.f / 128.f);
+  const float lift = a0 < 1e-18f ? 0x1p66f : 1.f;        // keeps 1 / a finite and the remainder in range; exact
+  const float a = a0 * lift * 0x1p-7f, inv = __frcp_rn(a), f = lift * (127.f / 128.f);
+  const unsigned long long a2 = pair(-a, -a), inv2 = pair(inv, inv), f2 = pair(f, f), magic = pair(12582912.f, 12582912.f);
   const uint32_t w[4] = {x.x, x.y, x.z, x.w};
   uint32_t code[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float v = __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16) * f;     // x 127 / 128, exact
-    float t = __fmaf_rn(v, inv, 12582912.f);             // 1.5 2^23: the sum's low bits are the nearest integer
-    const float c = t - 12582912.f;
-    const float e = __fmaf_rn(-c, a7, v);                // remainder, in units of a7
-    if (fabsf(e) == 0.5f * a7 && (__float_as_uint(t) & 1u)) t += e > 0.f ? 1.f : -1.f;
-    code[i] = __float_as_uint(t);
+  for (int i = 0; i < 4; ++i) {
+    const unsigned long long v = mul2(pair(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u)), f2);      // x 127 / 128, exact
+    const unsigned long long q = mul2(v, inv2);
+    const unsigned long long t = add2(fma2(fma2(q, a2, v), inv2, q), magic);
+    code[2 * i] = (uint32_t)t;                           // the low bits of each half are the nearest integer
+    code[2 * i + 1] = (uint32_t)(t >> 32);
   }
   uint2 r;
   r.x = __byte_perm(__byte_perm(code[0], code[1], 0x0040), __byte_perm(code[2], code[3], 0x0040), 0x5410);
@@ -71,7 +91,10 @@ __device__ __forceinline__ uint32_t largest(const uint4& x) {
 
 struct Strides { long long b, t, h; };
 
-// HD / 8 lanes share a row: 16 bytes of the key and 16 of the value each.
+// HD / 8 lanes share a row: 16 bytes of the key and 16 of the value each.  Memory bounds it with bf16 rows (4 sequences of 16000, 8 KV
+// heads of 128: 79 us, 6.6 TB/s read and written); with 8-bit ones, 87 us, 4.6 TB/s, the trip of each row's maximum through its lanes
+// and the codes' arithmetic stand between loads and stores (two rows a thread: 83 us, but 2.9 us instead of 2.2 for the
+// single token of a step).
 template <int HD, bool Q8, bool ALIGNED>
 __global__ void __launch_bounds__(THREADS) append_kernel(MeshKvCache c, const __nv_bfloat16* k, const __nv_bfloat16* v,
                                                          Strides ks, Strides vs, const int* pos,
@@ -79,26 +102,22 @@ __global__ void __launch_bounds__(THREADS) append_kernel(MeshKvCache c, const __
   constexpr int LANES = HD / 8;
   griddep_launch_dependents();
   griddep_wait();
-  const long long row = (long long)blockIdx.x * (THREADS / LANES) + threadIdx.x / LANES;     // (b, t, h), h fastest
+  const unsigned row = blockIdx.x * (THREADS / LANES) + threadIdx.x / LANES;       // (b, t, h), h fastest; fewer than 2^31
   const int lane = threadIdx.x % LANES;
-  const int h = (int)(row % c.kv_heads);
-  const long long bt = row / c.kv_heads;
-  const int t = (int)(bt % T);
-  const long long b = bt / T;
-  bool there = b < c.B;
-  long long slot = 0;
-  if (there) {
-    slot = (long long)pos[b] + t;
-    there = t < (counts ? counts[b] : T) && slot >= 0 && slot < c.max_seq;
-  }
+  const unsigned bt = row / (unsigned)c.kv_heads, h = row - bt * c.kv_heads;
+  const long long b = bt / (unsigned)T, t = bt - (unsigned)b * T;
+  long long at = -1;
   uint4 kx = make_uint4(0, 0, 0, 0), vx = kx;
-  if (there) {
-    kx = load8<ALIGNED>(k + b * ks.b + t * ks.t + h * ks.h + lane * 8);
-    vx = load8<ALIGNED>(v + b * vs.b + t * vs.t + h * vs.h + lane * 8);
+  if (b < c.B) {
+    const long long slot = pos[b] + t;
+    if (t < (counts ? counts[b] : T) && slot >= 0 && slot < c.max_seq) {
+      at = (b * c.kv_heads + h) * c.max_seq + slot;
+      kx = load8<ALIGNED>(k + b * ks.b + t * ks.t + h * ks.h + lane * 8);
+      vx = load8<ALIGNED>(v + b * vs.b + t * vs.t + h * vs.h + lane * 8);
+    }
   }
-  const long long at = (b * c.kv_heads + h) * c.max_seq + slot;
   if (!Q8) {
-    if (there) {
+    if (at >= 0) {
       reinterpret_cast<uint4*>(c.k)[at * LANES + lane] = kx;
       reinterpret_cast<uint4*>(c.v)[at * LANES + lane] = vx;
     }
@@ -107,15 +126,12 @@ __global__ void __launch_bounds__(THREADS) append_kernel(MeshKvCache c, const __
   uint32_t top = largest(kx) | largest(vx) << 16;        // both rows at once
 #pragma unroll
   for (int o = LANES / 2; o > 0; o >>= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
-  float k_scale, v_scale;
-  const uint2 kc = encode8(kx, top & 0xffffu, k_scale), vc = encode8(vx, top >> 16, v_scale);
-  if (!there) return;
+  const uint2 kc = encode8(kx, top & 0xffffu), vc = encode8(vx, top >> 16);
+  const float scale = scale_of(lane & 1 ? top >> 16 : top & 0xffffu);
+  if (at < 0) return;
   reinterpret_cast<uint2*>(c.k)[at * LANES + lane] = kc;
   reinterpret_cast<uint2*>(c.v)[at * LANES + lane] = vc;
-  if (lane == 0) {
-    c.k_scale[at] = k_scale;
-    c.v_scale[at] = v_scale;
-  }
+  if (lane < 2) (lane ? c.v_scale : c.k_scale)[at] = scale;
 }
 
 // Eight codes times their row's scale, rounded once.
@@ -131,35 +147,51 @@ __device__ __forceinline__ uint4 decode8(const uint2& x, float scale) {
   return r;
 }
 
-template <int HD, bool Q8>
+// N rows a thread.  With 8-bit rows a thread has half of the bytes on their way that it has with bf16 ones, so where the grid is large,
+// two rows: 8 KV heads of 128, 4 sequences of 16000, 62 us (6.4 TB/s read and written) instead of 70; with 500 rows each one row a
+// thread takes half a microsecond less.  Rows of bf16 take as long either way.
+constexpr long long TWO = 4096;                          // CTAs, of one row a thread
+template <int HD, bool Q8, int N>
 __global__ void __launch_bounds__(THREADS) read_kernel(MeshKvCache c, uint4* k_out, uint4* v_out,
                                                        const int* start, const int* counts, int T) {
   constexpr int LANES = HD / 8;
   griddep_launch_dependents();
   griddep_wait();
-  const long long row = (long long)blockIdx.x * (THREADS / LANES) + threadIdx.x / LANES;
   const int lane = threadIdx.x % LANES;
-  const int h = (int)(row % c.kv_heads);
-  const long long bt = row / c.kv_heads;
-  const int t = (int)(bt % T);
-  const long long b = bt / T;
-  if (b >= c.B) return;
-  const long long slot = (long long)start[b] + t;
-  uint4 kx = make_uint4(0, 0, 0, 0), vx = kx;
-  if (t < (counts ? counts[b] : T) && slot >= 0 && slot < c.max_seq) {
+  uint4 kx[N], vx[N];
+  float k_scale[N], v_scale[N];
+  bool there[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const unsigned row = (blockIdx.x * N + i) * (THREADS / LANES) + threadIdx.x / LANES;
+    const unsigned bt = row / (unsigned)c.kv_heads, h = row - bt * c.kv_heads;
+    const long long b = bt / (unsigned)T, t = bt - (unsigned)b * T;
+    there[i] = b < c.B;
+    kx[i] = vx[i] = make_uint4(0, 0, 0, 0);
+    k_scale[i] = v_scale[i] = 0.f;
+    if (!there[i]) continue;
+    const long long slot = (long long)start[b] + t;
+    if (t >= (counts ? counts[b] : T) || slot < 0 || slot >= c.max_seq) continue;
     const long long at = (b * c.kv_heads + h) * c.max_seq + slot;
     if (Q8) {
       const uint2 kc = reinterpret_cast<const uint2*>(c.k)[at * LANES + lane];
       const uint2 vc = reinterpret_cast<const uint2*>(c.v)[at * LANES + lane];
-      kx = decode8(kc, c.k_scale[at]);
-      vx = decode8(vc, c.v_scale[at]);
+      kx[i].x = kc.x; kx[i].y = kc.y;
+      vx[i].x = vc.x; vx[i].y = vc.y;
+      k_scale[i] = c.k_scale[at];
+      v_scale[i] = c.v_scale[at];
     } else {
-      kx = reinterpret_cast<const uint4*>(c.k)[at * LANES + lane];
-      vx = reinterpret_cast<const uint4*>(c.v)[at * LANES + lane];
+      kx[i] = reinterpret_cast<const uint4*>(c.k)[at * LANES + lane];
+      vx[i] = reinterpret_cast<const uint4*>(c.v)[at * LANES + lane];
     }
   }
-  k_out[row * LANES + lane] = kx;
-  v_out[row * LANES + lane] = vx;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (!there[i]) continue;
+    const long long row = ((long long)blockIdx.x * N + i) * (THREADS / LANES) + threadIdx.x / LANES;
+    k_out[row * LANES + lane] = Q8 ? decode8(make_uint2(kx[i].x, kx[i].y), k_scale[i]) : kx[i];
+    v_out[row * LANES + lane] = Q8 ? decode8(make_uint2(vx[i].x, vx[i].y), v_scale[i]) : vx[i];
+  }
 }
 
 constexpr int KEEP_MOST = 64, KEEP_LAYERS = 64;
@@ -169,7 +201,8 @@ struct KeepArgs {
 };
 
 // One CTA moves the rows of one (layer, key or value, sequence, head): all of them into registers, a barrier, all out again,
-// so an entry may read a slot that another one writes.  At most 64 rows of 512 bytes: 8 x 16 bytes a thread.
+// so an entry may read a slot that another one writes.  At most 64 rows of 512 bytes: 8 x 16 bytes a thread.  One launch for all
+// layers, which is what it costs: 6 rows of 8 sequences in 30 layers 3.1 us, 64 rows (62 MB read and written) 9 us.
 template <int ROW>                                       // bytes of a row
 __global__ void __launch_bounds__(THREADS) keep_kernel(const __grid_constant__ KeepArgs a, const int* pos,
                                                        const int* path, const int* counts, int N,
@@ -246,7 +279,7 @@ extern "C" int mesh_kv_append(const MeshKvCache* c, const void* k, const void* v
   if (c->B == 0 || T <= 0) return 0;
   const int lanes = c->head_dim / 8, per = kv::THREADS / lanes;
   const long long rows = (long long)c->B * T * c->kv_heads, blocks = (rows + per - 1) / per;
-  if (blocks > 0x7fffffffll) return set_error(-2, "kv_append: too many rows for one call");
+  if (rows + per > 0x7fffffffll) return set_error(-2, "kv_append: too many rows for one call");
   const bool aligned = !((((uintptr_t)k | (uintptr_t)v) % 16) || ((k_sb | k_st | k_sh | v_sb | v_st | v_sh) % 8));
   const kv::Strides ks = {k_sb, k_st, k_sh}, vs = {v_sb, v_st, v_sh};
   const dim3 grid((unsigned)blocks);
@@ -269,12 +302,15 @@ extern "C" int mesh_kv_read(const MeshKvCache* c, void* k_out, void* v_out, cons
   if (c->B == 0 || T <= 0) return 0;
   if (((uintptr_t)k_out | (uintptr_t)v_out) % 16) return set_error(-2, "kv_read: the results must start on a multiple of 16 bytes");
   const int per = kv::THREADS / (c->head_dim / 8);
-  const long long rows = (long long)c->B * T * c->kv_heads, blocks = (rows + per - 1) / per;
-  if (blocks > 0x7fffffffll) return set_error(-2, "kv_read: too many rows for one call");
+  const long long rows = (long long)c->B * T * c->kv_heads;
+  long long blocks = (rows + per - 1) / per;
+  const bool two = c->bits == 8 && blocks >= kv::TWO;
+  if (two) blocks = (blocks + 1) / 2;
+  if (rows + 2 * per > 0x7fffffffll) return set_error(-2, "kv_read: too many rows for one call");
   const dim3 grid((unsigned)blocks);
 #define MESH_READ(HD)                                                                                                          \
-  MESH_CUDA_OK(kv::launch(c->bits == 8 ? kv::read_kernel<HD, true> : kv::read_kernel<HD, false>, grid, kv::THREADS, stream, *c, \
-                          (uint4*)k_out, (uint4*)v_out, start, counts, T))
+  MESH_CUDA_OK(kv::launch(two ? kv::read_kernel<HD, true, 2> : c->bits == 8 ? kv::read_kernel<HD, true, 1> : kv::read_kernel<HD, false, 1>, \
+                          grid, kv::THREADS, stream, *c, (uint4*)k_out, (uint4*)v_out, start, counts, T))
   switch (c->head_dim) {
     case 64: MESH_READ(64); break;
     case 128: MESH_READ(128); break;
