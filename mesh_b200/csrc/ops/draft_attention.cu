@@ -421,11 +421,17 @@ __global__ void __launch_bounds__(Cfg<HD, Q8>::WARPS * 32, 1) attention_kernel(c
         const float4 v = o_s[(w * NT + i) * 32 + lane];
         acc.x += w0 * v.x; acc.y += w0 * v.y; acc.z += w1 * v.z; acc.w += w1 * v.w;
       }
-      if (!whole) a.part[((long long)slot * NT + i) * 32 + lane] = acc;
+      if (!whole && !a.cluster) a.part[((long long)slot * NT + i) * 32 + lane] = acc;
     }
     sum[y] = acc;
   }
-  if (!whole) {
+  if (!whole && a.cluster) {                              // for the cluster's CTAs
+    __syncthreads();
+#pragma unroll
+    for (int y = 0; y < TURNS; ++y)
+      if (y * C::WARPS + warp < NT) o_s[(y * C::WARPS + warp) * 32 + lane] = sum[y];
+    if (threadIdx.x < ROWS) ml_s[0][threadIdx.x] = make_float2(m_s[threadIdx.x], l_s[threadIdx.x]);
+  } else if (!whole) {
     if (threadIdx.x < ROWS) a.part_ml[slot * ROWS + threadIdx.x] = make_float2(m_s[threadIdx.x], l_s[threadIdx.x]);
   } else {
     __syncthreads();
@@ -450,6 +456,52 @@ __global__ void __launch_bounds__(Cfg<HD, Q8>::WARPS * 32, 1) attention_kernel(c
   }
   __syncthreads();                                        // shared memory is the next item's
   }
+
+  // ---- a cluster's item that was cut: each CTA joins some of the tiles of columns
+  const int ranks = walk.ranks;
+  if (ranks <= 1) return;                                 // the same in all CTAs of the cluster; 0 without clusters
+  cluster_sync_all();
+  const Item x = item_of_cluster(a);
+  const int n_rows = sequence(a, x.b).count * G - x.tile * ROWS;
+  const uint32_t o_at = smem_u32(smem + C::QB), ml_at = smem_u32(ml_s);
+  for (int i = warp * a.cluster + blockIdx.x % a.cluster; i < NT; i += C::WARPS * a.cluster) {
+    float2 u[MOST_RANKS][2];
+    float4 v[MOST_RANKS];
+    float mm[2] = {-CUDART_INF_F, -CUDART_INF_F}, ll[2] = {0.f, 0.f};
+#pragma unroll
+    for (int r = 0; r < MOST_RANKS; ++r) {
+      if (r >= ranks) break;
+      u[r][0] = cluster_load2(ml_at + n * 8, r);
+      u[r][1] = cluster_load2(ml_at + (n + 8) * 8, r);
+      v[r] = cluster_load4(o_at + (i * 32 + lane) * 16, r);
+    }
+#pragma unroll
+    for (int r = 0; r < MOST_RANKS; ++r) {
+      if (r >= ranks) break;
+      mm[0] = fmaxf(mm[0], u[r][0].x);
+      mm[1] = fmaxf(mm[1], u[r][1].x);
+    }
+    const float ref[2] = {mm[0] == -CUDART_INF_F ? 0.f : mm[0], mm[1] == -CUDART_INF_F ? 0.f : mm[1]};
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int r = 0; r < MOST_RANKS; ++r) {
+      if (r >= ranks) break;
+      const float w0 = ex2(u[r][0].x - ref[0]), w1 = ex2(u[r][1].x - ref[1]);
+      ll[0] += w0 * u[r][0].y;
+      ll[1] += w1 * u[r][1].y;
+      acc.x += w0 * v[r].x; acc.y += w0 * v[r].y; acc.z += w1 * v[r].z; acc.w += w1 * v[r].w;
+    }
+    const float i0 = ll[0] == 0.f ? 0.f : 1.f / ll[0], i1 = ll[1] == 0.f ? 0.f : 1.f / ll[1];
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      const int row = n + 8 * y, r = x.tile * ROWS + row;
+      if (row >= n_rows) continue;
+      __nv_bfloat16* dst = a.out + x.b * a.o_sb + (r / G) * a.o_st + (long long)(x.hk * G + r % G) * HD;
+      dst[column<C::VW>(i, 2 * t4)] = __float2bfloat16_rn(y ? acc.z * i1 : acc.x * i0);
+      dst[column<C::VW>(i, 2 * t4 + 1)] = __float2bfloat16_rn(y ? acc.w * i1 : acc.y * i0);
+    }
+  }
+  cluster_sync_all();                                     // the others have read this CTA's part
 }
 
 // Joins the shares of the items that were cut.  SPLIT: a CTA per item and tile of 8 columns, whose warps take the shares in turn (few items
@@ -536,11 +588,26 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args 
 // bits, 4 heads a group, 8 sequences: single tokens over 12000 keys 57.7 us cut equally, 60.4 in pieces 5 longer; 64 drafts over 4000
 // keys 99.2 us and, in pieces 9 longer, 92.6.
 constexpr int FEW = 4, WIDE_FEW = 12;
+// Units that the longest share of a cluster's item may have beyond an equal one, with the cache filled: what the second kernel and cut items
+// cost.  8 KV heads of 128 in 8 bits, 4 heads a group, with clusters and with the second kernel: one token of one sequence over 1000
+// keys 9.0 and 10.6 us, 8000 keys (3.0 units) 16.2 and 16.0; 16 sequences over 2000 keys (1.5) 23.0 and 26.9, 8000 keys (5.7) 62.7 and
+// 60.9; 64 drafts of 4 sequences over 4000 keys (4.2) 52.8 and 58.2, 8000 keys (8.4) 88.5 and 80.9; 32 of one over 4000 keys
+// (4.4) 26.6 and 25.6.
+constexpr double LONGER = 3, WIDE_LONGER = 4.3;
 
 // The kernel for many rows, with tiles of 128, from three tiles of 16 on: it has a longer start and end, and this one fetches the
 // keys once per tile.  Eight sequences, 8 KV heads of 128 in 8 bits, 4 heads a group, this kernel and the other one: 8 drafts over
 // 500 keys 14 and 21 us, over 12000 keys 100 and 119 us (bf16: 112 and 102); 12 drafts 25 and 22, 142 and 120 us.
 static bool wide(const MeshKvCache* c, const MeshDraftAttention* a) { return a->T * (a->q_heads / c->kv_heads) > 2 * ROWS; }
+
+static int clusters(const MeshKvCache* c, bool w, int ranks) {
+  const bool q8 = c->bits == 8;
+  if (w) return wide_clusters(c->head_dim, q8, ranks);
+#define MESH_CLUSTERS(HD, Q8) clusters_at_once<Cfg<HD, Q8>::WARPS * 32, Cfg<HD, Q8>::SMEM>(attention_kernel<HD, Q8>, ranks)
+  if (q8) return c->head_dim == 64 ? MESH_CLUSTERS(64, true) : c->head_dim == 128 ? MESH_CLUSTERS(128, true) : MESH_CLUSTERS(256, true);
+  return c->head_dim == 64 ? MESH_CLUSTERS(64, false) : c->head_dim == 128 ? MESH_CLUSTERS(128, false) : MESH_CLUSTERS(256, false);
+#undef MESH_CLUSTERS
+}
 
 static void cut(const MeshKvCache* c, const MeshDraftAttention* a, Args& p) {
   const bool w = wide(c, a), q8 = c->bits == 8;
@@ -556,6 +623,14 @@ static void cut(const MeshKvCache* c, const MeshDraftAttention* a, Args& p) {
   const long long most = a->splits > 0 ? a->splits : sm_count();
   p.shares = (int)(units < most ? units : most);
   p.few = a->splits > 0 ? 0 : w ? WIDE_FEW : FEW;
+  p.cluster = 0;
+  const long long items = (long long)c->B * c->kv_heads * p.tiles, longest = (keys + p.unit - 1) / p.unit;
+  if (a->splits > 0 || items > most) return;
+  for (int ranks = MOST_RANKS; ranks >= 1; ranks /= 2) {
+    if (ranks / 2 >= longest || ranks * items > most || (ranks > 1 && clusters(c, w, ranks) < items)) continue;
+    if (longest * (1.0 / ranks - 1.0 * items / most) <= (w ? WIDE_LONGER : LONGER)) p.cluster = ranks;
+    return;
+  }
 }
 
 static int check(const MeshKvCache* c, const MeshDraftAttention* a) {
@@ -582,7 +657,7 @@ static int run(const Args& p, void* stream) {
     MESH_CUDA_OK(cudaFuncSetAttribute(attention_kernel<HD, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
     configured.fetch_or(1ull << (dev & 63));
   }
-  MESH_CUDA_OK(launch(attention_kernel<HD, Q8>, dim3(p.shares), C::WARPS * 32, C::SMEM, stream, p));
+  MESH_CUDA_OK(launch(attention_kernel<HD, Q8>, dim3(grid_of(p)), C::WARPS * 32, C::SMEM, stream, p));
   if (p.part) {
     const unsigned items = (unsigned)(p.B * p.kv_heads * p.tiles);
     if (p.shares > 2ll * items) MESH_CUDA_OK(launch(join_kernel<HD, Q8, true>, dim3(items, HD / 8), 256, 0, stream, p));
@@ -599,7 +674,7 @@ extern "C" long long mesh_draft_attention_scratch(const MeshKvCache* c, const Me
   if (check(c, a)) return -1;
   Args p;
   cut(c, a, p);
-  return p.shares <= 1 ? 0 : 2ll * p.shares * p.rows * (c->head_dim + 2);
+  return p.shares <= 1 || p.cluster ? 0 : 2ll * p.shares * p.rows * (c->head_dim + 2);
 }
 
 extern "C" int mesh_draft_attention(const MeshKvCache* c, const MeshDraftAttention* a, void* stream) {
@@ -621,7 +696,7 @@ extern "C" int mesh_draft_attention(const MeshKvCache* c, const MeshDraftAttenti
   if ((long long)c->B * c->kv_heads * p.tiles * ((c->max_seq + p.unit - 1) / p.unit + 1) > 0x7fffffff || p.shares > 0x3fffffff)
     return set_error(-2, "draft_attention: too many rows and keys for one call");
   p.scale_log2 = a->scale * 1.4426950408889634f;
-  if (p.shares > 1) {
+  if (p.shares > 1 && !p.cluster) {
     if (!a->scratch || (uintptr_t)a->scratch % 16) return set_error(-2, "draft_attention: scratch memory must be given and start on a multiple of 16 bytes");
     p.part = (float4*)a->scratch;
     p.part_ml = (float2*)(a->scratch + 2ll * p.shares * p.rows * c->head_dim);

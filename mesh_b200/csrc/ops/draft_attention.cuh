@@ -24,6 +24,7 @@ struct Args {
   float4* part; float2* part_ml;      // two slots per CTA: the output as its threads hold it, and {m, l} of the rows
   int shares;                         // CTAs of the attention kernel
   int few;                            // see cut_work; 0: equal shares in any case
+  int cluster;                        // CTAs of an item, a cluster (see item_of_cluster); 0: shares of all keys, and a kernel that joins them
   Status* status;
 };
 
@@ -172,10 +173,30 @@ struct Stretch {
 struct Walk {
   int at, stop;                       // units, relative to the first of sequence b
   int b, piece; bool first;
+  int ranks;                          // clusters: CTAs that have keys of the item
 };
+// Where contexts are short a second kernel would cost a third of the time: then an item is a cluster's, cut evenly among its CTAs, which
+// join their results through distributed shared memory.  It may be no item, if its sequence has fewer tiles.
+struct Item {
+  int b, hk, tile;
+};
+__device__ __forceinline__ Item item_of_cluster(const Args& a) {
+  const int item = blockIdx.x / a.cluster;
+  return {item / a.tiles / a.kv_heads, item / a.tiles % a.kv_heads, item % a.tiles};
+}
 __device__ __forceinline__ void begin_walk(const Args& a, Walk* w) {
+  if (a.cluster) {
+    const Item x = item_of_cluster(a);
+    const Load l = load_of(a, x.b, 1);
+    const int rank = blockIdx.x % a.cluster, per = (l.units + a.cluster - 1) / a.cluster, first = (x.hk * l.tiles + x.tile) * l.units;
+    if ((threadIdx.x & 31) == 0) {
+      const bool there = x.tile < l.tiles;
+      *w = {there ? first + min(rank * per, l.units) : 0, there ? first + min((rank + 1) * per, l.units) : 0, x.b, 1, true, there ? (l.units + per - 1) / per : 0};
+    }
+    return;
+  }
   const Cut c = cut_work(a);
-  if ((threadIdx.x & 31) == 0) { w->at = w->stop = 0; w->b = 0; w->piece = c.piece; w->first = true; }
+  if ((threadIdx.x & 31) == 0) *w = {0, 0, 0, c.piece, true, 0};
   if ((int)blockIdx.x < min(c.shares, c.total)) {
     const int w0 = share_begin(c, blockIdx.x), w1 = share_begin(c, blockIdx.x + 1);
     int before;
@@ -234,6 +255,19 @@ __device__ __forceinline__ void shares_of_item(const Args& a, int b, int hk, int
   }
 }
 
+// Four floats, or two, of another CTA's shared memory.
+__device__ __forceinline__ float4 cluster_load4(uint32_t at, int cta) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(mapa_u32(at, cta)) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 cluster_load2(uint32_t at, int cta) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(mapa_u32(at, cta)) : "memory");
+  return v;
+}
+constexpr int MOST_RANKS = 8;         // CTAs of a cluster
+
 template <class... P>
 static cudaError_t launch(void (*kern)(P...), dim3 grid, int threads, int smem, void* stream, const Args& a) {
   cudaLaunchConfig_t cfg;
@@ -242,17 +276,57 @@ static cudaError_t launch(void (*kern)(P...), dim3 grid, int threads, int smem, 
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = (cudaStream_t)stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = a.cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = a.cluster > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kern, a);
 }
+
+// Clusters of 2, 4 or 8 CTAs that the current device runs at the same time, a CTA taking an SM: it depends on how the SMs lie together, which
+// differs from device to device (sixteen of eight fit into 148 SMs, but not always into their groups).  0 if it cannot be told.
+template <int THREADS, int SMEM, class... P>
+static int clusters_at_once(void (*kern)(P...), int ranks) {
+  static std::atomic<int> known[64][4];                   // one more than it; kernels of the same sizes have the same
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  std::atomic<int>& k = known[dev & 63][ranks == 8 ? 3 : ranks == 4 ? 2 : 1];
+  if (k.load()) return k.load() - 1;
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(ranks * 64);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = SMEM;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ranks;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  k.store(n + 1);
+  return n;
+}
+
+static inline unsigned grid_of(const Args& a) { return a.cluster ? (unsigned)(a.B * a.kv_heads * a.tiles * a.cluster) : (unsigned)a.shares; }
 
 // The kernel for many query rows (draft_attention_wide.cu): rows of a tile, keys of a unit, and the call.
 constexpr int WIDE_ROWS = 128, WIDE_UNIT = 64;
 int run_wide(const Args& p, int head_dim, bool q8, void* stream);
+int wide_clusters(int head_dim, bool q8, int ranks);
 
 }  // namespace draft
 }  // namespace mesh

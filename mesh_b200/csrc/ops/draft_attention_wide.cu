@@ -154,6 +154,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
   __shared__ Walk walk_s;
   __shared__ float top_s[2][2][2][TT];                      // [group][its block & 1][half][row]
   __shared__ float m_s[2][TT], sum_s[4][TT];                // [group][row]: reference points; [group, half][row]
+  __shared__ float2 ml_s[TT];                               // of a cluster's part
   __shared__ volatile int over_s;                           // blocks whose second product is over
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = a.q_heads / a.kv_heads;
 
@@ -649,6 +650,11 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
 #pragma unroll
             for (int i = 0; i < 8; ++i) p[i] = w[i];
           }
+        } else if (real && a.cluster) {                   // the only stretch: the rings are not used again
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            reinterpret_cast<float4*>(gen)[(c * 4 + i) * TT + row] =
+                make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
         } else if (real) {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
@@ -657,7 +663,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
         }
         __syncwarp();
       }
-      if (!x.whole && real && quarter == 0) a.part_ml[(long long)x.slot * TT + row] = make_float2(m, l);
+      if (!x.whole && real && quarter == 0) (a.cluster ? ml_s[row] : a.part_ml[(long long)x.slot * TT + row]) = make_float2(m, l);
       __syncwarp();
     }
   }
@@ -667,6 +673,41 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
     tc_fence_after();
     tmem_dealloc<1>(tmem, 512);
   }
+  // ---- a cluster's item that was cut: each CTA joins some groups of 8 columns
+  const int ranks = walk_s.ranks;
+  if (ranks <= 1) return;                                   // the same in all CTAs of the cluster; 0 without clusters
+  cluster_sync_all();
+  const Item item = item_of_cluster(a);
+  const int n_rows = min(sequence(a, item.b).count * G - item.tile * TT, TT);
+  for (int e = threadIdx.x; e < TT * (HD / 8 / a.cluster); e += THREADS) {
+    const int row = e % TT, i = 2 * (e / TT * a.cluster + blockIdx.x % a.cluster), r = item.tile * TT + row;
+    if (row >= n_rows) continue;
+    float m = -CUDART_INF_F, l = 0.f;
+    for (int c = 0; c < ranks; ++c) m = fmaxf(m, cluster_load2(smem_u32(ml_s + row), c).x);
+    const float ref = m == -CUDART_INF_F ? 0.f : m;
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int c = 0; c < ranks; ++c) {
+      const float2 ml = cluster_load2(smem_u32(ml_s + row), c);
+      const float4 u = cluster_load4(base + (i * TT + row) * 16, c), v = cluster_load4(base + ((i + 1) * TT + row) * 16, c);
+      const float wt = ex2(ml.x - ref);
+      l += wt * ml.y;
+      acc[0] += wt * u.x; acc[1] += wt * u.y; acc[2] += wt * u.z; acc[3] += wt * u.w;
+      acc[4] += wt * v.x; acc[5] += wt * v.y; acc[6] += wt * v.z; acc[7] += wt * v.w;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + item.b * a.o_sb + (r / G) * a.o_st + (long long)(item.hk * G + r % G) * HD + i * 4);
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = pack16(false, acc[2 * j] * inv, acc[2 * j + 1] * inv);
+    if ((reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
+      *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) dst[j] = w[j];
+    }
+  }
+  cluster_sync_all();                                       // the others have read this CTA's part
 }
 
 // Joins the shares of the items that were cut, a thread per row and 8 columns.  SPLIT: a CTA per item and 8 columns, four groups of threads
@@ -742,7 +783,7 @@ int run(const Args& p, void* stream) {
     MESH_CUDA_OK(cudaFuncSetAttribute(wide_kernel<HD, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
     configured.fetch_or(1ull << (dev & 63));
   }
-  MESH_CUDA_OK(launch(wide_kernel<HD, Q8>, dim3(p.shares), THREADS, C::SMEM, stream, p));
+  MESH_CUDA_OK(launch(wide_kernel<HD, Q8>, dim3(grid_of(p)), THREADS, C::SMEM, stream, p));
   if (p.part) {
     const unsigned items = (unsigned)(p.B * p.kv_heads * p.tiles);
     if (p.shares > 8ll * items) MESH_CUDA_OK(launch(wide_join_kernel<HD, true>, dim3(items, HD / 8), GROUPS * TT, 0, stream, p));
@@ -752,6 +793,13 @@ int run(const Args& p, void* stream) {
 }
 
 }  // namespace
+
+int wide_clusters(int head_dim, bool q8, int ranks) {
+#define MESH_CLUSTERS(HD, Q8) clusters_at_once<THREADS, Wide<HD, Q8>::SMEM>(wide_kernel<HD, Q8>, ranks)
+  if (q8) return head_dim == 64 ? MESH_CLUSTERS(64, true) : head_dim == 128 ? MESH_CLUSTERS(128, true) : MESH_CLUSTERS(256, true);
+  return head_dim == 64 ? MESH_CLUSTERS(64, false) : head_dim == 128 ? MESH_CLUSTERS(128, false) : MESH_CLUSTERS(256, false);
+#undef MESH_CLUSTERS
+}
 
 int run_wide(const Args& p, int head_dim, bool q8, void* stream) {
   switch (head_dim * 2 + q8) {

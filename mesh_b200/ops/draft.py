@@ -84,7 +84,8 @@ def draft_attention(q: torch.Tensor, cache: KVCache, pos: torch.Tensor, *, count
     key = (T, qh, window, splits, scale)
     floats = cache._scratch.get(key)
     if floats is None:                           # a function of the sizes alone; also checks the arguments
-        floats = _lib().mesh_draft_attention_scratch(cache._at, _ARGS.pack(*args, 0, cache._status))
+        with torch.cuda.device(cache._index):    # (-1: none) how the work is cut depends on the device
+            floats = _lib().mesh_draft_attention_scratch(cache._at, _ARGS.pack(*args, 0, cache._status))
         if floats < 0:
             raise ValueError(_native.last_error())
         if len(cache._scratch) > 256:            # a scale of every call's own
@@ -92,7 +93,7 @@ def draft_attention(q: torch.Tensor, cache: KVCache, pos: torch.Tensor, *, count
         cache._scratch[key] = floats
     if B == 0 or T == 0:
         return out
-    if floats == 0 or cache._index < 0:
+    if floats == 0 or cache._index < 0:          # one kernel, whose clusters join their shares themselves
         _launch(cache._index, "mesh_draft_attention", 1, cache._at, _ARGS.pack(*args, 0, cache._status))
     else:
         # scratch of the call's own: calls on other streams and other captured graphs share nothing

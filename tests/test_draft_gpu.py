@@ -303,6 +303,48 @@ def test_attention(case, bits, hd):
         assert _same(again[b, :n], out[b, :n]) and not again[b, n:].any()
 
 
+CUTS = [
+    # B, T, G, H, S, positions, counts: short caches, where a cluster has an item and its CTAs join their parts, and more items than SMs
+    (1, 2, 4, 2, 1500, [1400], None),                                 # few items: clusters of 8
+    (3, 1, 4, 8, 2000, [0, 60, 1999], None),                          # 24 items; the first two lie in one CTA
+    (8, 3, 2, 8, 900, [0, 100, 897, 300, 890, 500, 2, 899], [3, 0, 1, 2, 3, 3, 3, 3]),      # 64 items; one sequence has none
+    (16, 1, 2, 8, 400, [25 * i for i in range(16)], None),            # 128 items, a CTA each
+    (40, 1, 1, 8, 300, [7 * i for i in range(40)], None),             # 320 items
+    (2, 40, 4, 1, 900, [850, 3], [40, 10]),                           # tiles of 128 rows; the second sequence has one tile of two
+    (5, 33, 4, 3, 500, [0, 31, 64, 400, 467], [33, 32, 1, 0, 33]),
+    (2, 9, 16, 12, 700, [690, 63], None),                             # 48 items of 128 rows, the last 16 in tiles of their own
+]
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("case", CUTS, ids=str)
+def test_attention_of_short_caches(case, bits, hd):
+    from mesh_b200.ops.draft import draft_attention
+    B, T, G, H, S, positions, counts = case
+    g = _gen(B * T + hd)
+    cache = _cache(B, H, S, hd, bits, g)
+    q = _randn(B, T, G * H, hd, g=g, scale=1.5)
+    pos, counts, visible = _i32(positions), None if counts is None else _i32(counts), _words(B, T, "tree", g)
+    want = _attend64(q, cache, pos, counts, visible, 0, hd ** -0.5)
+    for splits in (0, 148):                                           # shares of all keys, joined by the second kernel
+        _check(draft_attention(q, cache, pos, counts=counts, visible=visible, splits=splits), want, bits, S, hd)
+
+
+@pytest.mark.parametrize("T", [2, 12])
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("positions", [[1500] * 6, [0, 40, 6000, 90, 3, 20990], [1], [700] * 33 + [20990, 8]], ids=["alike", "ragged", "one", "many"])
+def test_attention_in_a_long_cache(positions, bits, T):
+    """Contexts much shorter than the cache: items in equal pieces, or shares that end within items, by the lengths found on the device."""
+    from mesh_b200.ops.draft import draft_attention
+    B, G, H, S, hd = len(positions), 4, 2, 21000, 64
+    g = _gen(B + T)
+    cache = _cache(B, H, S, hd, bits, g)
+    q = _randn(B, T, G * H, hd, g=g, scale=1.5)
+    pos, visible = _i32(positions), _words(B, T, "tree", g)
+    _check(draft_attention(q, cache, pos, visible=visible), _attend64(q, cache, pos, None, visible, 0, hd ** -0.5), bits, S, hd)
+
+
 @pytest.mark.parametrize("bits", [8, 16])
 def test_attention_rows_that_see_nothing(bits):
     from mesh_b200.ops.draft import draft_attention
