@@ -626,8 +626,8 @@ static void cut(const MeshKvCache* c, const MeshDraftAttention* a, Args& p) {
   p.cluster = 0;
   const long long items = (long long)c->B * c->kv_heads * p.tiles, longest = (keys + p.unit - 1) / p.unit;
   if (a->splits > 0 || items > most) return;
-  for (int ranks = MOST_RANKS; ranks >= 1; ranks /= 2) {
-    if (ranks / 2 >= longest || ranks * items > most || (ranks > 1 && clusters(c, w, ranks) < items)) continue;
+  for (int ranks = MOST_RANKS; ranks >= 1; --ranks) {
+    if (ranks > longest || ranks * items > most || (ranks > 1 && clusters(c, w, ranks) < items)) continue;
     if (longest * (1.0 / ranks - 1.0 * items / most) <= (w ? WIDE_LONGER : LONGER)) p.cluster = ranks;
     return;
   }

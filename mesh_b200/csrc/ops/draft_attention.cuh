@@ -288,17 +288,17 @@ static cudaError_t launch(void (*kern)(P...), dim3 grid, int threads, int smem, 
   return cudaLaunchKernelEx(&cfg, kern, a);
 }
 
-// Clusters of 2, 4 or 8 CTAs that the current device runs at the same time, a CTA taking an SM: it depends on how the SMs lie together, which
+// Clusters of `ranks` CTAs that the current device runs at the same time, a CTA taking an SM: it depends on how the SMs lie together, which
 // differs from device to device (sixteen of eight fit into 148 SMs, but not always into their groups).  0 if it cannot be told.
 template <int THREADS, int SMEM, class... P>
 static int clusters_at_once(void (*kern)(P...), int ranks) {
-  static std::atomic<int> known[64][4];                   // one more than it; kernels of the same sizes have the same
+  static std::atomic<int> known[64][MOST_RANKS + 1];                   // one more than it; kernels of the same sizes have the same
   int dev = 0, n = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) {
     cudaGetLastError();
     return 0;
   }
-  std::atomic<int>& k = known[dev & 63][ranks == 8 ? 3 : ranks == 4 ? 2 : 1];
+  std::atomic<int>& k = known[dev & 63][ranks];
   if (k.load()) return k.load() - 1;
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));

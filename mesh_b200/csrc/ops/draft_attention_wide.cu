@@ -679,9 +679,9 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
   cluster_sync_all();
   const Item item = item_of_cluster(a);
   const int n_rows = min(sequence(a, item.b).count * G - item.tile * TT, TT);
-  for (int e = threadIdx.x; e < TT * (HD / 8 / a.cluster); e += THREADS) {
+  for (int e = threadIdx.x; e < TT * ((HD / 8 + a.cluster - 1) / a.cluster); e += THREADS) {
     const int row = e % TT, i = 2 * (e / TT * a.cluster + blockIdx.x % a.cluster), r = item.tile * TT + row;
-    if (row >= n_rows) continue;
+    if (row >= n_rows || i >= HD / 4) continue;
     float m = -CUDART_INF_F, l = 0.f;
     for (int c = 0; c < ranks; ++c) m = fmaxf(m, cluster_load2(smem_u32(ml_s + row), c).x);
     const float ref = m == -CUDART_INF_F ? 0.f : m;
