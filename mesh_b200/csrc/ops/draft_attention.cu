@@ -517,6 +517,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args 
   const int tile = blockIdx.x % a.tiles, hk = blockIdx.x / a.tiles % a.kv_heads, b = blockIdx.x / a.tiles / a.kv_heads;
   // All wait: what comes after this kernel relies on the one before it.  And none looks at the lengths before: they are older than
   // that kernel, but only the wait keeps a read from finding what its line held before them.
+  griddep_launch_dependents();
   griddep_wait();
   if (warp == 0) shares_of_item(a, b, hk, tile, c_s);
   __syncthreads();

@@ -724,6 +724,7 @@ __global__ void __launch_bounds__(GROUPS * TT) wide_join_kernel(const __grid_con
   const int i = SPLIT ? blockIdx.y * 2 : blockIdx.y * 8 + group * 2;       // group of 4 columns
   // All wait: what comes after this kernel relies on the one before it.  And none looks at the lengths before: they are older than
   // that kernel, but only the wait keeps a read from finding what its line held before them.
+  griddep_launch_dependents();
   griddep_wait();
   if (warp == 0) shares_of_item(a, b, hk, tile, c_s);
   __syncthreads();

@@ -287,8 +287,8 @@ class E2BDecoder:
         ``constraints``: arguments of ``ops/logits.py::constrain_logits`` for the ``B * T`` rows of logits.
         After a first call the step may be captured in a CUDA graph.
 
-        Up to 8 rows the logits are fp32 (as in ``decode``), beyond that they come from the bf16 product: equal ones are
-        likelier there, and the lowest id is taken.  One rank: each holds a part of the vocabulary, and the choice among the
+        Up to 8 rows (``B * T``) go through the kernels of ``decode``, with logits in fp32; more through the products of ``prefill``, with
+        logits in bf16: equal ones are likelier there, and the lowest id is taken.  One rank: each holds a part of the vocabulary, and the choice among the
         ranks' best is made for a token per sequence only."""
         c = self.cfg
         if self.world > 1:
@@ -302,19 +302,39 @@ class E2BDecoder:
         positions = (self.pos[:, None] + depth).clamp_(max=c.max_seq - 1).reshape(-1).to(torch.int32)
         x = self.emb[drafts.reshape(-1).long()]
         att = torch.zeros((B, T, qh, hd), dtype=torch.bfloat16, device=self.dev)       # rows behind counts are not written
-        for l, L in enumerate(self.layers):
-            h, _, _ = rmsnorm_fwd(x, L["n1"], c.eps)
-            qkv = self._mm(h, L, "wqkv")
-            rope_(qkv[:, :(qh + kvh) * hd].view(B * T, qh + kvh, hd), positions, self.cos, self.sin)
-            heads = qkv.view(B, T, qh + 2 * kvh, hd)
-            L["cache"].append(heads[:, :, qh:qh + kvh], heads[:, :, qh + kvh:], self.pos, counts)
-            draft_attention(heads[:, :, :qh], L["cache"], self.pos, counts=counts, visible=visible, window=c.window if c.is_local(l) else 0, out=att)
-            x = x + self._mm(att.view(B * T, qh * hd), L, "wo")
-            h, _, _ = rmsnorm_fwd(x, L["n2"], c.eps)
-            a, _ = glu_fwd(h, L["wgu"], act="gelu_tanh", save_gu=False)
-            x = x + self._mm(a, L, "wd")
+
+        def attend(L, l, q, k, v):
+            L["cache"].append(k, v, self.pos, counts)
+            draft_attention(q, L["cache"], self.pos, counts=counts, visible=visible, window=c.window if c.is_local(l) else 0, out=att)
+        few = B * T <= 8                         # rows that the decode step's kernels take at once: each reads its weights a single time
+        if few:
+            x1, q, h = torch.empty_like(x), x.new_empty((B, T, qh, hd)), x.new_empty((B * T, self.Fl))
+            k, v = x.new_empty((2, B, T, kvh, hd))
+            for l, L in enumerate(self.layers):
+                w, s = self._w(L, "wqkv")
+                D.decode_linear(x, w, scales=s, norm_w=L["n1"], eps=c.eps, mode=D.QKV,
+                                qkv=dict(q_heads=qh, kv_heads=kvh, head_dim=hd, pos=positions, cos=self.cos, sin=self.sin, q_out=q, k_cache=k,
+                                         v_cache=v, max_seq=0))
+                attend(L, l, q, k, v)
+                w, s = self._w(L, "wo")
+                D.decode_linear(att.view(B * T, qh * hd), w, scales=s, out=x1, residual=x)
+                w, s = self._w(L, "wgu")
+                D.decode_linear(x1, w, scales=s, norm_w=L["n2"], eps=c.eps, mode=D.GLU, act="gelu_tanh", out=h)
+                w, s = self._w(L, "wd")
+                D.decode_linear(h, w, scales=s, out=x, residual=x1)
+        else:
+            for l, L in enumerate(self.layers):
+                h, _, _ = rmsnorm_fwd(x, L["n1"], c.eps)
+                qkv = self._mm(h, L, "wqkv")
+                rope_(qkv[:, :(qh + kvh) * hd].view(B * T, qh + kvh, hd), positions, self.cos, self.sin)
+                heads = qkv.view(B, T, qh + 2 * kvh, hd)
+                attend(L, l, heads[:, :, :qh], heads[:, :, qh:qh + kvh], heads[:, :, qh + kvh:])
+                x = x + self._mm(att.view(B * T, qh * hd), L, "wo")
+                h, _, _ = rmsnorm_fwd(x, L["n2"], c.eps)
+                a, _ = glu_fwd(h, L["wgu"], act="gelu_tanh", save_gu=False)
+                x = x + self._mm(a, L, "wd")
         codes = dict(w=self.lm_q, scales=self.lm_s) if self.quant in ("w4", "w8") else dict(w=self.lm_head)
-        if B * T <= 8:
+        if few:
             logits = D.decode_linear(x, **codes, norm_w=self.nf, eps=c.eps, out_f32=True)
         else:
             h, _, _ = rmsnorm_fwd(x, self.nf, c.eps)
