@@ -12,10 +12,12 @@
 // Codes are widened once per 128 rows: as operands of a product in 8 bits the queries and probabilities would have to be rounded to 8
 // bits too.  Queries in tensor memory leave shared memory to the rings and its bandwidth to their stores and reads.  The
 // roles are chains of short steps, each a few instructions behind the one before, so there are many warps of few registers; and
-// they run different code on the same SM, so it is kept short.  What was slower, at 64 drafts x 4 heads over four
-// contexts of 20000-32704 keys of 256 in 8 bits: one group of softmax threads, 130 us; tiles held in registers ahead of
-// their turn and everything inlined (112 KB of code, one fetch in six missed the cache), 125; all loader threads at every
-// tile, 117; blocks of 128 keys with the queries in shared memory, 126; scores read twice from tensor memory, 165.
+// they run different code on the same SM, so it is kept short.  The first form, with one group of softmax threads and scores read
+// twice from tensor memory, took 165 us for 64 drafts x 4 heads over four contexts of 20000-32704 keys of 256 in 8 bits; this one takes
+// 136 (29 at the tensor cores' rate).  Slower on the way: tiles held in registers ahead of their turn and everything inlined (112 KB of code,
+// one fetch in six missed the cache); all loader threads at every tile; blocks of 128 keys with the queries in shared memory.
+// What bounds it is the way of a block through the roles, some 4700 clocks for 64 keys of 256, of which the products need 1000: 16 drafts
+// over 8 contexts of 8000-16000 keys of 128 in 8 bits take 121 us, with the softmax left out 92, with the widened codes not stored 112.
 #include "draft_attention.cuh"
 
 namespace mesh {

@@ -226,6 +226,8 @@ class E2BDecoder:
         """prompt int32 [B, T] (same on every rank) -> first generated token [B]; fills the KV caches."""
         c = self.cfg
         B, T = prompt.shape
+        if T > c.max_seq:
+            raise ValueError(f"prefill: a prompt of {T} tokens does not fit into caches of {c.max_seq}")
         hd, d = c.head_dim, c.d_model
         comm = self.ctx.comm if self.world > 1 else None
         x = self.emb[prompt.reshape(-1).long()]                                       # [B*T, d]
@@ -300,7 +302,7 @@ class E2BDecoder:
         hd, qh, kvh = c.head_dim, self.qh, self.kvh
         depth = torch.arange(T, dtype=torch.int32, device=self.dev) if visible is None else tree_depth(visible)
         positions = (self.pos[:, None] + depth).clamp_(max=c.max_seq - 1).reshape(-1).to(torch.int32)
-        x = self.emb[drafts.reshape(-1).long()]
+        x = self.emb[drafts.reshape(-1).long().clamp_(0, c.vocab - 1)]                 # drafts behind counts may be anything
         att = torch.zeros((B, T, qh, hd), dtype=torch.bfloat16, device=self.dev)       # rows behind counts are not written
 
         def attend(L, l, q, k, v):
@@ -363,6 +365,8 @@ class E2BDecoder:
                 if (rows[b][t] if rows is not None else t - 1) == path[-1] and d[b][t] == m[b][path[-1]]:
                     path.append(t)
             new.append([d[b][t] for t in path[1:]] + [m[b][t] for t in path[-1:]])
+            if path and new[b][-1] < 0:
+                raise ValueError(f"accept: sequence {b} may not go on: no token was allowed after its accepted drafts")
             paths.append(path)
         n = max(map(len, paths))
         ints = dict(dtype=torch.int32, device=self.dev)

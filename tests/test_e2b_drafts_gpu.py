@@ -116,6 +116,16 @@ def test_drafts_under_a_grammar_and_a_chain():
     words = torch.zeros((B * n, m.cfg.vocab // 32), dtype=torch.int32, device="cuda")
     words[:, 5] = 1 << 9
     assert (m.draft_step(drafts, constraints=dict(allowed=words)) == 5 * 32 + 9).all()
+    none = m.draft_step(drafts, constraints=dict(allowed=torch.zeros_like(words)))
+    assert (none == -1).all()
+    with pytest.raises(ValueError, match="no token was allowed"):
+        m.accept(drafts, none)
+    assert m.pos.tolist() == [T] * B
+    some = m.draft_step(drafts, counts=torch.tensor([2, 0], dtype=torch.int32, device="cuda"))
+    padded = drafts.clone()
+    padded[0, 2:], padded[1] = -1, 2**31 - 1                        # what lies behind the counts may be anything
+    again = m.draft_step(padded, counts=torch.tensor([2, 0], dtype=torch.int32, device="cuda"))
+    assert torch.equal(some[0, :2], again[0, :2])
     chosen = m.draft_step(drafts)
     drafts[:, 1] = chosen[:, 0]
     new = m.accept(drafts, m.draft_step(drafts))
@@ -144,6 +154,8 @@ def test_captured_step_of_drafts_follows_its_inputs():
 
 def test_refusals():
     from mesh_b200.models.e2b import E2BDecoder
+    with pytest.raises(ValueError, match="does not fit"):
+        _model(1, "bf16", 8, 97)
     with pytest.raises(ValueError, match="cache_bits"):
         E2BDecoder(_small_cfg(), _solo_ctx(), 1, cache_bits=4)
     m, _, _ = _model(1, "bf16", 16, 8)
