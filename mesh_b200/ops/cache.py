@@ -136,7 +136,7 @@ class KVCache:
         if T < 0:
             raise ValueError("read: T must not be negative")
         p, n = _ints(start, "read: start", self.device, (B,)), _ints(counts, "read: counts", self.device, (B,))
-        k = torch.empty((B, T, H, hd), dtype=torch.bfloat16, device=self.device)
+        k = torch.empty(B, T, H, hd, dtype=torch.bfloat16, device=self.device)
         v = torch.empty_like(k)
         if B and T:
             _launch(self._index, "mesh_kv_read", 1, self._at, k.data_ptr(), v.data_ptr(), p, n, T)

@@ -70,7 +70,7 @@ def draft_attention(q: torch.Tensor, cache: KVCache, pos: torch.Tensor, *, count
         raise ValueError(f"draft_attention: {qh} query heads are not a multiple of {H} KV heads")
     if out is None:
         # nodes behind counts are not written: zeros there rather than what the memory held
-        out = (torch.empty if counts is None else torch.zeros)(shape, dtype=bf16, device=dev)
+        out = (torch.empty if counts is None else torch.zeros)(B, T, qh, hd, dtype=bf16, device=dev)
     elif out.shape != shape or out.dtype is not bf16 or out.device != dev:
         raise ValueError("draft_attention: out must be like q")
     qs, os = q.stride(), out.stride()
