@@ -14,10 +14,10 @@
 // roles are chains of short steps, each a few instructions behind the one before, so there are many warps of few registers; and
 // they run different code on the same SM, so it is kept short.  The first form, with one group of softmax threads and scores read
 // twice from tensor memory, took 165 us for 64 drafts x 4 heads over four contexts of 20000-32704 keys of 256 in 8 bits; this one takes
-// 136 (29 at the tensor cores' rate).  Slower on the way: tiles held in registers ahead of their turn and everything inlined (112 KB of code,
+// 125 (29 at the tensor cores' rate).  Slower on the way: tiles held in registers ahead of their turn and everything inlined (112 KB of code,
 // one fetch in six missed the cache); all loader threads at every tile; blocks of 128 keys with the queries in shared memory.
-// What bounds it is the way of a block through the roles, some 4700 clocks for 64 keys of 256, of which the products need 1000: 16 drafts
-// over 8 contexts of 8000-16000 keys of 128 in 8 bits take 121 us, with the softmax left out 92, with the widened codes not stored 112.
+// What bounds it is the way of a block through the roles, some 4300 clocks for 64 keys of 256, of which the products need 1000: of 121
+// us for 16 drafts over 8 contexts of 8000-16000 keys of 128 in 8 bits 92 were left without the softmax, 112 without the widened codes' stores.
 #include "draft_attention.cuh"
 
 namespace mesh {
@@ -41,7 +41,9 @@ struct Wide {
   // 2 STAGES - 1 before: what the warp has not handed over must be younger.
   static constexpr int BEHIND = CPT >= 4 ? 3 : 2;
   static_assert(Q8 || (BEHIND - 1) * LOAD_WARPS <= (2 * STAGES - 2) * CPT, "a loader would wait for what it has not handed over");
-  static constexpr int RAWS = Q8 ? 3 : 0;                   // chunks of codes that a warp has under way
+  // Chunks of codes that a warp has under way: a third would take memory from the first-level cache, which holds what the softmax warps have
+  // no registers for (64 drafts over 20000-32704 keys of 256: 125 us, 136 with three, 134 with two and the memory of three).
+  static constexpr int RAWS = Q8 ? 2 : 0;
   static constexpr int N_BARS = 1 + 4 * STAGES + 3 * NB + 2 + SCALES + RAWS * LOAD_WARPS;
   static constexpr int SCALE_BYTES = Q8 ? SCALES * 3 * KB * 4 : 0;
   static constexpr int SMEM = 2 * STAGES * TILE + RAWS * LOAD_WARPS * CHUNK + SCALE_BYTES + 8 * N_BARS + 64 + 1024;
