@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
       mbar_init(bar(P_FULL + s), GROUP);
       mbar_init(bar(O_DONE + s), 1);
     }
-    for (int s = 0; s < 2; ++s) mbar_init(bar(M_READY + s), TT);
+    for (int s = 0; s < 2; ++s) mbar_init(bar(M_READY + s), GROUP);
     over_s = 0;
     for (int s = 0; s < SCALES; ++s) mbar_init(bar(SC_FULL + s), 1);
     for (int s = 0; s < C::RAWS * LOAD_WARPS; ++s) mbar_init(bar(RAW_FULL + s), 1);
@@ -531,7 +531,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
           top_s[group][n >> 1 & 1][half][row] = top;
         }
         both();                                           // and every score is in registers: P may overwrite them
-        if (!works && half == 0) mbar_arrive(bar(M_READY + group));
+        if (!works) mbar_arrive(bar(M_READY + group));
         if (works) {
           const float top = fmaxf(top_s[group][n >> 1 & 1][0][row], top_s[group][n >> 1 & 1][1][row]);
           float alpha = 1.f, now = -CUDART_INF_F;         // the point that the other group left for the block before
@@ -543,10 +543,10 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
             alpha = ex2(now - (top - LIFT));
             now = top - LIFT;
           }
-          if (half == 0) {
-            m_s[group][row] = now;
-            mbar_arrive(bar(M_READY + group));
-          }
+          if (half == 0) m_s[group][row] = now;
+          // By both halves: the other group may write its next points, and pass its barrier's next phase, only when every thread here has
+          // read the last ones.
+          mbar_arrive(bar(M_READY + group));
           if (m != now) {
             l *= ex2(m - now);                            // nothing summed yet: 0
             m = now;

@@ -331,6 +331,22 @@ def test_attention_of_short_caches(case, bits, hd):
         _check(draft_attention(q, cache, pos, counts=counts, visible=visible, splits=splits), want, bits, S, hd)
 
 
+@pytest.mark.parametrize("bits,hd,T", [(8, 128, 16), (16, 128, 16), (8, 256, 64), (16, 256, 12), (8, 64, 33)])
+def test_attention_of_many_rows_repeats(bits, hd, T):
+    """Many passes over long contexts give the same bits: no group of threads runs ahead of what another has still to read."""
+    from mesh_b200.ops.draft import draft_attention
+    from mesh_b200.utils.status import check_status
+    B, G, H, S = 4, 4, 8, 12000
+    g = _gen(hd + T)
+    cache = _cache(B, H, S, hd, bits, g)
+    q = _randn(B, T, G * H, hd, g=g, scale=3.0)                       # large scores: the reference points move
+    pos, visible = _i32([11000, 6001, 9000, 11900]), _words(B, T, "tree", g)
+    first = draft_attention(q, cache, pos, visible=visible)
+    for _ in range(100):
+        assert _same(draft_attention(q, cache, pos, visible=visible), first)
+    check_status()
+
+
 @pytest.mark.parametrize("T", [2, 12])
 @pytest.mark.parametrize("bits", [8, 16])
 @pytest.mark.parametrize("positions", [[1500] * 6, [0, 40, 6000, 90, 3, 20990], [1], [700] * 33 + [20990, 8]], ids=["alike", "ragged", "one", "many"])
