@@ -33,7 +33,9 @@ constexpr int CHUNK = 4096, PIECES = CHUNK / (32 * 16);     // bytes of stored r
 template <int HD, bool Q8>
 struct Wide {
   static constexpr int TILE = KB * HD * 2;
-  static constexpr int STAGES = HD < 256 ? 4 : Q8 ? 2 : 3;
+  // No more than pays, for the first-level cache's sake: heads of 256 in bf16 with three stages 62.2 us, with two 60.5 (64 drafts of 4
+  // sequences over 6000-12000 keys); of 128 in 8 bits with four 99.2, with three 97.8, in bf16 86.3 and 88.1 (16 drafts of 8).
+  static constexpr int STAGES = HD == 256 ? 2 : HD == 128 && Q8 ? 3 : 4;
   static constexpr int NB = HD < 256 ? 4 : 2;               // blocks whose S is in tensor memory
   static constexpr int RB = Q8 ? HD : 2 * HD, NC = RB / 16;           // bytes and 16-byte pieces of a stored row
   static constexpr int CPT = KB * RB / CHUNK;               // chunks of a tile
@@ -780,6 +782,7 @@ __global__ void __launch_bounds__(GROUPS * TT) wide_join_kernel(const __grid_con
 template <int HD, bool Q8>
 int run(const Args& p, void* stream) {
   using C = Wide<HD, Q8>;
+  static_assert(HD * TT * 4 <= 2 * C::STAGES * C::TILE, "a cluster's part takes the rings' place");
   static_assert(C::SMEM <= 222 * 1024 && C::CPT * CHUNK == KB * C::RB && C::Q_COL + HD / 2 <= 512 && SCALES >= C::STAGES + C::NB, "shared memory of a CTA");
   static std::atomic<unsigned long long> configured{0};   // a bit per device
   int dev = 0;
