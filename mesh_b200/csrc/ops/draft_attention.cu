@@ -596,11 +596,6 @@ constexpr int FEW = 4, WIDE_FEW = 12;
 // (4.4) 26.6 and 25.6.
 constexpr double LONGER = 3, WIDE_LONGER = 4.3;
 
-// The kernel for many rows, with tiles of 128, from three tiles of 16 on: it has a longer start and end, and this one fetches the
-// keys once per tile.  Eight sequences, 8 KV heads of 128 in 8 bits, 4 heads a group, this kernel and the other one: 8 drafts over
-// 500 keys 14 and 21 us, over 12000 keys 100 and 119 us (bf16: 112 and 102); 12 drafts 25 and 22, 142 and 120 us.
-static bool wide(const MeshKvCache* c, const MeshDraftAttention* a) { return a->T * (a->q_heads / c->kv_heads) > 2 * ROWS; }
-
 static int clusters(const MeshKvCache* c, bool w, int ranks) {
   const bool q8 = c->bits == 8;
   if (w) return wide_clusters(c->head_dim, q8, ranks);
@@ -610,28 +605,55 @@ static int clusters(const MeshKvCache* c, bool w, int ranks) {
 #undef MESH_CLUSTERS
 }
 
-static void cut(const MeshKvCache* c, const MeshDraftAttention* a, Args& p) {
-  const bool w = wide(c, a), q8 = c->bits == 8;
-  p.rows = w ? WIDE_ROWS : ROWS;
-  p.unit = w ? WIDE_UNIT
-             : c->head_dim == 64 ? (q8 ? Cfg<64, true>::UNIT : Cfg<64, false>::UNIT)
-             : c->head_dim == 128 ? (q8 ? Cfg<128, true>::UNIT : Cfg<128, false>::UNIT) : (q8 ? Cfg<256, true>::UNIT : Cfg<256, false>::UNIT);
-  p.tiles = (a->T * (a->q_heads / c->kv_heads) + p.rows - 1) / p.rows;
-  // CTAs: one per SM, or per unit of work where the longest sequences have fewer
+static int unit_of(const MeshKvCache* c, bool w) {
+  const bool q8 = c->bits == 8;
+  if (w) return WIDE_UNIT;
+  return c->head_dim == 64 ? (q8 ? Cfg<64, true>::UNIT : Cfg<64, false>::UNIT)
+       : c->head_dim == 128 ? (q8 ? Cfg<128, true>::UNIT : Cfg<128, false>::UNIT) : (q8 ? Cfg<256, true>::UNIT : Cfg<256, false>::UNIT);
+}
+static int tiles_of(const MeshKvCache* c, const MeshDraftAttention* a, bool w) {
+  const int rows = w ? WIDE_ROWS : ROWS;
+  return (a->T * (a->q_heads / c->kv_heads) + rows - 1) / rows;
+}
+// Units of keys that the longest sequence may have.
+static long long longest_of(const MeshKvCache* c, const MeshDraftAttention* a, bool w) {
   long long keys = c->max_seq;
   if (a->window > 0 && (long long)a->window + a->T < keys) keys = (long long)a->window + a->T;
-  const long long units = (long long)c->B * c->kv_heads * p.tiles * ((keys + p.unit - 1) / p.unit);
+  return (keys + unit_of(c, w) - 1) / unit_of(c, w);
+}
+// CTAs of a cluster that has an item; 0: the keys are cut into shares of all.
+static int ranks_of(const MeshKvCache* c, const MeshDraftAttention* a, bool w) {
+  const long long items = (long long)c->B * c->kv_heads * tiles_of(c, a, w), longest = longest_of(c, a, w), most = sm_count();
+  if (a->splits > 0 || items > most) return 0;
+  for (int ranks = MOST_RANKS; ranks >= 1; --ranks) {
+    if (ranks > longest || ranks * items > most || (ranks > 1 && clusters(c, w, ranks) < items)) continue;
+    return longest * (1.0 / ranks - 1.0 * items / most) <= (w ? WIDE_LONGER : LONGER) ? ranks : 0;
+  }
+  return 0;
+}
+
+// The kernel for many rows, with tiles of 128, from three tiles of 16 on: it has a longer start and end, and this one fetches the
+// keys once per tile.  Eight sequences, 8 KV heads of 128 in 8 bits, 4 heads a group, this kernel and the other one: 8 drafts over
+// 500 keys 14 and 21 us, over 12000 keys 100 and 119 us (bf16: 112 and 102); 12 drafts 25 and 22, 142 and 120 us.
+// But where clusters have all tiles of 16 at once and a CTA only a few units, the shorter start counts: 16 drafts of 4 sequences over
+// 500 keys 10.8 and 15.7 us, over 1000 (6 units) 14.6 and 16.7, over 2000 (11) 21.4 and 21.0 (bf16: 14.2 and 14.3, 21.2 and 18.0).
+constexpr int UNITS = 6;
+static bool wide(const MeshKvCache* c, const MeshDraftAttention* a) {
+  if (a->T * (a->q_heads / c->kv_heads) <= 2 * ROWS) return false;
+  return longest_of(c, a, false) > UNITS * ranks_of(c, a, false);
+}
+
+static void cut(const MeshKvCache* c, const MeshDraftAttention* a, Args& p) {
+  const bool w = wide(c, a);
+  p.rows = w ? WIDE_ROWS : ROWS;
+  p.unit = unit_of(c, w);
+  p.tiles = tiles_of(c, a, w);
+  // CTAs: one per SM, or per unit of work where the longest sequences have fewer
+  const long long units = (long long)c->B * c->kv_heads * p.tiles * longest_of(c, a, w);
   const long long most = a->splits > 0 ? a->splits : sm_count();
   p.shares = (int)(units < most ? units : most);
   p.few = a->splits > 0 ? 0 : w ? WIDE_FEW : FEW;
-  p.cluster = 0;
-  const long long items = (long long)c->B * c->kv_heads * p.tiles, longest = (keys + p.unit - 1) / p.unit;
-  if (a->splits > 0 || items > most) return;
-  for (int ranks = MOST_RANKS; ranks >= 1; --ranks) {
-    if (ranks > longest || ranks * items > most || (ranks > 1 && clusters(c, w, ranks) < items)) continue;
-    if (longest * (1.0 / ranks - 1.0 * items / most) <= (w ? WIDE_LONGER : LONGER)) p.cluster = ranks;
-    return;
-  }
+  p.cluster = ranks_of(c, a, w);
 }
 
 static int check(const MeshKvCache* c, const MeshDraftAttention* a) {

@@ -313,6 +313,8 @@ CUTS = [
     (2, 40, 4, 1, 900, [850, 3], [40, 10]),                           # tiles of 128 rows; the second sequence has one tile of two
     (5, 33, 4, 3, 500, [0, 31, 64, 400, 467], [33, 32, 1, 0, 33]),
     (2, 9, 16, 12, 700, [690, 63], None),                             # 48 items of 128 rows, the last 16 in tiles of their own
+    (4, 40, 4, 8, 600, [0, 100, 300, 560], [40, 33, 3, 0]),           # 64 items of 128 rows, some sequences with one tile of two
+    (1, 64, 8, 2, 2500, [2436], None),                                # 8 items of 128 rows
 ]
 
 
