@@ -32,7 +32,7 @@ int mesh_kv_keep(const MeshKvCache* caches, int n, const int* pos, const int* pa
 typedef struct MeshDraftAttention {
   const void* q; void* out; long long q_sb, q_st, o_sb, o_st;
   const int* pos; const int* counts; const long long* visible;
-  int T, q_heads, window, splits;     // splits: CTAs among which all keys are shared out; 0: one per SM
+  int T, q_heads, window, splits;     // splits: CTAs among which all keys are shared out; 0: as it pays
   float scale; float* scratch; void* status;
 } MeshDraftAttention;
 long long mesh_draft_attention_scratch(const MeshKvCache* c, const MeshDraftAttention* a);

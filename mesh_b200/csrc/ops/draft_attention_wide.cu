@@ -1,4 +1,4 @@
-// Attention of drafts with many query rows (more than 16 drafts times heads of a group) on the 5th-generation tensor cores.
+// Attention of drafts with many query rows (which: `wide` in draft_attention.cu) on the 5th-generation tensor cores.
 //
 // A tile is 128 query rows of one (sequence, KV head); a CTA goes through its stretches of 64-key blocks (how the work is cut and
 // the formulas: draft_attention.cuh, draft_attention.cu).  Warps 0-15: softmax, in two groups that take the blocks in turn, in each

@@ -55,7 +55,7 @@ def draft_attention(q: torch.Tensor, cache: KVCache, pos: torch.Tensor, *, count
     :meth:`KVCache.append` has put it.  ``visible [B, T]`` int64: bit j says that the node sees node j (``None``: the ones before it and itself);
     ``counts [B]`` int32: nodes of each sequence (``None``: T); later ones are neither computed nor written.  A node that
     sees nothing gets zeros.  A ``window`` must not be shorter than T.  ``splits``: CTAs among which the keys of all sequences are shared
-    out, in equal shares (0: one per SM).
+    out, in equal shares (0: what pays for these sizes).
 
     Sums of the softmax are fp32; its weights are rounded to fp16 (8-bit rows) or bf16 (bf16 rows) before the second product."""
     B, H, S, hd = cache.k.shape
