@@ -64,6 +64,37 @@ __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatil
   if (!__all_sync(0xffffffffu, ok)) ok = __all_sync(0xffffffffu, wait_on(bar, parity, abort_smem, st, site));
   return ok;
 }
+// Until more than n blocks are over, bounded alike.  For a converged warp, whose lanes leave together: one of them looks for all.
+__device__ __noinline__ bool wait_over(const volatile int* over, int n, volatile int* abort_smem, Status* st) {
+  const unsigned long long t0 = globaltimer_ns();
+  for (uint32_t it = 1;; ++it) {
+    int end = 0;                                            // 1: over, 2: given up
+    if ((threadIdx.x & 31) == 0) {
+      const int now = *over;
+      if (now > n) {
+        end = 1;
+      } else if (*abort_smem) {
+        end = 2;
+      } else if ((it & 0x3fu) == 0) {
+        const bool canceled = status_aborted(st);
+        if (canceled || globaltimer_ns() - t0 > MESH_WAIT_LIMIT_NS) {
+          *abort_smem = 1;
+          status_record(st, canceled ? MESH_CANCELED : MESH_TIMEOUT, SITE_SMEM_EMPTY, n, now, it);
+          end = 2;
+        }
+      }
+    }
+    end = __shfl_sync(0xffffffffu, end, 0);
+    if (end) return end == 1;
+  }
+}
+// A role that gave up: its copies and products under way, each a phase of a barrier, have to be over before the CTA ends.  Bounded too,
+// and whatever the others do.
+__device__ __noinline__ void drain(uint32_t bar, uint32_t parity) {
+  const unsigned long long t0 = globaltimer_ns();
+  while (!mbar_try_wait(bar, parity))
+    if (globaltimer_ns() - t0 > MESH_WAIT_LIMIT_NS) return;
+}
 // 16 bytes, or zeros where `there` is false.
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
@@ -210,17 +241,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
     auto place_free = [&]() {
       const int n = t.n();
       if (n < STAGES) return true;
-      if (n >= 2 * STAGES && over_s <= n - 2 * STAGES) {
-        const unsigned long long t0 = globaltimer_ns();
-        while (over_s <= n - 2 * STAGES) {
-          if (*abort_smem) return false;
-          if (globaltimer_ns() - t0 > MESH_WAIT_LIMIT_NS || status_aborted(a.status)) {
-            *abort_smem = 1;
-            status_record(a.status, MESH_TIMEOUT, SITE_SMEM_EMPTY, n, over_s, 0);
-            return false;
-          }
-        }
-      }
+      if (n >= 2 * STAGES && !__all_sync(0xffffffffu, over_s > n - 2 * STAGES) && !wait_over(&over_s, n - 2 * STAGES, abort_smem, a.status)) return false;
       return wait_warp(bar((t.key ? K_EMPTY : V_EMPTY) + n % STAGES), (n / STAGES - 1) & 1, abort_smem, a.status, SITE_SMEM_EMPTY);
     };
     if (Q8) {
@@ -228,9 +249,10 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
       Tiles ahead;
       Walk ahead_walk = walk;
       const uint32_t own = sRaw + w0 * (RAWS * CHUNK), own_full = bar(RAW_FULL) + 8 * w0 * RAWS;
-      auto fetch = [&](int q, int place) {                // starts the copy of a chunk; what lies behind the last slot is not read
-        if (!ahead.find(a, ahead_walk, q / C::CPT)) return;
-        const int part = q % C::CPT, bytes = min(max(ahead.rows() * C::RB - part * CHUNK, 0), CHUNK);
+      // Starts the copy of a chunk; what lies behind the last slot is not read, and behind the last chunk nothing: a place's phase ends at once.
+      auto fetch = [&](int q, int place) {
+        const bool there = ahead.find(a, ahead_walk, q / C::CPT);
+        const int part = q % C::CPT, bytes = there ? min(max(ahead.rows() * C::RB - part * CHUNK, 0), CHUNK) : 0;
         if (lane == 0) {
           mbar_expect_tx(own_full + 8 * place, bytes);
           if (bytes)
@@ -254,7 +276,6 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
           }
         }
         ok = wait_warp(own_full + 8 * place, phase, abort_smem, a.status, SITE_SMEM_FULL) && place_free();
-        ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         const uint8_t* src = gen + (own - base) + place * CHUNK;
         uint8_t* dst = gen + ((t.key ? sK : sV) + s * C::TILE - base);
@@ -289,6 +310,13 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
           mbar_arrive(bar((t.key ? K_FULL : V_FULL) + s));
         }
         fetch(q + RAWS * LOAD_WARPS, place);
+        if (++place == RAWS) {
+          place = 0;
+          phase ^= 1;
+        }
+      }
+      for (int i = 0; !ok && i < RAWS; ++i) {
+        drain(own_full + 8 * place, phase);
         if (++place == RAWS) {
           place = 0;
           phase ^= 1;
@@ -330,7 +358,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
           const int part = q % C::CPT, s = t.n() % STAGES, rows = t.rows();
           const uint32_t dst = (t.key ? sK : sV) + s * C::TILE;
           const uint8_t* src = (t.key ? a.k : a.v) + (t.at + t.j * KB) * C::RB;
-          ok = __all_sync(0xffffffffu, place_free());
+          ok = place_free();
           if (!ok) break;
 #pragma unroll 4
           for (int i = 0; i < PIECES; ++i) {
@@ -352,6 +380,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
         clean[0] = new_clean;
         of[0] = t.stretch;
       }
+      asm volatile("cp.async.wait_all;" ::: "memory");      // nothing is under way, unless this warp gave up
     }
   } else if (warp == S_WARP) {
     // ------------------------------------------------------------------ S = Q K^T (warp-uniform, one elected lane issues)
@@ -390,6 +419,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
         __syncwarp();
       }
     }
+    if (!ok && n > 0) drain(bar(S_FULL + (n - 1) % NB), (n - 1) / NB & 1);
   } else if (warp == O_WARP) {
     // ------------------------------------------------------------------ O += P V
     constexpr uint32_t idesc = umma_idesc_bf16(TT, HD, 0, 1) & ~FP16;                       // B = V is MN-major
@@ -416,6 +446,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
         __syncwarp();
       }
     }
+    if (!ok && n > 0) drain(bar(O_DONE + (n - 1) % NB), (n - 1) / NB & 1);
   } else if (warp < LOAD_WARP) {
     // ------------------------------------------------------------------ softmax: two threads per query row = TMEM lane
     constexpr float LIFT = Q8 ? 6.f : 0.f;                // with the 2^8 that a reference may lag behind, w stays below 2^14
