@@ -147,6 +147,7 @@ class E2BDecoder:
             torch.cuda.synchronize()
             ctx.rdv.barrier("e2b-slots")
         self.graph = None
+        self.filled = 0                          # no sequence's ``pos`` is above it (unless set by hand)
 
     # ------------------------------------------------------------------ pieces
     def _w(self, L, name):
@@ -266,6 +267,7 @@ class E2BDecoder:
         else:
             D.decode_linear(last, self.lm_head, norm_w=self.nf, eps=c.eps, out=self.logits)
         self.pos.fill_(T - 1)
+        self.filled = T
         D.decode_argmax(self.logits, self.tok, self.pos, vocab_offset=self.rank * self.Vl, rank=self.rank, world=self.world,
                         xchg_ptrs=self.xchg.ptrs() if self.world > 1 else None, step=self.step)
         return self.tok.clone()
@@ -285,7 +287,8 @@ class E2BDecoder:
         """Run a tree of drafts of every sequence through the model at once: ``drafts`` int32 ``[B, T]``, T <= 64, whose first is the
         sequence's last token (``self.tok``), with ``visible`` (``ops/draft.py::tree_visible``; ``None``: a chain) and ``counts``
         (drafts of each sequence; ``None``: T) -> int32 ``[B, T]``, the token that the model chooses after each of them.  Their rows lie in
-        slots ``pos .. pos + T`` of the caches, which must be there, until ``accept`` or the next step; ``pos`` and ``tok`` stay.
+        slots ``pos .. pos + T`` of the caches until ``accept`` or the next step; ``pos`` and ``tok`` stay.  Drafts for which the caches have no
+        slot left are not computed, like those behind ``counts``; -1 is chosen after them.
         ``constraints``: arguments of ``ops/logits.py::constrain_logits`` for the ``B * T`` rows of logits.
         After a first call the step may be captured in a CUDA graph.
 
@@ -300,7 +303,12 @@ class E2BDecoder:
         self.caches()
         B, T = drafts.shape
         hd, qh, kvh = c.head_dim, self.qh, self.kvh
-        depth = torch.arange(T, dtype=torch.int32, device=self.dev) if visible is None else tree_depth(visible)
+        if counts is not None and (counts.dtype != torch.int32 or counts.shape != (B,) or counts.device != self.pos.device):
+            raise ValueError(f"draft_step: counts must be int32 [{B}] on {self.pos.device}, got {counts.dtype} {list(counts.shape)} on {counts.device}")
+        room = c.max_seq - self.pos              # slots that are left
+        counts = room if counts is None else torch.minimum(counts, room)
+        order = torch.arange(T, dtype=torch.int32, device=self.dev)
+        depth = order if visible is None else tree_depth(visible)
         positions = (self.pos[:, None] + depth).clamp_(max=c.max_seq - 1).reshape(-1).to(torch.int32)
         x = self.emb[drafts.reshape(-1).long().clamp_(0, c.vocab - 1)]                 # drafts behind counts may be anything
         att = torch.zeros((B, T, qh, hd), dtype=torch.bfloat16, device=self.dev)       # rows behind counts are not written
@@ -347,21 +355,25 @@ class E2BDecoder:
                 logits = gemm(h, self.lm_head)
         chosen = torch.empty(B * T, dtype=torch.int32, device=self.dev)
         constrain_logits(logits, tokens=chosen, **(constraints or {}))
-        return chosen.view(B, T)
+        return chosen.view(B, T).masked_fill_(order >= room[:, None], -1)
 
     def accept(self, drafts: torch.Tensor, chosen: torch.Tensor, parents=None, counts: torch.Tensor | None = None) -> list[list[int]]:
         """Keep the branch of the last ``draft_step`` that follows the model's own choices: from the root on, a child that is the
         token chosen after its parent (the first of equal ones).  ``parents [B][T]`` as in ``tree_visible`` (``None``: a chain).  Its rows
         move to the front in every layer, ``pos`` moves past them, ``tok`` becomes the token chosen at its end.  Returns
-        each sequence's new tokens: the accepted drafts and that one, at least one."""
+        each sequence's new tokens: the accepted drafts and that one, at least one.  A branch ends with the caches; with ``pos`` at their
+        end the last token has no slot, and the sequence may not go on (with ``counts`` of 0 the others may)."""
         B, T = drafts.shape
         d, m = drafts.tolist(), chosen.tolist()
+        at, tok = torch.stack([self.pos, self.tok]).tolist()
         rows = parents.tolist() if isinstance(parents, torch.Tensor) else parents
         most = counts.tolist() if counts is not None else [T] * B
         paths, new = [], []
         for b in range(B):
+            if most[b] > 0 and at[b] >= self.cfg.max_seq:
+                raise ValueError(f"accept: sequence {b} may not go on: its caches of {self.cfg.max_seq} tokens are full")
             path = [0] if most[b] > 0 else []
-            for t in range(1, min(T, most[b])):
+            for t in range(1, min(T, most[b], self.cfg.max_seq - at[b])):
                 if (rows[b][t] if rows is not None else t - 1) == path[-1] and d[b][t] == m[b][path[-1]]:
                     path.append(t)
             new.append([d[b][t] for t in path[1:]] + [m[b][t] for t in path[-1:]])
@@ -373,10 +385,20 @@ class E2BDecoder:
         kept = torch.tensor([len(p) for p in paths], **ints)
         self.caches().keep(self.pos, torch.tensor([p + [-1] * (n - len(p)) for p in paths], **ints), kept)
         self.pos += kept
-        self.tok.copy_(torch.tensor([t[-1] if t else old for t, old in zip(new, self.tok.tolist())], **ints))
+        self.filled = max(p + len(path) for p, path in zip(at, paths))
+        self.tok.copy_(torch.tensor([t[-1] if t else old for t, old in zip(new, tok)], **ints))
         return new
 
     # ------------------------------------------------------------------ decode
+    def _need(self, steps: int, what: str):
+        """Refuses ``steps`` more tokens where a cache has not that many slots left: a token's row would be the next head's.  ``pos`` is
+        fetched only if the tokens counted here would not fit: it may have been set back by hand."""
+        if self.filled + steps > self.cfg.max_seq:
+            self.filled = int(self.pos.max())
+            if self.filled + steps > self.cfg.max_seq:
+                raise ValueError(f"{what}: {steps} more tokens do not fit into caches of {self.cfg.max_seq}, of which {self.filled} are in use")
+        self.filled += steps
+
     def weight_bytes(self) -> int:
         """Bytes of weights (codes and scales when quantised) one decode step reads on this rank."""
         n = 0
@@ -416,6 +438,7 @@ class E2BDecoder:
             self.stepk, self.graph = st, None
             return saved
         self.stepk = None
+        self._need(1, "capture")
         s = torch.cuda.Stream(device=self.dev)
         s.wait_stream(torch.cuda.current_stream())
         saved = (self.pos.clone(), self.tok.clone(), self.step.clone())
@@ -435,9 +458,10 @@ class E2BDecoder:
         return saved
 
     def decode(self, steps: int, record: bool = True) -> torch.Tensor:
-        """Greedy-decode ``steps`` tokens per sequence by replaying the captured step."""
+        """Greedy-decode ``steps`` tokens per sequence by replaying the captured step.  The caches must have a slot for each."""
         if self.graph is None and getattr(self, "stepk", None) is None:
             raise RuntimeError("call capture() first")
+        self._need(steps, "decode")
         for i in range(steps):
             if self.graph is not None:
                 self.graph.replay()
