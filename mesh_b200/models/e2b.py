@@ -374,7 +374,7 @@ class E2BDecoder:
                 raise ValueError(f"accept: sequence {b} may not go on: its caches of {self.cfg.max_seq} tokens are full")
             path = [0] if most[b] > 0 else []
             for t in range(1, min(T, most[b], self.cfg.max_seq - at[b])):
-                if (rows[b][t] if rows is not None else t - 1) == path[-1] and d[b][t] == m[b][path[-1]]:
+                if (rows[b][t] if rows is not None else t - 1) == path[-1] and d[b][t] == m[b][path[-1]] >= 0:       # -1: no token
                     path.append(t)
             new.append([d[b][t] for t in path[1:]] + [m[b][t] for t in path[-1:]])
             if path and new[b][-1] < 0:

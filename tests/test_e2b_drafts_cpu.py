@@ -67,3 +67,12 @@ def test_decoding_past_the_caches_is_refused():
     m.graph = object()
     with pytest.raises(ValueError, match="do not fit"):
         m.decode(77)
+
+
+def test_a_draft_that_is_no_token_is_not_accepted():
+    """-1 pads a tree and says that no token was allowed: the two are not the same token."""
+    m = _decoder([4])
+    with pytest.raises(ValueError, match="no token was allowed"):
+        m.accept(_i32([[5, -1]]), _i32([[-1, 7]]))
+    assert m.pos.tolist() == [4] and not m._group.calls
+    assert m.accept(_i32([[5, -1, 6]]), _i32([[6, 7, 8]]), [[-1, 0, 0]]) == [[6, 8]]
