@@ -10,14 +10,14 @@
 namespace mesh {
 namespace gemm {
 
-// 2-D map over a row-major bf16 matrix [rows, cols] with leading dimension ld (elements).
+// 2-D map over a row-major bf16 (or fp32) matrix [rows, cols] with leading dimension ld (elements).
 static bool make_map_2d(CUtensorMap* tm, const void* base, uint64_t cols, uint64_t rows, uint64_t ld,
-                        uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle swz) {
+                        uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle swz, bool f32 = false) {
   cuuint64_t dims[2] = {cols, rows};
-  cuuint64_t strides[1] = {ld * 2};
+  cuuint64_t strides[1] = {ld * (f32 ? 4 : 2)};
   cuuint32_t box[2] = {box_cols, box_rows};
   cuuint32_t estr[2] = {1, 1};
-  return encode_tiled(tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box, estr, swz);
+  return encode_tiled(tm, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box, estr, swz);
 }
 
 // 3-D map that makes a row-major [k_rows, mn_cols] matrix look like [mn_cols/64][k_rows][64], so
@@ -131,7 +131,7 @@ extern "C" int mesh_gemm_bf16(const MeshGemmArgs* a, void* stream_v) {
   const int bq = a->b_bits;
   if (bq != 0) {
     if (bq != 4 && bq != 8) return set_error(-3, "gemm: quantised weights are 4-bit or 8-bit (b_bits %d)", bq);
-    if (a->b_mn || a->a_mn || a->epi != EPI_STORE || a->tiles != nullptr || a->ag_src != nullptr)
+    if (a->b_mn || a->a_mn || (a->epi != EPI_STORE && a->epi != EPI_STORE_F32) || a->tiles != nullptr || a->ag_src != nullptr)
       return set_error(-3, "gemm: quantised weights need K-major operands, a plain store epilogue and a dense grid");
     if (a->K % 64) return set_error(-3, "gemm: quantised weights need K %% 64 == 0 (one scale per 64 k)");
     if (a->b_scales == nullptr || (uintptr_t)a->B % 16 || ((bq == 4 ? a->K / 2 : a->K) % 16))
@@ -201,7 +201,12 @@ extern "C" int mesh_gemm_bf16(const MeshGemmArgs* a, void* stream_v) {
   else if (a->b_mn) ok = ok && make_map_mn(&p.tmB, a->B, (uint64_t)a->N, (uint64_t)(a->b_rows ? a->b_rows : a->K), (uint64_t)a->ldb, bn_cta / 64);
   else         ok = ok && make_map_2d(&p.tmB, a->B, (uint64_t)a->K, b_rows, (uint64_t)a->ldb, BK,
                                       a->epi == EPI_GLU_FWD ? BN / 2 : bn_cta, CU_TENSOR_MAP_SWIZZLE_128B);
-  if (a->epi != EPI_SCATTER) {
+  if (a->epi == EPI_STORE_F32) {
+    if (a->a_mn || a->b_mn || ag || a->tiles != nullptr) return set_error(-6, "gemm: an fp32 result needs K-major operands and a dense grid");
+    if (a->ldd % 4 || (uintptr_t)a->D % 16) return set_error(-2, "gemm: fp32 D must be 16-byte aligned with ld %% 4 == 0");
+    ok = ok && make_map_2d(&p.tmD, a->D, (uint64_t)(a->d_cols ? a->d_cols : a->N), (uint64_t)(a->d_rows ? a->d_rows : a->M), (uint64_t)a->ldd, 32, 32,
+                           CU_TENSOR_MAP_SWIZZLE_128B, true);
+  } else if (a->epi != EPI_SCATTER) {
     if (a->ldd % 8 || (uintptr_t)a->D % 16) return set_error(-2, "gemm: D must be 16-byte aligned with ld %% 8 == 0");
     const uint64_t d_cols = (uint64_t)(a->d_cols ? a->d_cols : a->N);
     const uint64_t d_rows = (uint64_t)(a->d_rows ? a->d_rows : a->M);
@@ -233,17 +238,21 @@ extern "C" int mesh_gemm_bf16(const MeshGemmArgs* a, void* stream_v) {
     return launch<AM, BMJ, E, G, 256, false>(p, ctas, stream, dependent);              \
   } while (0)
   if (bq != 0) {
-#define MESH_LAUNCH_Q(Q)                                                               \
+#define MESH_LAUNCH_Q(E, Q)                                                            \
     do {                                                                               \
       if (bn == 128) {                                                                 \
-        if (pair) return launch<0, 0, EPI_STORE, false, 128, true, Q>(p, ctas, stream, dependent);  \
-        return launch<0, 0, EPI_STORE, false, 128, false, Q>(p, ctas, stream, dependent);           \
+        if (pair) return launch<0, 0, E, false, 128, true, Q>(p, ctas, stream, dependent);  \
+        return launch<0, 0, E, false, 128, false, Q>(p, ctas, stream, dependent);           \
       }                                                                                \
-      if (pair) return launch<0, 0, EPI_STORE, false, 256, true, Q>(p, ctas, stream, dependent);    \
-      return launch<0, 0, EPI_STORE, false, 256, false, Q>(p, ctas, stream, dependent);             \
+      if (pair) return launch<0, 0, E, false, 256, true, Q>(p, ctas, stream, dependent);    \
+      return launch<0, 0, E, false, 256, false, Q>(p, ctas, stream, dependent);             \
     } while (0)
-    if (bq == 4) MESH_LAUNCH_Q(4);
-    MESH_LAUNCH_Q(8);
+    if (a->epi == EPI_STORE_F32) {
+      if (bq == 4) MESH_LAUNCH_Q(EPI_STORE_F32, 4);
+      MESH_LAUNCH_Q(EPI_STORE_F32, 8);
+    }
+    if (bq == 4) MESH_LAUNCH_Q(EPI_STORE, 4);
+    MESH_LAUNCH_Q(EPI_STORE, 8);
 #undef MESH_LAUNCH_Q
   }
   switch (a->epi) {
@@ -273,6 +282,8 @@ extern "C" int mesh_gemm_bf16(const MeshGemmArgs* a, void* stream_v) {
       if (a->a_mn) return set_error(-6, "gemm: reduce-scatter fusion needs K-major A");
       if (a->b_mn) MESH_LAUNCH(0, 1, EPI_SCATTER, false);
       MESH_LAUNCH(0, 0, EPI_SCATTER, false);
+    case EPI_STORE_F32:
+      MESH_LAUNCH(0, 0, EPI_STORE_F32, false);
     default:
       return set_error(-7, "gemm: unknown epilogue %d", a->epi);
   }

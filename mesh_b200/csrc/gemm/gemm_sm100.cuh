@@ -55,6 +55,7 @@ enum Epilogue : int {
   EPI_GLU_FWD = 1,      // D = act(g) * u  (+ optional D2 = [g | u])
   EPI_GLU_BWD = 2,      // D = [dg | du] from acc = dAct and aux = [g | u]
   EPI_SCATTER = 3,      // partial tile -> owner rank's receive slot (+ arrival counter)
+  EPI_STORE_F32 = 4,    // D = acc in fp32
 };
 enum Activation : int { ACT_SILU = 0, ACT_GELU_TANH = 1 };
 
@@ -295,7 +296,7 @@ template <int A_MN, int B_MN, int EPI, bool AG, int BN_T, bool PAIR, int BQ = 0>
 __global__ void __launch_bounds__(NUM_THREADS + ((AG || BQ != 0) ? 32 * COMM_WARPS : 0), 1)
 gemm_kernel(const __grid_constant__ Params p) {
   static_assert(!(AG && BQ != 0), "the extra warps push the all-gather or dequantise weights, not both");
-  static_assert(BQ == 0 || (!B_MN && (EPI == EPI_STORE)), "quantised weights: K-major B, plain store epilogue");
+  static_assert(BQ == 0 || (!B_MN && (EPI == EPI_STORE || EPI == EPI_STORE_F32)), "quantised weights: K-major B, plain store epilogue");
   // tile width is a template parameter: 256 or 128; a CTA stages BN (single) or BN/2 (pair) rows of B
   constexpr int BN = BN_T;
   constexpr int CTAS = PAIR ? 2 : 1;
@@ -554,6 +555,25 @@ gemm_kernel(const __grid_constant__ Params p) {
           for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
           uint32_t box = claim_box();
           stage_row(box, lane, v);
+          emit_box(&p.tmD, box, n0 + c * 32, m0 + q * 32);
+        }
+      } else if constexpr (EPI == EPI_STORE_F32) {
+        // logits that a token is chosen from: rounded to bf16, the largest of a large vocabulary would often be several
+        const int n0 = wk.d_col0;
+#pragma unroll 1
+        for (int c = 0; c < BN / 32; ++c) {
+          if (n0 + c * 32 >= p.N || q * 32 >= wk.d_rows) break;
+          uint32_t r[32];
+          tmem_ld_32x32(taddr + c * 32, r);
+          tmem_ld_wait();
+          if (lane == 0) tma_store_wait_read<1>();     // two 4 KiB boxes per warp, used alternately
+          __syncwarp();
+          const uint32_t box = my_staging + buf * 2 * EPI_BOX_BYTES;
+          buf ^= 1;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(box + lane * 128 + ((j ^ (lane & 7)) << 4)), "r"(r[4 * j]),
+                         "r"(r[4 * j + 1]), "r"(r[4 * j + 2]), "r"(r[4 * j + 3]) : "memory");
           emit_box(&p.tmD, box, n0 + c * 32, m0 + q * 32);
         }
       } else if constexpr (EPI == EPI_GLU_FWD) {

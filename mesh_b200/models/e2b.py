@@ -292,8 +292,7 @@ class E2BDecoder:
         ``constraints``: arguments of ``ops/logits.py::constrain_logits`` for the ``B * T`` rows of logits.
         After a first call the step may be captured in a CUDA graph.
 
-        Up to 8 rows (``B * T``) go through the kernels of ``decode``, with logits in fp32; more through the products of ``prefill``, with
-        logits in bf16: equal ones are likelier there, and the lowest id is taken.  One rank: each holds a part of the vocabulary, and the choice among the
+        Up to 8 rows (``B * T``) go through the kernels of ``decode``, more through the products of ``prefill``; the logits are fp32.  One rank: each holds a part of the vocabulary, and the choice among the
         ranks' best is made for a token per sequence only."""
         c = self.cfg
         if self.world > 1:
@@ -350,9 +349,9 @@ class E2BDecoder:
             h, _, _ = rmsnorm_fwd(x, self.nf, c.eps)
             if self.quant in ("w4", "w8"):
                 from ..ops.gemm import gemm_q
-                logits = gemm_q(h, self.lm_q, self.lm_s)
+                logits = gemm_q(h, self.lm_q, self.lm_s, out_f32=True)
             else:
-                logits = gemm(h, self.lm_head)
+                logits = gemm(h, self.lm_head, out_f32=True)
         chosen = torch.empty(B * T, dtype=torch.int32, device=self.dev)
         constrain_logits(logits, tokens=chosen, **(constraints or {}))
         return chosen.view(B, T).masked_fill_(order >= room[:, None], -1)

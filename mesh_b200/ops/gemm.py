@@ -17,7 +17,7 @@ import torch
 from .. import _native
 from ..utils.status import status_block
 
-EPI_STORE, EPI_GLU_FWD, EPI_GLU_BWD, EPI_SCATTER = 0, 1, 2, 3
+EPI_STORE, EPI_GLU_FWD, EPI_GLU_BWD, EPI_SCATTER, EPI_STORE_F32 = 0, 1, 2, 3, 4
 ACT = {"silu": 0, "swiglu": 0, "gelu_tanh": 1, "geglu": 1}
 
 
@@ -54,7 +54,8 @@ class trace:
 
 
 def _label(a: _native.GemmArgs) -> str:
-    epi = {EPI_STORE: "store", EPI_GLU_FWD: "glu_fwd", EPI_GLU_BWD: "glu_bwd", EPI_SCATTER: "reduce_scatter"}[a.epi]
+    epi = {EPI_STORE: "store", EPI_GLU_FWD: "glu_fwd", EPI_GLU_BWD: "glu_bwd", EPI_SCATTER: "reduce_scatter",
+           EPI_STORE_F32: "store_f32"}[a.epi]
     pre = "all_gather+" if a.ag_src else ""
     return f"{pre}gemm[{a.M}x{a.N}x{a.K}{' A^T' if a.a_mn else ''}{' B^T' if a.b_mn else ''}]->{epi}"
 
@@ -148,18 +149,34 @@ def tile_n_for(M: int, N: int) -> int:
     return _native.lib().mesh_gemm_choose_tile_n(M, N, 0)
 
 
-def gemm(a: torch.Tensor, b: torch.Tensor, *, a_mn: bool = False, b_mn: bool = False,
-         out: torch.Tensor | None = None, num_ctas: int = 0, tile_n: int = 0, pair: int = 0, **flow) -> torch.Tensor:
+def _set_f32(g: _native.GemmArgs, a: torch.Tensor, M: int, N: int, out: torch.Tensor | None) -> torch.Tensor:
+    """The accumulators go out as they are, in fp32."""
+    if out is None:
+        out = torch.empty((M, N), dtype=torch.float32, device=a.device)
+    elif out.dtype != torch.float32 or out.shape != (M, N) or out.device != a.device or out.stride(1) != 1:
+        raise ValueError(f"out: expected a row-major fp32 [{M}, {N}] on {a.device}, got {out.dtype} {tuple(out.shape)} {out.stride()} on {out.device}")
+    g.D, g.ldd, g.d_cols, g.epi = out.data_ptr(), out.stride(0), N, EPI_STORE_F32
+    return out
+
+
+def gemm(a: torch.Tensor, b: torch.Tensor, *, a_mn: bool = False, b_mn: bool = False, out: torch.Tensor | None = None,
+         out_f32: bool = False, num_ctas: int = 0, tile_n: int = 0, pair: int = 0, **flow) -> torch.Tensor:
     """``out[M,N] = A[M,K] @ B[N,K]^T`` with fp32 accumulation.
 
-    ``a_mn``: ``a`` is stored ``[K, M]``;  ``b_mn``: ``b`` is stored ``[K, N]``.  ``flow``: see :func:`chain`.
+    ``a_mn``: ``a`` is stored ``[K, M]``;  ``b_mn``: ``b`` is stored ``[K, N]``.  ``out_f32``: the result in fp32 instead of bf16 (neither
+    operand stored transposed).  ``flow``: see :func:`chain`.
     """
     g, M, N, K = _base_args(a, b, a_mn, b_mn)
-    if out is None:
-        out = a.new_empty((M, N))
+    if out_f32:
+        if a_mn or b_mn:
+            raise ValueError("gemm: an fp32 result needs operands that are not stored transposed")
+        out = _set_f32(g, a, M, N, out)
     else:
-        _check2d(out, "out")
-    g.D, g.ldd, g.d_cols = out.data_ptr(), out.stride(0), out.shape[1]
+        if out is None:
+            out = a.new_empty((M, N))
+        else:
+            _check2d(out, "out")
+        g.D, g.ldd, g.d_cols = out.data_ptr(), out.stride(0), out.shape[1]
     g.num_ctas, g.tile_n, g.pair = num_ctas, tile_n, pair      # epi: EPI_STORE is 0
     if flow:
         chain(g, **flow)
@@ -168,9 +185,10 @@ def gemm(a: torch.Tensor, b: torch.Tensor, *, a_mn: bool = False, b_mn: bool = F
 
 
 def gemm_q(a: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, *, out: torch.Tensor | None = None,
-           num_ctas: int = 0, tile_n: int = 0, pair: int = 0) -> torch.Tensor:
+           out_f32: bool = False, num_ctas: int = 0, tile_n: int = 0, pair: int = 0) -> torch.Tensor:
     """``out[M, N] = a[M, K] @ W[N, K]^T`` with ``W`` group-quantised: ``codes`` uint8 ``[N, K/2]`` (4-bit,
-    :func:`mesh_b200.ops.decode.quantize_w4`) or ``[N, K]`` (8-bit, ``quantize_w8``) and ``scales`` fp16 ``[N, K/64]``.
+    :func:`mesh_b200.ops.decode.quantize_w4`) or ``[N, K]`` (8-bit, ``quantize_w8``) and ``scales`` fp16 ``[N, K/64]``.  ``out_f32``: the
+    result in fp32 instead of bf16.
 
     The codes are dequantised in registers by four extra warps of the GEMM kernel and written straight into the
     tensor cores' shared-memory stages: the bf16 matrix never exists in global memory (K13 of the reference's operation
@@ -190,11 +208,14 @@ def gemm_q(a: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, *, out: t
     g.M, g.N, g.K = M, N, K
     g.lda, g.ldb = a.stride(0), K
     g.a_rows, g.b_rows = M, N
-    if out is None:
-        out = torch.empty((M, N), dtype=torch.bfloat16, device=a.device)
-    _check2d(out, "out")
-    g.D, g.ldd, g.d_cols = out.data_ptr(), out.stride(0), out.shape[1]
-    g.epi = EPI_STORE
+    if out_f32:
+        out = _set_f32(g, a, M, N, out)
+    else:
+        if out is None:
+            out = torch.empty((M, N), dtype=torch.bfloat16, device=a.device)
+        _check2d(out, "out")
+        g.D, g.ldd, g.d_cols = out.data_ptr(), out.stride(0), out.shape[1]
+        g.epi = EPI_STORE
     g.status = status_block(a.device).data_ptr()
     g.world = 1
     g.num_ctas, g.tile_n, g.pair = num_ctas, tile_n, pair

@@ -70,3 +70,25 @@ def test_a_decoder_runs_to_the_end_of_its_caches_and_no_further(bits):
     with pytest.raises(ValueError, match="do not fit"):
         m.decode(1)
     check_status()
+
+
+@pytest.mark.parametrize("quant", ["bf16", "w4", "w8"])
+def test_more_than_eight_rows_choose_from_fp32_logits(quant):
+    """Two tokens are raised above all others, the one of the higher id by 2^-11 of its logit more, less than half a step of bf16 (2^-9 to 2^-8): it is
+    chosen in every row."""
+    B, n = 2, 12
+    m, _, g = _model(B, quant, 16, 20)
+    drafts = torch.randint(0, m.cfg.vocab, (B, n), generator=g, dtype=torch.int32).cuda()
+    logits = torch.empty((B * n, m.cfg.vocab), device="cuda")
+    plain = m.draft_step(drafts, constraints=dict(out=logits))
+    assert torch.equal(plain.view(-1).long(), logits.argmax(-1))
+    assert not torch.equal(logits, logits.bfloat16().float())
+    low, high = 7, 300
+    l = logits[:, [low, high]].double()
+    up = 2.0 ** -11 * l.abs().amax(-1)
+    # sums of magnitudes below 256 are off by at most 2^-17 in fp32, and so are the biases
+    assert l.abs().max() + 128 < 256 and up.min() > 4 * 2.0 ** -17
+    bias = torch.stack([128 - l[:, 0], 128 - l[:, 1] + up], 1).float()
+    ids = torch.tensor([[low, high]], dtype=torch.int32, device="cuda").expand(B * n, -1)
+    chosen = m.draft_step(drafts, constraints=dict(bias_ids=ids.contiguous(), bias=bias))
+    assert (chosen == high).all()
