@@ -289,18 +289,61 @@ __global__ void __launch_bounds__(THREADS, 6) constrain_kernel(const __grid_cons
   a.tokens[row] = best == -CUDART_INF_F ? -1 : bi + a.vocab_offset;
 }
 
+// Listed ids that a piece has room for.
+static int entries_of(const MeshLogits* a) {
+  const int listed = a->hist + a->nbias;
+  return listed < PIECE ? (listed + 1) / 2 * 2 : PIECE;
+}
+static int smem_of(int entries) { return entries > 0 ? LISTS + entries * ENTRY : 0; }
+
+template <bool HALF, int CTAS>
+static cudaError_t configure(int dev) {
+  static std::atomic<unsigned long long> configured{0};   // a bit per device
+  if (configured.load() >> (dev & 63) & 1) return cudaSuccess;
+  cudaError_t e = cudaFuncSetAttribute(constrain_kernel<HALF, CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_of(PIECE));
+  if (e == cudaSuccess && CTAS > 8) e = cudaFuncSetAttribute(constrain_kernel<HALF, CTAS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess) configured.fetch_or(1ull << (dev & 63));
+  return e;
+}
+
+// Whether the current device can run a cluster of sixteen with this much shared memory a CTA: it is no size that every device has, and the
+// CTAs need so many SMs of one group with that room.  Asked once for every 16 KB.
+template <bool HALF>
+static bool sixteen_fit(int smem) {
+  constexpr int STEP = 16 * 1024;
+  static std::atomic<int> known[64][(LISTS + PIECE * ENTRY) / STEP + 2];               // 1: no, 2: yes
+  int dev = 0, n = 0;
+  bool ok = cudaGetDevice(&dev) == cudaSuccess;
+  std::atomic<int>& k = known[dev & 63][(smem + STEP - 1) / STEP];
+  if (ok && k.load()) return k.load() == 2;
+  const int most = smem_of(PIECE), asked = (smem + STEP - 1) / STEP * STEP;
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(16);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = asked < most ? asked : most;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 16;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  ok = ok && configure<HALF, 16>(dev) == cudaSuccess && cudaOccupancyMaxActiveClusters(&n, constrain_kernel<HALF, 16>, &cfg) == cudaSuccess;
+  if (!ok) {
+    cudaGetLastError();                                   // eight will do
+    return false;
+  }
+  k.store(n > 0 ? 2 : 1);
+  return n > 0;
+}
+
 template <bool HALF, int CTAS>
 static int run(const MeshLogits* a, void* stream) {
-  static std::atomic<unsigned long long> configured{0};   // a bit per device
   int dev = 0;
   MESH_CUDA_OK(cudaGetDevice(&dev));
-  if (!(configured.load() >> (dev & 63) & 1)) {
-    MESH_CUDA_OK(cudaFuncSetAttribute(constrain_kernel<HALF, CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, LISTS + PIECE * ENTRY));
-    if (CTAS > 8) MESH_CUDA_OK(cudaFuncSetAttribute(constrain_kernel<HALF, CTAS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    configured.fetch_or(1ull << (dev & 63));
-  }
-  const int listed = a->hist + a->nbias, entries = listed < PIECE ? (listed + 1) / 2 * 2 : PIECE;
-  const int smem = entries > 0 ? LISTS + entries * ENTRY : 0;
+  MESH_CUDA_OK((configure<HALF, CTAS>(dev)));
+  const int entries = entries_of(a), smem = smem_of(entries);
   const int vectors = !((uintptr_t)a->logits % 16) && a->ldl % Vec<HALF>::N == 0 && !((uintptr_t)a->out % 16) && a->ldo % Vec<HALF>::N == 0;
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
@@ -333,7 +376,8 @@ extern "C" int mesh_constrain_logits(const MeshLogits* a, void* stream) {
   if (a->nbias > 32767) return set_error(-2, "constrain_logits: at most 32767 biases");
   if (!a->out && !a->tokens) return set_error(-2, "constrain_logits: nothing asked for");
   if (a->rows == 0) return 0;
-  const int ctas = a->vocab <= ONE_CTA_VOCAB ? 1 : a->vocab <= EIGHT_CTA_VOCAB ? 8 : 16;
+  const int smem = smem_of(entries_of(a));
+  const int ctas = a->vocab <= ONE_CTA_VOCAB ? 1 : a->vocab <= EIGHT_CTA_VOCAB || !(a->half ? sixteen_fit<true>(smem) : sixteen_fit<false>(smem)) ? 8 : 16;
 #define MESH_CONSTRAIN(HALF) (ctas == 1 ? run<HALF, 1>(a, stream) : ctas == 8 ? run<HALF, 8>(a, stream) : run<HALF, 16>(a, stream))
   return a->half ? MESH_CONSTRAIN(true) : MESH_CONSTRAIN(false);
 #undef MESH_CONSTRAIN
