@@ -145,7 +145,7 @@ __device__ __forceinline__ uint32_t finite_or_zero(uint32_t w) {
 // Where the tiles of keys and values lie.  Per stretch they come in the order the products take them: K0 K1 V0 K2 V1 ... V(last).
 struct Tiles {                                             // (the walk apart: what a call takes the address of stays in memory)
   Stretch x;
-  int first = 0, blocks = 0, n0 = 0, stretch = -1;        // tiles before this stretch, its blocks, blocks before it
+  int first = 0, blocks = 0, n0 = 0, stretch = -1;        // tiles before this stretch, its blocks, blocks before it, stretches with keys
   long long at = 0;                                       // row of its first slot
   bool key = false;
   int j = 0;                                              // block within the stretch
@@ -158,8 +158,8 @@ struct Tiles {                                             // (the walk apart: w
       Stretch y;
       if (!next_stretch(a, walk, y)) return false;
       x = y;
-      ++stretch;
       blocks = blocks_of(x);
+      stretch += blocks > 0;
       at = ((long long)x.b * a.kv_heads + x.hk) * a.max_seq + x.k_lo;
     }
     o -= first;
@@ -187,7 +187,8 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
                 S_FULL = V_EMPTY + STAGES, P_FULL = S_FULL + NB, O_DONE = P_FULL + NB, M_READY = O_DONE + NB, SC_FULL = M_READY + 2, RAW_FULL = SC_FULL + SCALES;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen + (bars - base) + 8 * C::N_BARS);
   volatile int* abort_smem = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  volatile int* spoilt_s = reinterpret_cast<volatile int*>(tmem_slot + 2);     // [8]: stretch + 1 whose values had to be cleaned; loaders are at most 5 stretches ahead
+  // [8]: stretch + 1 whose values had to be cleaned.  Only stretches with keys count: loaders are at most 5 of them ahead.
+  volatile int* spoilt_s = reinterpret_cast<volatile int*>(tmem_slot + 2);
   __shared__ Walk walk_s;
   __shared__ float top_s[2][2][2][TT];                      // [group][its block & 1][half][row]
   __shared__ float m_s[2][TT], sum_s[4][TT];                // [group][row]: reference points; [group, half][row]
@@ -459,10 +460,10 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
     // Every warp of these passes the same barriers whatever happens: a wait that ran out makes the others run out, it ends no loop.
     for (Stretch y; next_stretch(a, walk, y);) {
       x = y;
-      ++stretch;
       const int blocks = blocks_of(x), r = x.tile * TT + row, t = min(r / G, a.T - 1), h = x.hk * G + r % G;
       const bool real = row < x.n_rows;
       float unit = 1.f;
+      stretch += blocks > 0;
       if (blocks > 0) {                                   // a quarter of a row of Q into its place
         const __nv_bfloat16* src = a.q + x.b * a.q_sb + t * a.q_st + (long long)h * HD + quarter * (HD / 4);
         const bool vec = (reinterpret_cast<uintptr_t>(src) & 15) == 0;
@@ -647,7 +648,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const __grid_constant_
       }
       all();                                              // they have been read
       if (!ok || !works) continue;
-      const bool spoilt = !Q8 && spoilt_s[stretch & 7] == stretch + 1;
+      const bool spoilt = !Q8 && blocks > 0 && spoilt_s[stretch & 7] == stretch + 1;
       const float inv = !x.whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
       __nv_bfloat16* dst = a.out + x.b * a.o_sb + t * a.o_st + (long long)h * HD;
       const bool vec = (reinterpret_cast<uintptr_t>(dst) & 15) == 0;

@@ -226,6 +226,22 @@ def test_many_rows_past_32_bits(bits):
     _check(got, want, bits, 2 * T, hd)
 
 
+def test_a_sequence_without_keys_between_others_with_infinite_values():
+    """Contexts that fill the cache and a window of one: nothing to see.  Eight of them between two sequences whose values are not finite."""
+    from mesh_b200.ops.draft import draft_attention
+    g = _gen(14)
+    B, H, S, hd, G = 9, 1, 128, 64, 40
+    cache = _cache(B, H, S, hd, 16, g)
+    pos = _i32([100] + [S] * 7 + [100])
+    cache.v[0, 0, 100, 7], cache.v[8, 0, 100, 9] = math.inf, -math.inf
+    q = _randn(B, 1, G, hd, g=g)
+    for _ in range(20):
+        got = draft_attention(q, cache, pos, window=1, splits=1)
+        assert not got[1:8].any()
+        for b in (0, 8):                                                  # a node that sees itself alone
+            assert _same(got[b, 0], cache.v[b, 0, 100].expand(G, hd)), b
+
+
 def test_many_rows_on_two_streams_and_in_a_graph():
     """Calls with scratch memory of their own: two streams at once, and a captured call beside eager ones."""
     from mesh_b200.ops.draft import draft_attention
