@@ -74,12 +74,12 @@ def draft_attention(q: torch.Tensor, cache: KVCache, pos: torch.Tensor, *, count
     elif out.shape != shape or out.dtype is not bf16 or out.device != dev:
         raise ValueError("draft_attention: out must be like q")
     qs, os = q.stride(), out.stride()
-    if qs[3] != 1 or os[3] != 1 or qs[2] != hd or os[2] != hd:
+    if qs[3] != 1 or os[3] != 1 or (qh > 1 and (qs[2] != hd or os[2] != hd)):
         raise ValueError("draft_attention: heads of q and out must be dense")
     if visible is not None and (visible.dtype is not torch.int64 or visible.shape != (B, T) or visible.device != dev or not visible.is_contiguous()):
         raise ValueError(f"draft_attention: visible must be a contiguous int64 [{B}, {T}] on {dev}")
     p, n = _ints(pos, "draft_attention: pos", dev, (B,)), _ints(counts, "draft_attention: counts", dev, (B,))
-    args = (q.data_ptr(), out.data_ptr(), qs[0], qs[1], os[0], os[1], p, n, 0 if visible is None else visible.data_ptr(), T, qh, window, splits,
+    args = (q.data_ptr(), out.data_ptr(), qs[0], qs[1], os[0] if B > 1 else 0, os[1] if T > 1 else 0, p, n, 0 if visible is None else visible.data_ptr(), T, qh, window, splits,
             hd ** -0.5 if scale is None else scale)
     key = (T, qh, window, splits, scale)
     floats = cache._scratch.get(key)

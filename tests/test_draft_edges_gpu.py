@@ -267,6 +267,22 @@ def test_many_rows_on_two_streams_and_in_a_graph():
         assert all(_same(x, want[i]) for x in got[i])
 
 
+@pytest.mark.parametrize("T", [1, 40])
+@pytest.mark.parametrize("bits", [8, 16])
+def test_strides_of_dimensions_of_one_do_not_matter(bits, T):
+    from mesh_b200.ops.draft import draft_attention
+    g = _gen(15)
+    B, S, hd = (1, 90, 64) if T == 1 else (2, 90, 64)
+    cache = _cache(B, 1, S, hd, bits, g)
+    pos = _i32([40, 13][:B])
+    room, want = torch.zeros(16384, dtype=BF16, device=DEV), _randn(B, T, 1, hd, g=g)
+    q = room.as_strided((B, T, 1, hd), (7001, 71, 5, 1))
+    q.copy_(want)
+    out = torch.zeros(16384, dtype=BF16, device=DEV).as_strided((B, T, 1, hd), (7001 if B == 1 else 7002, 71 if T == 1 else 72, 5, 1))
+    draft_attention(q, cache, pos, out=out, splits=1)
+    _check(out, _attend64(want, cache, pos, None, None, 0, hd ** -0.5), bits, S, hd)
+
+
 # ------------------------------------------------------------------------------------------------------------ rows of the cache
 @pytest.mark.parametrize("hd,T", [(128, 9001), (64, 17011), (256, 4099)])
 def test_reading_many_rows(hd, T):
