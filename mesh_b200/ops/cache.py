@@ -71,6 +71,12 @@ def _ints(t: torch.Tensor | None, name: str, device: torch.device, shape: tuple)
     return t.data_ptr()
 
 
+def _meet(tensors) -> bool:
+    """Whether two of these contiguous tensors have bytes in common."""
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in tensors if t is not None and t.numel())
+    return any(a[1] > b[0] for a, b in zip(spans, spans[1:]))
+
+
 class KVCache:
     """Handle of one layer's cache: ``k``, ``v`` ``[B, kv_heads, max_seq, head_dim]`` in bf16, or int8 codes with ``k_scale``,
     ``v_scale`` ``[B, kv_heads, max_seq]`` in fp32.  The tensors must keep their addresses while the handle is used."""
@@ -150,7 +156,7 @@ class KVCache:
 
 
 class CacheGroup:
-    """The caches of a model's layers, of one geometry, moved together."""
+    """The caches of a model's layers, of one geometry, moved together: each in memory of its own, keys and values too."""
 
     def __init__(self, caches: list[KVCache]):
         if not caches:
@@ -159,6 +165,8 @@ class CacheGroup:
         for c in caches:
             if c.k.shape != c0.k.shape or c.bits != c0.bits or c.device != c0.device:
                 raise ValueError("CacheGroup: the caches must have one shape, type and device")
+        if _meet([t for c in caches for t in (c.k, c.v, c.k_scale, c.v_scale)]):
+            raise ValueError("CacheGroup: the caches must not share memory: rows moved twice would be wrong ones")
         self.caches, self.device = list(caches), c0.device
         self._arr = (_Cache * len(caches))(*[c._c for c in caches])
         self._at, self._index = ctypes.addressof(self._arr), c0._index

@@ -4,6 +4,7 @@ import torch
 
 from test_draft_cpu import BF16, _cache, _i32
 
+from mesh_b200.ops.cache import CacheGroup, KVCache
 from mesh_b200.ops.draft import draft_attention
 
 
@@ -21,3 +22,21 @@ def test_strides_of_dimensions_of_one_do_not_matter():
         draft_attention(q, two, _i32(3, 4), out=q.clone(memory_format=torch.preserve_format))
     with pytest.raises(ValueError, match="dense"):
         draft_attention(x.as_strided((2, 3, 2, 64), (1000, 200, 100, 1)), two, _i32(3, 4))
+
+
+def test_a_group_moves_every_row_once():
+    """The same cache twice, one tensor for keys and values, scales of two caches in one: their rows would be moved by two CTAs at once."""
+    a, b = _cache(), _cache()
+    CacheGroup([a, b])
+    parts = torch.zeros(3, 2, 2, 32, 64, dtype=torch.int8)
+    scales = torch.zeros(4, 2, 2, 32)
+    CacheGroup([KVCache(parts[0], parts[1], scales[0], scales[1])])                     # neighbours in one tensor
+    for group in ([a, b, a], [a, KVCache(a.k, a.v, a.k_scale, a.v_scale)], [KVCache(parts[0], parts[0], scales[0], scales[1])],
+                  [KVCache(parts[0], parts[1], scales[0], scales[0])], [a, KVCache(b.k, b.v, a.v_scale, b.v_scale)],
+                  [KVCache(parts[0], parts[1], scales[0], scales[1]), KVCache(parts[1], parts[2], scales[2], scales[3])]):
+        with pytest.raises(ValueError, match="share memory"):
+            CacheGroup(group)
+    x = torch.zeros(2 * 2 * 32 * 64 + 64, dtype=BF16)
+    with pytest.raises(ValueError, match="share memory"):
+        CacheGroup([KVCache(x[:-64].view(2, 2, 32, 64), x[64:].view(2, 2, 32, 64))])
+    CacheGroup([_cache(B=0), _cache(B=0)])
