@@ -106,6 +106,7 @@ class KVCache:
                          0 if v_scale is None else v_scale.data_ptr(), B, H, S, hd, self.bits)
         self._at, self._index = ctypes.addressof(self._c), _index(k.device)
         self._status = status_block(k.device).data_ptr() if self._index >= 0 else 0
+        self._shared = _meet((k, v, k_scale, v_scale))
         self._scratch: dict = {}                 # floats of scratch by the sizes of a call (ops/draft.py)
 
     @classmethod
@@ -120,8 +121,8 @@ class KVCache:
 
     def append(self, k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor, counts: torch.Tensor | None = None) -> None:
         """Row ``k[b, t]``, ``v[b, t]`` (``[B, T, kv_heads, head_dim]`` bf16, any strides with a dense last dimension: columns of a fused
-        projection, for instance) goes to slot ``pos[b] + t`` for ``t < counts[b]`` (int32; ``None``: all).  Rows outside the
-        cache are not written."""
+        projection, for instance; not rows of this cache) goes to slot ``pos[b] + t`` for ``t < counts[b]`` (int32; ``None``: all).  Rows
+        outside the cache are not written."""
         B, H, S, hd = self.k.shape
         T = k.shape[1] if k.dim() == 4 else -1
         for x in (k, v):
@@ -131,6 +132,8 @@ class KVCache:
         if ks[3] != 1 or vs[3] != 1:
             raise ValueError("append: the last dimension must be dense")
         p, n = _ints(pos, "append: pos", self.device, (B,)), _ints(counts, "append: counts", self.device, (B,))
+        if self._shared:
+            raise ValueError("append: keys and values of this cache share memory: it can be read, not written")
         if B == 0 or T == 0:
             return
         _launch(self._index, "mesh_kv_append", 1, self._at, k.data_ptr(), v.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], p, n, T)

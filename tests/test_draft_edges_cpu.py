@@ -40,3 +40,15 @@ def test_a_group_moves_every_row_once():
     with pytest.raises(ValueError, match="share memory"):
         CacheGroup([KVCache(x[:-64].view(2, 2, 32, 64), x[64:].view(2, 2, 32, 64))])
     CacheGroup([_cache(B=0), _cache(B=0)])
+
+
+def test_a_cache_of_one_tensor_is_not_written():
+    """Keys and values in the same memory may be attended to and read; appended, one would overwrite the other."""
+    k, s = torch.zeros(2, 2, 32, 64, dtype=torch.int8), torch.zeros(2, 2, 2, 32)
+    x, pos = torch.zeros(2, 3, 2, 64, dtype=BF16), _i32(0, 1)
+    for c in (KVCache(k, k, s[0], s[1]), KVCache(k, k.clone(), s[0], s[0]), KVCache(k.to(BF16), k.to(BF16)[:]), KVCache(*[k.to(BF16)] * 2)):
+        with pytest.raises(ValueError, match="share memory|GPU") as e:
+            c.append(x, x, pos)
+        assert ("share" in str(e.value)) == (c.k.data_ptr() == c.v.data_ptr() or c.bits == 8)
+        with pytest.raises(ValueError, match="GPU"):
+            draft_attention(x, c, pos)
