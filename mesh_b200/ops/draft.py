@@ -45,6 +45,12 @@ def tree_depth(visible: torch.Tensor) -> torch.Tensor:
     return (((visible[..., None] >> bits) & 1).sum(-1).clamp(min=1) - 1).to(torch.int32)
 
 
+def _overlap(strides, B: int, T: int, row: int) -> bool:
+    """Whether rows [b, t] of `row` values may meet."""
+    (s1, n1), (s2, n2) = sorted(((strides[0], B), (strides[1], T)))
+    return (n1 > 1 and s1 < row) or (n2 > 1 and s2 < (n1 - 1) * s1 + row)
+
+
 def draft_attention(q: torch.Tensor, cache: KVCache, pos: torch.Tensor, *, counts: torch.Tensor | None = None,
                     visible: torch.Tensor | None = None, window: int = 0, scale: float | None = None,
                     out: torch.Tensor | None = None, splits: int = 0) -> torch.Tensor:
@@ -54,7 +60,7 @@ def draft_attention(q: torch.Tensor, cache: KVCache, pos: torch.Tensor, *, count
     node's position is ``pos`` plus the bits set in its word, less one); node t lies in slot ``pos[b] + t``, where
     :meth:`KVCache.append` has put it.  ``visible [B, T]`` int64: bit j says that the node sees node j (``None``: the ones before it and itself);
     ``counts [B]`` int32: nodes of each sequence (``None``: T); later ones are neither computed nor written.  A node that
-    sees nothing gets zeros.  A ``window`` must not be shorter than T.  ``splits``: CTAs among which the keys of all sequences are shared
+    sees nothing gets zeros.  ``out`` may be ``q``, but must not meet it otherwise.  A ``window`` must not be shorter than T.  ``splits``: CTAs among which the keys of all sequences are shared
     out, in equal shares (0: what pays for these sizes).
 
     Sums of the softmax are fp32; its weights are rounded to fp16 (8-bit rows) or bf16 (bf16 rows) before the second product."""
@@ -73,6 +79,8 @@ def draft_attention(q: torch.Tensor, cache: KVCache, pos: torch.Tensor, *, count
         out = (torch.empty if counts is None else torch.zeros)(B, T, qh, hd, dtype=bf16, device=dev)
     elif out.shape != shape or out.dtype is not bf16 or out.device != dev:
         raise ValueError("draft_attention: out must be like q")
+    elif _overlap(out.stride(), B, T, qh * hd):
+        raise ValueError("draft_attention: rows of out overlap")
     qs, os = q.stride(), out.stride()
     if qs[3] != 1 or os[3] != 1 or (qh > 1 and (qs[2] != hd or os[2] != hd)):
         raise ValueError("draft_attention: heads of q and out must be dense")

@@ -52,3 +52,19 @@ def test_a_cache_of_one_tensor_is_not_written():
         assert ("share" in str(e.value)) == (c.k.data_ptr() == c.v.data_ptr() or c.bits == 8)
         with pytest.raises(ValueError, match="GPU"):
             draft_attention(x, c, pos)
+
+
+def test_attention_refuses_an_output_whose_rows_overlap():
+    c, pos, row = _cache(), _i32(0, 1), 4 * 64
+    q, x = torch.zeros(2, 3, 4, 64, dtype=BF16), torch.zeros(4096, dtype=BF16)
+    for sb, st in ((0, row), (3 * row, 0), (row, row), (2 * row, row), (row, row - 64), (3 * row - 2, row), (row, 2 * row - 2), (0, 0)):
+        with pytest.raises(ValueError, match="overlap"):
+            draft_attention(q, c, pos, out=x.as_strided(q.shape, (sb, st, 64, 1)))
+    for sb, st in ((3 * row, row), (row, 2 * row), (5 * row, row + 8), (row + 2, 2 * row + 4)):
+        out = x.as_strided(q.shape, (sb, st, 64, 1))
+        with pytest.raises(ValueError, match="GPU"):
+            draft_attention(q, c, pos, out=out)
+        with pytest.raises(ValueError, match="GPU"):
+            draft_attention(out, c, pos, out=out)
+    with pytest.raises(ValueError, match="GPU"):
+        draft_attention(x.as_strided(q.shape, (0, 0, 64, 1)), c, pos)                  # queries may be shared

@@ -283,6 +283,18 @@ def test_strides_of_dimensions_of_one_do_not_matter(bits, T):
     _check(out, _attend64(want, cache, pos, None, None, 0, hd ** -0.5), bits, S, hd)
 
 
+@pytest.mark.parametrize("T,splits", [(3, 0), (3, 5), (40, 0), (40, 7)])
+def test_attention_over_its_own_queries(T, splits):
+    """``out`` may be ``q``; sequences and tokens may lie in either order."""
+    from mesh_b200.ops.draft import draft_attention
+    g = _gen(16)
+    cache = _cache(3, 2, 700, 128, 8, g)
+    q = _randn(T, 3, 8, 128, g=g).transpose(0, 1)
+    pos = _i32([640, 100, 3])
+    want = draft_attention(q.contiguous(), cache, pos, splits=splits)
+    assert draft_attention(q, cache, pos, out=q, splits=splits) is q and _same(q, want)
+
+
 # ------------------------------------------------------------------------------------------------------------ rows of the cache
 @pytest.mark.parametrize("hd,T", [(128, 9001), (64, 17011), (256, 4099)])
 def test_reading_many_rows(hd, T):
