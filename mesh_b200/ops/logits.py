@@ -29,6 +29,18 @@ def _rows2d(t: torch.Tensor, name: str, dtype, device, rows: int, cols: int | No
     return t.data_ptr(), stride[0], shape[1]
 
 
+def _rows_meet(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether rows of two matrices of one shape and type, at other places, may have bytes in common."""
+    R, V = a.shape
+    size, lda, ldb = a.element_size(), a.stride(0), b.stride(0)
+    at, bt = a.data_ptr(), b.data_ptr()
+    if R == 0 or at + ((R - 1) * lda + V) * size <= bt or bt + ((R - 1) * ldb + V) * size <= at:
+        return False
+    if R == 1:
+        return at != bt
+    return lda != ldb or not V * size <= (bt - at) % (lda * size) <= (lda - V) * size       # other columns of a wider matrix do not
+
+
 def _per_row(t: torch.Tensor | None, name: str, device, rows: int) -> int:
     if t is None:
         return 0
@@ -51,7 +63,7 @@ def constrain_logits(logits: torch.Tensor, *, history: torch.Tensor | None = Non
     * ``bias [R, m]`` added at ``bias_ids [R, m]`` (the first ``bias_len[r]``); of an id listed twice the last entry counts;
     * ``allowed [R, ceil(V / 32)]`` int32: -inf where bit ``id % 32`` of word ``id // 32`` is clear (ids of this shard).
 
-    ``out``: where the result goes, in the logits' type (may be ``logits``); ``tokens [R]`` int32: the id of the largest result (not yet
+    ``out``: where the result goes, in the logits' type (may be ``logits``, but must not meet them otherwise); ``tokens [R]`` int32: the id of the largest result (not yet
     rounded to the logits' type), the lowest of equal ones, -1 where nothing is above -inf (NaN is never chosen).  At least one of them; returns
     ``out``, or ``tokens`` without it.  Lists may be shared by rows (``expand``).  With a vocabulary cut over ranks: ``out=logits`` on every
     rank, then ``decode_argmax``."""
@@ -71,6 +83,10 @@ def constrain_logits(logits: torch.Tensor, *, history: torch.Tensor | None = Non
         o, ldo, _ = _rows2d(out, "out", logits.dtype, dev, R, V)
         if R > 1 and ldo < V:
             raise ValueError("constrain_logits: rows of out overlap")
+        if (o != logits.data_ptr() or ldo != ldl) and _rows_meet(logits, out):
+            raise ValueError("constrain_logits: out must be the logits themselves or memory apart from them")
+    if not 0 <= vocab_offset <= 2**31 - 1 - V:
+        raise ValueError(f"constrain_logits: ids {vocab_offset} .. {vocab_offset + V} are not all int32 and positive")
     h, ldh, hist = 0, 0, 0
     if history is not None:
         h, ldh, hist = _rows2d(history, "history", torch.int32, dev, R)

@@ -1,4 +1,6 @@
 """What the operators for drafted tokens take and refuse, beside ``test_draft_cpu``."""
+import random
+
 import pytest
 import torch
 
@@ -68,3 +70,25 @@ def test_attention_refuses_an_output_whose_rows_overlap():
             draft_attention(out, c, pos, out=out)
     with pytest.raises(ValueError, match="GPU"):
         draft_attention(x.as_strided(q.shape, (0, 0, 64, 1)), c, pos)                  # queries may be shared
+
+
+def test_rows_of_two_matrices_that_meet():
+    """Against the addresses themselves; matrices of unequal strides whose spans meet count as meeting."""
+    from mesh_b200.ops.logits import _rows_meet
+    x, rng, both = torch.zeros(400), random.Random(1), set()
+    for _ in range(3000):
+        R, V = rng.randint(0, 4), rng.randint(1, 20)
+        lda, ldb = (rng.randint(V, 60) for _ in range(2))
+        if rng.random() < 0.7:
+            ldb = lda
+        a, b = (x.as_strided((R, V), (ld, 1), rng.randint(0, 100)) for ld in (lda, ldb))
+        if a.data_ptr() == b.data_ptr() and (lda == ldb or R <= 1):
+            continue                                                                    # in place
+        cells = [{(t.data_ptr() + 4 * (r * t.stride(0) + c)) for r in range(R) for c in range(V)} for t in (a, b)]
+        meet = bool(cells[0] & cells[1])
+        got = _rows_meet(a, b)
+        assert got or not meet
+        if R <= 1 or lda == ldb:
+            assert got == meet
+        both.add((got, meet))
+    assert both >= {(True, True), (False, False)}

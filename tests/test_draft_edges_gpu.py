@@ -314,3 +314,27 @@ def test_reading_many_rows(hd, T):
                 there = min(m, S - s)
                 assert _same(got[b, :there], full[b, :, s:s + there].transpose(0, 1).to(BF16))
                 assert not got[b, there:].any()
+
+
+# ------------------------------------------------------------------------------------------------------------ logits
+def test_logits_refuse_an_output_that_meets_them():
+    from mesh_b200.ops.logits import constrain_logits
+    room = torch.randn(4, 300, device=DEV)
+    x = room[:, :128]
+    for out in (room[:, 1:129], room[:, 127:255], room.view(-1)[64:64 + 512].view(4, 128), room.view(-1)[:512].view(4, 128)):
+        with pytest.raises(ValueError, match="apart"):
+            constrain_logits(x, out=out)
+    with pytest.raises(ValueError, match="apart"):
+        constrain_logits(x[:1], out=room[:1, 8:136])
+    was = room.clone()
+    assert _same(constrain_logits(x, out=room[:, 128:256]), was[:, :128]) and _same(constrain_logits(x, out=x), was[:, :128])
+    assert _same(constrain_logits(x[:1], out=x[:1].as_strided((1, 128), (999, 1))), was[:1, :128])
+    assert _same(room[:, :128], was[:, :128]) and _same(room[:, 256:], was[:, 256:])
+    tok = torch.zeros(4, dtype=torch.int32, device=DEV)
+    for offset in (-1, 2**31 - 128, 2**31, 2**40):
+        with pytest.raises(ValueError, match="ids"):
+            constrain_logits(x, tokens=tok, vocab_offset=offset)
+    last = 2**31 - 1 - 128
+    h = torch.full((4, 1), last + 127, dtype=torch.int32, device=DEV)
+    constrain_logits(x, tokens=tok, vocab_offset=last, history=h, presence=torch.full((4,), -100.0, device=DEV))
+    assert tok.tolist() == [last + 127] * 4
