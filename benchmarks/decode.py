@@ -157,6 +157,7 @@ def main():
     ap.add_argument("--impl", default="mesh", choices=["mesh", "baseline"])
     ap.add_argument("--steps", type=int, default=256)
     ap.add_argument("--prompt", type=int, default=512)
+    ap.add_argument("--cache-bits", type=int, default=16, choices=[8, 16], help="mesh arm: bits of the key/value cache")
     ap.add_argument("--explain", action="store_true",
                     help="baseline arm: where a decode step's time goes (kernels of one eager step by device time)")
     a = ap.parse_args()
@@ -164,7 +165,7 @@ def main():
     from mesh_b200.models.e2b import E2BConfig, bench_decode
     cfg = E2BConfig()
     if a.impl == "mesh":
-        rec = bench_decode(ctx, steps=a.steps, prompt_len=a.prompt)
+        rec = bench_decode(ctx, steps=a.steps, prompt_len=a.prompt, cache_bits=a.cache_bits)
         from mesh_b200.utils.status import check_status
         check_status()
     else:
