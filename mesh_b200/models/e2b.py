@@ -14,7 +14,8 @@ replayed: no host round trip between tokens (design/e2b-crossover-2026-09-16.md:
 
 With ``cache_bits=8`` the key/value cache is kept in 8-bit codes (``ops/cache.py``): half of the bytes that a long context costs, and room
 for twice the tokens.  ``draft_step`` runs a tree of drafted tokens through the model at once and ``accept`` keeps the branch
-that the model itself would have taken.
+that follows the model's choices in that step, from fp32 logits as in ``decode``.  Activations are bf16 and summed in another order than
+there, so of two tokens whose logits nearly tie a step of drafts may take the other one.
 """
 from __future__ import annotations
 
@@ -363,8 +364,9 @@ class E2BDecoder:
         each sequence's new tokens: the accepted drafts and that one, at least one.  A branch ends with the caches; with ``pos`` at their
         end the last token has no slot, and the sequence may not go on (with ``counts`` of 0 the others may)."""
         B, T = drafts.shape
-        d, m = drafts.tolist(), chosen.tolist()
-        at, tok = torch.stack([self.pos, self.tok]).tolist()
+        flat = torch.cat([x.reshape(-1).to(self.pos) for x in (self.pos, self.tok, drafts, chosen)]).tolist()        # one trip to the host
+        at, tok = flat[:B], flat[B:2 * B]
+        d, m = ([flat[i + b * T:i + (b + 1) * T] for b in range(B)] for i in (2 * B, (2 + T) * B))
         rows = parents.tolist() if isinstance(parents, torch.Tensor) else parents
         most = counts.tolist() if counts is not None else [T] * B
         paths, new = [], []
