@@ -14,7 +14,7 @@
 // roles are chains of short steps, each a few instructions behind the one before, so there are many warps of few registers; and
 // they run different code on the same SM, so it is kept short.  The first form, with one group of softmax threads and scores read
 // twice from tensor memory, took 165 us for 64 drafts x 4 heads over four contexts of 20000-32704 keys of 256 in 8 bits; this one takes
-// 125 (29 at the tensor cores' rate).  Slower on the way: tiles held in registers ahead of their turn and everything inlined (112 KB of code,
+// 126 (29 at the tensor cores' rate).  Slower on the way: tiles held in registers ahead of their turn and everything inlined (112 KB of code,
 // one fetch in six missed the cache); all loader threads at every tile; blocks of 128 keys with the queries in shared memory.
 // What bounds it is the way of a block through the roles, some 4300 clocks for 64 keys of 256, of which the products need 1000: of 121
 // us for 16 drafts over 8 contexts of 8000-16000 keys of 128 in 8 bits 92 were left without the softmax, 112 without the widened codes' stores.

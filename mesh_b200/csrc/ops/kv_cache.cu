@@ -93,8 +93,8 @@ struct Strides { long long b, t, h; };
 
 // HD / 8 lanes share a row: 16 bytes of the key and 16 of the value each.  Memory bounds it with bf16 rows (4 sequences of 16000, 8 KV
 // heads of 128: 79 us, 6.6 TB/s read and written); with 8-bit ones, 87 us, 4.6 TB/s, the trip of each row's maximum through its lanes
-// and the codes' arithmetic stand between loads and stores (two rows a thread: 83 us, but 2.9 us instead of 2.2 for the
-// single token of a step).
+// and the codes' arithmetic stand between loads and stores.  Two rows a thread take 83 us there and, for the single token of a step,
+// 2.9 instead of 2.2: one row a thread for all sizes (read_kernel has both forms).
 template <int HD, bool Q8, bool ALIGNED>
 __global__ void __launch_bounds__(THREADS) append_kernel(MeshKvCache c, const __nv_bfloat16* k, const __nv_bfloat16* v,
                                                          Strides ks, Strides vs, const int* pos,

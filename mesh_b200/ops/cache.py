@@ -139,8 +139,9 @@ class KVCache:
         _launch(self._index, "mesh_kv_append", 1, self._at, k.data_ptr(), v.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], p, n, T)
 
     def read(self, start: torch.Tensor, T: int, counts: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
-        """Rows ``start[b] .. start[b] + T`` as dense bf16 ``[B, T, kv_heads, head_dim]`` keys and values (what
-        ``ops.attention.flash_attention`` takes); zero behind ``counts[b]`` and outside the cache."""
+        """Rows ``start[b] .. start[b] + T`` as dense bf16 ``[B, T, kv_heads, head_dim]`` keys and values; zero behind ``counts[b]`` and
+        outside the cache.  ``ops.attention.flash_attention`` takes them where all sequences are equally long; it has no lengths, and
+        rows of zeros would take weight."""
         B, H, S, hd = self.k.shape
         if T < 0:
             raise ValueError("read: T must not be negative")

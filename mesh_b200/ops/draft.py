@@ -63,7 +63,8 @@ def draft_attention(q: torch.Tensor, cache: KVCache, pos: torch.Tensor, *, count
     sees nothing gets zeros.  ``out`` may be ``q``, but must not meet it otherwise.  A ``window`` must not be shorter than T.  ``splits``: CTAs among which the keys of all sequences are shared
     out, in equal shares (0: what pays for these sizes).
 
-    Sums of the softmax are fp32; its weights are rounded to fp16 (8-bit rows) or bf16 (bf16 rows) before the second product."""
+    Sums of the softmax are fp32; its weights are rounded to fp16 (8-bit rows) or bf16 (bf16 rows, half a step of the result's own type;
+    ``ops.decode.DecodeAttention`` over the same rows keeps them in fp32) before the second product."""
     B, H, S, hd = cache.k.shape
     dev, bf16 = cache.device, torch.bfloat16
     shape = q.shape
