@@ -364,6 +364,8 @@ class E2BDecoder:
         each sequence's new tokens: the accepted drafts and that one, at least one.  A branch ends with the caches; with ``pos`` at their
         end the last token has no slot, and the sequence may not go on (with ``counts`` of 0 the others may)."""
         B, T = drafts.shape
+        if chosen.shape != drafts.shape:
+            raise ValueError(f"accept: chosen must be what draft_step returned for drafts {list(drafts.shape)}, got {list(chosen.shape)}")
         flat = torch.cat([x.reshape(-1).to(self.pos) for x in (self.pos, self.tok, drafts, chosen)]).tolist()        # one trip to the host
         at, tok = flat[:B], flat[B:2 * B]
         d, m = ([flat[i + b * T:i + (b + 1) * T] for b in range(B)] for i in (2 * B, (2 + T) * B))

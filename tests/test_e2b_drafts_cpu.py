@@ -76,3 +76,12 @@ def test_a_draft_that_is_no_token_is_not_accepted():
         m.accept(_i32([[5, -1]]), _i32([[-1, 7]]))
     assert m.pos.tolist() == [4] and not m._group.calls
     assert m.accept(_i32([[5, -1, 6]]), _i32([[6, 7, 8]]), [[-1, 0, 0]]) == [[6, 8]]
+
+
+def test_choices_of_other_drafts_are_refused():
+    m = _decoder([4, 5])
+    drafts, chosen = _matching(2, 6)
+    for bad in (chosen[:, :5], chosen[:1], chosen.reshape(-1), torch.cat([chosen, chosen])):
+        with pytest.raises(ValueError, match="chosen"):
+            m.accept(drafts, bad)
+    assert m.pos.tolist() == [4, 5] and not m._group.calls
