@@ -338,3 +338,48 @@ def test_logits_refuse_an_output_that_meets_them():
     h = torch.full((4, 1), last + 127, dtype=torch.int32, device=DEV)
     constrain_logits(x, tokens=tok, vocab_offset=last, history=h, presence=torch.full((4,), -100.0, device=DEV))
     assert tok.tolist() == [last + 127] * 4
+
+
+# ------------------------------------------------------------------------------------------------------------ graphs
+_FIRST = """
+import torch
+from mesh_b200.ops.cache import CacheGroup, KVCache
+from mesh_b200.ops.draft import draft_attention
+from mesh_b200.ops.logits import constrain_logits
+def make(seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    r = lambda *s: torch.randn(s, generator=g, device="cuda").bfloat16()
+    return r(2, 40, 8, 128), r(2, 40, 2, 128), r(2, 40, 2, 128), torch.randn((2, 262144), generator=g, device="cuda")
+caches = [KVCache.empty(2, 2, 900, 128), KVCache.empty(2, 2, 20000, 128, bits=16)]
+pos, tok = torch.tensor([700, 30], dtype=torch.int32, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
+path, h = torch.tensor([[0, 3, 2]] * 2, dtype=torch.int32, device="cuda"), torch.arange(5000, dtype=torch.int32, device="cuda")[None].expand(2, -1)
+one = torch.ones(2, device="cuda")
+def step(q, k, v, x):
+    out = []
+    for c in caches:
+        c.append(k, v, pos)
+        out += [draft_attention(q, c, pos), draft_attention(q[:, :2], c, pos), *c.read(pos, 40)]
+        CacheGroup([c]).keep(pos, path)
+    return out + [constrain_logits(x, history=h, presence=one, out=torch.empty_like(x), tokens=tok)]
+x = make(1)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = step(*x)
+for a, b in zip(x, make(2)):
+    a.copy_(b)
+graph.replay()
+kept = [t.clone() for t in got] + [tok.clone()]
+want = step(*make(2)) + [tok]
+assert all(torch.equal(a, b) for a, b in zip(kept, want))
+print("the same")
+"""
+
+
+def test_the_first_calls_of_a_process_are_captured():
+    """Kernels are loaded and configured, and the device is asked what it can run, while a stream is being captured."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    r = subprocess.run([sys.executable, "-c", _FIRST], capture_output=True, text=True, timeout=300, cwd=Path(__file__).resolve().parent.parent)
+    assert r.returncode == 0 and "the same" in r.stdout, r.stderr[-2000:]
