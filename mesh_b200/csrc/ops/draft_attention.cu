@@ -17,9 +17,9 @@
 // in fp32).  w is multiplied by 2^6 first (in m), so it stays below 2^14 and fp16 holds it in full down to 2^-20, in part down to
 // 2^-30, of the largest; its rounding to 11 bits is an eighth of bf16's.  With a bf16 cache queries and values are bf16 as they are
 // and w is rounded to bf16, half a step of the result's own type: over a window of 512 keys results are off by 0.0022 (root of the mean
-// square, relative), and by 0.0017, their own rounding, with weights in fp32 (as the decode step's attention has them).  A second product with what the
-// rounding leaves makes up for that, but takes 1 to 10 % more time (33 drafts of heads of 64 11.6 us instead of 10.8, the window 16.1 instead of
-// 15.4, 16 drafts in the other kernel 96 instead of 87), and turns an infinite value that is seen into a NaN.
+// square, relative), and by 0.0017, their own rounding, with weights in fp32 (as the decode step's attention has them).  A second product
+// with what the rounding leaves makes up for that, but takes 1 to 10 % more time (33 drafts of heads of 64 11.6 us instead of 10.8, the
+// window 16.1 instead of 15.4, 16 drafts in the other kernel 96 instead of 87), and turns an infinite value that is seen into a NaN.
 //
 // Measured: 16 sequences of 4000 to 32767 keys, 8 KV heads of 128 in 8 bits, 4 query heads each, one token: 142 us, 4.4 TB/s of keys
 // and values.  What bounds it is the issue of instructions (2.4 a clock and SM), 525 of a warp for a block of 16 keys: some 176 widen
@@ -639,8 +639,9 @@ static int ranks_of(const MeshKvCache* c, const MeshDraftAttention* a, bool w) {
 // keys once per tile.  Eight sequences in caches half to wholly filled, 8 KV heads of 128 in 8 bits, 4 heads a group, this kernel and the
 // other one: 8 drafts in caches of 2000 keys 21.8 and 29.7 us, of 6000 55.8 and 60.2, of 16000 100 and 119; 12 drafts in full ones of 500 keys 24.7
 // and 17.0, of 12000 136 and 121.  With bf16 rows two full tiles are where they meet: 8 drafts in caches of 2000 keys 21.3 and 26.5 us, of 6000
-// 55.3 and 53.7, of 12000 93.8 and 83.8 (heads of 256: 18.8 and 21.8, 39.5 and 38.5, 57.2 and 55.5; 5 drafts of 12000 keys of 128, 65.8 and 82.4).  The host knows how long a cache
-// is, not how full, so the kernel that wins in all shorter contexts has them too.
+// 55.3 and 53.7, of 12000 93.8 and 83.8 (heads of 256: 18.8 and 21.8, 39.5 and 38.5, 57.2 and 55.5); 5 drafts, of which some sequences have one
+// tile, in caches of 12000 keys of 128 65.8 and 82.4.  The host knows how long a cache is, not how full: the kernel that wins in all
+// shorter contexts has them too.
 // But where clusters have all tiles of 16 at once and a CTA only a few units, the shorter start counts: 16 drafts of 4 sequences over
 // 500 keys 10.8 and 15.7 us, over 1000 (6 units) 14.6 and 16.7, over 2000 (11) 21.4 and 21.0 (bf16: 14.2 and 14.3, 21.2 and 18.0).
 constexpr int UNITS = 6;

@@ -293,8 +293,8 @@ class E2BDecoder:
         ``constraints``: arguments of ``ops/logits.py::constrain_logits`` for the ``B * T`` rows of logits.
         After a first call the step may be captured in a CUDA graph.
 
-        Up to 8 rows (``B * T``) go through the kernels of ``decode``, more through the products of ``prefill``; the logits are fp32.  One rank: each holds a part of the vocabulary, and the choice among the
-        ranks' best is made for a token per sequence only."""
+        Up to 8 rows (``B * T``) go through the kernels of ``decode``, more through the products of ``prefill``; the logits are fp32.  One
+        rank: each holds a part of the vocabulary, and the choice among the ranks' best is made for a token per sequence only."""
         c = self.cfg
         if self.world > 1:
             raise ValueError("draft_step: one rank only")

@@ -60,8 +60,8 @@ def draft_attention(q: torch.Tensor, cache: KVCache, pos: torch.Tensor, *, count
     node's position is ``pos`` plus the bits set in its word, less one); node t lies in slot ``pos[b] + t``, where
     :meth:`KVCache.append` has put it.  ``visible [B, T]`` int64: bit j says that the node sees node j (``None``: the ones before it and itself);
     ``counts [B]`` int32: nodes of each sequence (``None``: T); later ones are neither computed nor written.  A node that
-    sees nothing gets zeros.  ``out`` may be ``q``, but must not meet it otherwise.  A ``window`` must not be shorter than T.  ``splits``: CTAs among which the keys of all sequences are shared
-    out, in equal shares (0: what pays for these sizes).
+    sees nothing gets zeros.  ``out`` may be ``q``, but must not meet it otherwise.  A ``window`` must not be shorter than T.
+    ``splits``: CTAs among which the keys of all sequences are shared out, in equal shares (0: what pays for these sizes).
 
     Sums of the softmax are fp32; its weights are rounded to fp16 (8-bit rows) or bf16 (bf16 rows, half a step of the result's own type;
     ``ops.decode.DecodeAttention`` over the same rows keeps them in fp32) before the second product."""

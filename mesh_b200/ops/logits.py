@@ -63,10 +63,10 @@ def constrain_logits(logits: torch.Tensor, *, history: torch.Tensor | None = Non
     * ``bias [R, m]`` added at ``bias_ids [R, m]`` (the first ``bias_len[r]``); of an id listed twice the last entry counts;
     * ``allowed [R, ceil(V / 32)]`` int32: -inf where bit ``id % 32`` of word ``id // 32`` is clear (ids of this shard).
 
-    ``out``: where the result goes, in the logits' type (may be ``logits``, but must not meet them otherwise); ``tokens [R]`` int32: the id of the largest result (not yet
-    rounded to the logits' type), the lowest of equal ones, -1 where nothing is above -inf (NaN is never chosen).  At least one of them; returns
-    ``out``, or ``tokens`` without it.  Lists may be shared by rows (``expand``).  With a vocabulary cut over ranks: ``out=logits`` on every
-    rank, then ``decode_argmax``."""
+    ``out``: where the result goes, in the logits' type (may be ``logits``, but must not meet them otherwise); ``tokens [R]`` int32: the
+    id of the largest result (not yet rounded to the logits' type), the lowest of equal ones, -1 where nothing is above -inf (NaN is never
+    chosen).  At least one of them; returns ``out``, or ``tokens`` without it.  Lists may be shared by rows (``expand``).  With a vocabulary
+    cut over ranks: ``out=logits`` on every rank, then ``decode_argmax``."""
     if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16) or not logits.is_cuda:
         raise ValueError(f"constrain_logits: logits must be fp32 or bf16 [R, V] on a GPU, got {logits.dtype} {list(logits.shape)} on {logits.device}")
     R, V = logits.shape
