@@ -285,8 +285,8 @@ class E2BDecoder:
 
     def draft_step(self, drafts: torch.Tensor, visible: torch.Tensor | None = None, counts: torch.Tensor | None = None,
                    constraints: dict | None = None) -> torch.Tensor:
-        """Run a tree of drafts of every sequence through the model at once: ``drafts`` int32 ``[B, T]``, T <= 64, whose first is the
-        sequence's last token (``self.tok``), with ``visible`` (``ops/draft.py::tree_visible``; ``None``: a chain) and ``counts``
+        """Run a tree of drafts of every sequence through the model at once: ``drafts`` int32 ``[B, T]``, T <= 64 (and no more than the
+        window), whose first is the sequence's last token (``self.tok``), with ``visible`` (``ops/draft.py::tree_visible``; ``None``: a chain) and ``counts``
         (drafts of each sequence; ``None``: T) -> int32 ``[B, T]``, the token that the model chooses after each of them.  Their rows lie in
         slots ``pos .. pos + T`` of the caches until ``accept`` or the next step; ``pos`` and ``tok`` stay.  Drafts for which the caches have no
         slot left are not computed, like those behind ``counts``; -1 is chosen after them.
@@ -303,6 +303,8 @@ class E2BDecoder:
         self.caches()
         B, T = drafts.shape
         hd, qh, kvh = c.head_dim, self.qh, self.kvh
+        if drafts.shape[1] > c.window and any(map(c.is_local, range(c.layers))):
+            raise ValueError(f"draft_step: {drafts.shape[1]} drafts are more than the window of {c.window}")
         if counts is not None and (counts.dtype != torch.int32 or counts.shape != (B,) or counts.device != self.pos.device):
             raise ValueError(f"draft_step: counts must be int32 [{B}] on {self.pos.device}, got {counts.dtype} {list(counts.shape)} on {counts.device}")
         room = c.max_seq - self.pos              # slots that are left

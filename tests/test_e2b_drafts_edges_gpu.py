@@ -92,3 +92,12 @@ def test_more_than_eight_rows_choose_from_fp32_logits(quant):
     ids = torch.tensor([[low, high]], dtype=torch.int32, device="cuda").expand(B * n, -1)
     chosen = m.draft_step(drafts, constraints=dict(bias_ids=ids.contiguous(), bias=bias))
     assert (chosen == high).all()
+
+
+def test_more_drafts_than_the_window_are_refused_before_a_row_is_written():
+    m, _, g = _model(1, "bf16", 8, 20)
+    rows = [L["cache"].k.clone() for L in m.layers]
+    with pytest.raises(ValueError, match="window of 16"):
+        m.draft_step(torch.zeros((1, 17), dtype=torch.int32, device="cuda"))
+    assert all(torch.equal(L["cache"].k, was) for L, was in zip(m.layers, rows))
+    m.draft_step(torch.zeros((1, 16), dtype=torch.int32, device="cuda"))
